@@ -335,6 +335,73 @@ int pts_kv_compact(void* kv_pool, int num_layers, int max_pages, int page_len, i
                    int batch, int max_accepted, int32_t* new_kv_len, int32_t* new_last_page_len,
                    pts_stream_t stream);
 
+/* --------------------------------------------------- sequences that share pages
+ * Page state kept on the device, for caches whose sequences share pages (several
+ * samples of one prompt, beams, requests under one system prompt):
+ *   page_refs  int32 [max_pages]            table entries that hold a page (0: free)
+ *   page_table int32 [num_rows, table_width] each sequence's pages in order, -1 past
+ *                                           its end; table_stride elements per row
+ *   kv_lens    int32 [num_rows]             tokens of each sequence
+ * A sequence of n tokens holds ceil(n / page_len) pages; fresh pages are the lowest
+ * free ones, as KvCachePool.allocate hands them out (flashinfer/cache_manager.py:
+ * 89-97).  The reference counts the pages of one beam search on the host
+ * (beam_search.py:415-616) and shares none between requests.
+ *
+ * The calls write an int32 status: 0, or a sum of
+ *   1 a row outside the table or a negative count   2 a row listed twice
+ *   4 a sequence longer than the table is wide       8 not enough free pages
+ * pts_cache_fork and pts_cache_extend change nothing when it is not 0.  At most
+ * 2^17 rows, 2^20 pages, 1024 forks and 4096 extended rows a call.  Calls on the
+ * same state belong on one stream.
+ *
+ * pts_cache_fork: page_table[dst_rows[i]] = page_table[src_rows[i]] as it was before
+ * the call, for every i at once (a row may be a source and a destination, as in a
+ * beam reorder; no row is a destination twice), with the lengths and the pages'
+ * counts; the destinations' former pages lose a holder.  No K/V moves. */
+int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
+                   int table_width, int max_pages, const int32_t* src_rows, const int32_t* dst_rows, int num_forks,
+                   int32_t* status, pts_stream_t stream);
+
+/* Make room for add_each[i] (or, where it is NULL, `add`) more tokens in every listed
+ * row: a partial last page that other sequences hold too is copied first (its filled
+ * slots, every layer, K and V; when every holder of the page is listed, the last of
+ * them keeps it), then fresh pages follow.  kv_pool [num_layers, max_pages, 2,
+ * page_len, row_bytes], row_bytes a multiple of 16.  Also writes the batch that the
+ * append and attention calls take, in the order of `rows`: page_indptr [batch + 1],
+ * page_indices (page_indices_size >= batch * table_width entries; those past
+ * page_indptr[batch] are left as they are), last_page_len [batch], seq_lens [batch]
+ * (with the added tokens).  With shared_pages [num_groups] and group_indptr
+ * [num_groups + 1] (listed rows group_indptr[g] .. group_indptr[g + 1] are group g,
+ * all rows in order): the number of leading pages, full before the call, that all
+ * rows of the group hold alike, for pts_tree_attn_run_shared.  workspace:
+ * pts_cache_workspace_size(max_pages, batch) bytes, any contents. */
+size_t pts_cache_workspace_size(int max_pages, int batch);
+int pts_cache_extend(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
+                     int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
+                     int table_width, const int32_t* rows, const int32_t* add_each, int add, int batch,
+                     const int32_t* group_indptr, int num_groups, int32_t* page_indptr, int32_t* page_indices,
+                     int64_t page_indices_size, int32_t* last_page_len, int32_t* seq_lens, int32_t* shared_pages,
+                     int32_t* status, void* workspace, size_t workspace_bytes, pts_stream_t stream);
+
+/* kv_lens[rows[i]] = min(kv_lens[rows[i]], new_lens[i]) (NULL or negative: 0); the
+ * pages past the new length lose this holder and their entries become -1.  A row
+ * listed twice ends at the smaller length; rows outside the table are skipped
+ * (status 1). */
+int pts_cache_truncate(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
+                       int table_width, int max_pages, int page_len, const int32_t* rows, const int32_t* new_lens,
+                       int num, int32_t* status, pts_stream_t stream);
+
+/* Close the pool's gaps: with n live pages (page_refs > 0), the k-th live page at or
+ * past n moves, in every layer, to the k-th free page below n; the other pages stay.
+ * Writes the new counts, the new table [num_rows, table_width] (contiguous), the map
+ * [max_pages] from old to new page (-1: free) and out_counts = {live, moved}.  The
+ * outputs must not overlap the inputs.  workspace: pts_cache_workspace_size(max_pages,
+ * 0) bytes, any contents. */
+int pts_cache_compact(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
+                      const int32_t* page_refs, const int32_t* page_table, int64_t table_stride, int num_rows,
+                      int table_width, int32_t* out_refs, int32_t* out_table, int32_t* out_map, int32_t* out_counts,
+                      void* workspace, size_t workspace_bytes, pts_stream_t stream);
+
 /* ------------------------------------------------------------------ attention
  * Ancestor bitmask of every tree row: bit j of row i's mask_words-word mask is
  * set when node j of the same request is i itself or one of its ancestors.

@@ -75,6 +75,13 @@ SIGNATURES = {
                                 C.c_int, vp]),
     "pts_kv_compact": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_int,
                                  vp, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp]),
+    "pts_cache_workspace_size": (sz, [C.c_int, C.c_int]),
+    "pts_cache_fork": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
+    "pts_cache_extend": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, i64, vp, C.c_int, C.c_int, vp, vp, C.c_int,
+                                   C.c_int, vp, C.c_int, vp, vp, i64, vp, vp, vp, vp, vp, sz, vp]),
+    "pts_cache_truncate": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
+    "pts_cache_compact": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, i64, C.c_int, C.c_int, vp, vp, vp, vp, vp,
+                                    sz, vp]),
     "pts_tree_mask_from_parents": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, vp]),
     "pts_tree_prepare": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp]),
     "pts_kv_append_rope": (C.c_int, [vp, i64, vp, C.c_int, vp, vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp,

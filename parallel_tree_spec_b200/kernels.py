@@ -7,10 +7,11 @@ raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import os
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -743,3 +744,198 @@ def kv_copy_pages(cache_data: torch.Tensor, src_pages: torch.Tensor, dst_pages: 
         raise ValueError("src_pages and dst_pages differ in length")
     _lib.call("pts_kv_copy_pages", cache_data.data_ptr(), L, P, page_len, H * D * cache_data.element_size(),
               src.data_ptr(), dst.data_ptr(), src.numel(), int(tokens), _stream(dev))
+
+
+# ------------------------------------------------- sequences that share pages
+class CacheBatch(NamedTuple):
+    """What ``cache_extend`` writes for its rows, in their order: the page lists
+    that the append and attention calls take, the lengths with the added tokens,
+    each group's common leading pages (None without groups), and the status."""
+    page_indptr: torch.Tensor
+    page_indices: torch.Tensor
+    last_page_len: torch.Tensor
+    seq_lens: torch.Tensor
+    shared_pages: Optional[torch.Tensor]
+    status: torch.Tensor
+
+
+class CompactedCache(NamedTuple):
+    """What ``cache_compact`` returns: the new page counts and table, the map from
+    old to new page (-1: free), and counts = (live pages, moved pages)."""
+    page_refs: torch.Tensor
+    page_table: torch.Tensor
+    page_map: torch.Tensor
+    counts: torch.Tensor
+
+
+CACHE_STATUS = {1: "a row outside the table or a negative count", 2: "a row listed twice",
+                4: "a sequence longer than the page table is wide", 8: "not enough free pages"}
+
+
+def check_cache_status(status: torch.Tensor) -> None:
+    """Raise for a status of the cache calls (reads it from the device): IndexError
+    for a row outside the table, ValueError for a row listed twice, RuntimeError when
+    the table is too narrow or the pool too small."""
+    code = int(status.item())
+    if code == 0:
+        return
+    msg = "; ".join(text for bit, text in CACHE_STATUS.items() if code & bit) or f"status {code}"
+    raise (IndexError if code & 1 else ValueError if code & 2 else RuntimeError)(msg)
+
+
+def _on(dev: torch.device):
+    """The launches' device as the current one (a no-op context where it is already)."""
+    if dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _cache_ints(name: str, t: torch.Tensor, dev: torch.device, size: Optional[int] = None) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+    if t.device != dev:
+        raise ValueError("all tensors must be on the same device")
+    if size is not None and t.numel() != size:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {size}")
+    return t
+
+
+def _page_state(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: Optional[torch.Tensor]):
+    dev = page_refs.device
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on a CUDA device (this path has no CPU implementation)")
+    _cache_ints("page_refs", page_refs, dev)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or \
+            page_table.stride(0) < page_table.shape[1]:
+        raise ValueError("page_table must be a 2-D int32 tensor with contiguous rows")
+    if page_table.device != dev:
+        raise ValueError("all tensors must be on the same device")
+    if kv_lens is not None:
+        _cache_ints("kv_lens", kv_lens, dev, page_table.shape[0])
+    return dev
+
+
+def _page_pool(pool: torch.Tensor, page_refs: torch.Tensor):
+    if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous [L, max_pages, 2, page_len, Hkv, D] tensor")
+    if pool.device != page_refs.device:
+        raise ValueError("all tensors must be on the same device")
+    if pool.shape[1] != page_refs.numel():
+        raise ValueError("page_refs needs one count per page of the pool")
+    L, P, _, pl, H, D = pool.shape
+    return L, P, pl, H * D * pool.element_size()
+
+
+def _status_word(status: Optional[torch.Tensor], dev: torch.device) -> torch.Tensor:
+    if status is None:
+        return torch.empty(1, dtype=torch.int32, device=dev)
+    return _cache_ints("status", status, dev, 1)
+
+
+def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, src_rows: torch.Tensor,
+               dst_rows: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Make sequence ``dst_rows[i]`` a fork of ``src_rows[i]``: it holds the same
+    pages and length, and its former pages lose a holder.  All rows are read before
+    any is written, so a beam reorder may name a row as source and destination; no
+    row is a destination twice.  No K/V moves: ``cache_extend`` copies a shared
+    partial page when one of its holders grows.  ``page_refs`` [P], ``page_table``
+    [R, W] (-1 past a sequence's end) and ``kv_lens`` [R] are int32 and updated in
+    place.  Returns the status word (``check_cache_status``)."""
+    dev = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("src_rows", src_rows, dev).numel()
+    _cache_ints("dst_rows", dst_rows, dev, n)
+    status = _status_word(status, dev)
+    if n == 0:
+        return status.zero_()
+    with _on(dev):
+        _lib.call("pts_cache_fork", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+                  kv_lens.data_ptr(), page_table.shape[0], page_table.shape[1], page_refs.numel(), src_rows.data_ptr(),
+                  dst_rows.data_ptr(), n, status.data_ptr(), _stream(dev))
+    return status
+
+
+def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                 rows: torch.Tensor, add: Union[int, torch.Tensor], group_indptr: Optional[torch.Tensor] = None,
+                 out=None, status: Optional[torch.Tensor] = None) -> CacheBatch:
+    """Make room for ``add`` more tokens (an int, or int32 [B]) in every listed
+    sequence: a partial last page that others hold too is copied, then the lowest free
+    pages follow.  Returns the batch of those rows; with ``group_indptr`` [G + 1]
+    (int32, over the listed rows) also each group's common leading pages, for
+    ``tree_attention_shared``.  ``out``: (page_indptr [B + 1], page_indices [B * W],
+    last_page_len [B], seq_lens [B], shared_pages [G] or None) to write into; entries of
+    page_indices past page_indptr[B] are left as they are.  A call that cannot be done
+    (see the status) changes nothing."""
+    dev = _page_state(page_refs, page_table, kv_lens)
+    L, P, pl, row_bytes = _page_pool(pool, page_refs)
+    B, (R, W) = _cache_ints("rows", rows, dev).numel(), page_table.shape
+    if B == 0:
+        raise ValueError("rows is empty")
+    each, add_all = None, 0
+    if isinstance(add, torch.Tensor):
+        each = _cache_ints("add", add, dev, B).data_ptr()
+    else:
+        add_all = int(add)
+    G = 0
+    if group_indptr is not None:
+        G = _cache_ints("group_indptr", group_indptr, dev).numel() - 1
+        if G < 1:
+            raise ValueError("group_indptr needs at least two entries")
+    if out is None:
+        e = lambda n: torch.empty(n, dtype=torch.int32, device=dev)
+        out = (e(B + 1), e(B * W), e(B), e(B), e(G) if G else None)
+    else:
+        out = tuple(out[:5])
+        for name, t, n in zip(("page_indptr", "page_indices", "last_page_len", "seq_lens"), out, (B + 1, None, B, B)):
+            _cache_ints(name, t, dev, n)
+        if G:
+            _cache_ints("shared_pages", out[4], dev, G)
+    status = _status_word(status, dev)
+    nbytes = _lib.lib().pts_cache_workspace_size(P, B)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.call("pts_cache_extend", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
+                  page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), R, W, rows.data_ptr(), each, add_all,
+                  B, group_indptr.data_ptr() if G else None, G, out[0].data_ptr(), out[1].data_ptr(), out[1].numel(),
+                  out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr() if G else None, status.data_ptr(),
+                  ws.data_ptr(), nbytes, _stream(dev))
+    return CacheBatch(*out, status)
+
+
+def cache_truncate(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, page_len: int,
+                   rows: torch.Tensor, new_lens: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cut the listed sequences to ``new_lens`` tokens (int32 [n]; None frees them):
+    pages past the new length lose this holder.  A sequence already shorter keeps its
+    length.  Returns the status word; rows outside the table are skipped."""
+    dev = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("rows", rows, dev).numel()
+    if new_lens is not None:
+        _cache_ints("new_lens", new_lens, dev, n)
+    status = _status_word(status, dev)
+    if n == 0:
+        return status.zero_()
+    with _on(dev):
+        _lib.call("pts_cache_truncate", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+                  kv_lens.data_ptr(), page_table.shape[0], page_table.shape[1], page_refs.numel(), int(page_len),
+                  rows.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, n, status.data_ptr(),
+                  _stream(dev))
+    return status
+
+
+def cache_compact(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.Tensor) -> CompactedCache:
+    """Close the gaps of ``pool``: its n live pages end up in pages 0 .. n-1, moving
+    only those at or past n.  Returns the new counts and table (the inputs keep their
+    values), the page map and the counts."""
+    dev = _page_state(page_refs, page_table, None)
+    L, P, pl, row_bytes = _page_pool(pool, page_refs)
+    R, W = page_table.shape
+    e = lambda *n: torch.empty(*n, dtype=torch.int32, device=dev)
+    out = CompactedCache(e(P), e(R, W), e(P), e(2))
+    nbytes = _lib.lib().pts_cache_workspace_size(P, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.call("pts_cache_compact", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
+                  page_table.data_ptr(), page_table.stride(0), R, W, out.page_refs.data_ptr(),
+                  out.page_table.data_ptr(), out.page_map.data_ptr(), out.counts.data_ptr(), ws.data_ptr(), nbytes,
+                  _stream(dev))
+    return out
