@@ -529,6 +529,30 @@ int pts_tree_attn_run_any(const void* q, const void* kv_layer, const int32_t* qo
                           float sm_scale, int elem_bytes, void* workspace, size_t workspace_bytes,
                           pts_stream_t stream);
 
+/* pts_tree_attn_run_any for requests that share leading pages: requests
+ * group_indptr[g] .. group_indptr[g+1] form group g (all requests, in order), and the
+ * first shared_pages[g] pages in the tables of all of them are the same pages.  The
+ * result is that of pts_tree_attn_run_any on the same tables; the shared pages are read
+ * once per group instead of once per request.  shared_pages[g] may be 0, and is cut
+ * to the pages that lie before every member's query rows.  Rows of q and out past
+ * qo_indptr[batch] are neither read nor written; a row that sees no slot is 0; slots
+ * past a request's length are not used.  max_qo_len bounds the rows of a request;
+ * max_kv_len and max_own_len (tokens after the shared pages; 0: not known) only
+ * choose the schedule.  workspace: pts_tree_attn_shared_workspace_size bytes with the
+ * same arguments, 256-byte aligned, any contents.  error (nullable, zeroed before its
+ * first use) receives a code when a CTA gave up waiting; the output is then not
+ * valid. */
+size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups, int total_q, int max_qo_len, int max_kv_len,
+                                           int max_own_len, int num_qo_heads, int num_kv_heads, int head_dim,
+                                           int page_len, int elem_bytes);
+int pts_tree_attn_run_shared(const void* q, const void* kv_layer, const int32_t* qo_indptr,
+                             const int32_t* page_indptr, const int32_t* page_indices, const int32_t* last_page_len,
+                             const uint64_t* mask_bits, int mask_words, const int32_t* group_indptr,
+                             const int32_t* shared_pages, int num_groups, void* out, int batch, int total_q,
+                             int max_qo_len, int max_kv_len, int max_own_len, int num_qo_heads, int num_kv_heads,
+                             int head_dim, int page_len, int max_pages, float sm_scale, int elem_bytes,
+                             void* workspace, size_t workspace_bytes, int32_t* error, pts_stream_t stream);
+
 /* pts_tree_attn_run with page tables per (request, KV head): head_page_indptr
  * [B*Hkv+1] and head_last_page_len [B*Hkv] indexed b * Hkv + h, every list
  * ending with the request's tree (its last N slots), for example the sparse

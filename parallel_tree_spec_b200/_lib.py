@@ -75,6 +75,10 @@ SIGNATURES = {
                                 C.c_int, vp]),
     "pts_kv_compact": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_int,
                                  vp, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp]),
+    "pts_tree_attn_shared_workspace_size": (sz, [C.c_int] * 11),
+    "pts_tree_attn_run_shared": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, C.c_int, vp, vp, C.c_int, vp, C.c_int, C.c_int,
+                                           C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, f32,
+                                           C.c_int, vp, sz, vp, vp]),
     "pts_cache_workspace_size": (sz, [C.c_int, C.c_int]),
     "pts_cache_fork": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
     "pts_cache_extend": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, i64, vp, C.c_int, C.c_int, vp, vp, C.c_int,

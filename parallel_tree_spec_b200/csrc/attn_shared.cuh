@@ -1,0 +1,65 @@
+// Tree attention for requests that share leading pages: what its kernels have in
+// common (attn_shared.cu: any type and shape; attn_prefix.cu: bf16 tensor cores).
+//
+// The requests group_indptr[g] .. group_indptr[g+1] form group g; the first
+// shared_pages[g] pages of each are the same pages.  A softmax row over the union
+// of two column sets is joined from the two sets' parts: with
+//   m = max s_j,  l = sum e^(s_j - m),  O = sum e^(s_j - m) v_j
+// of each set, M = max(m1, m2), L = l1 e^(m1-M) + l2 e^(m2-M) and likewise O.  So
+// the shared columns are one piece of work for all rows of a group, read once,
+// and each request's own columns another.
+#pragma once
+
+#include "common.cuh"
+
+namespace pts {
+
+struct SharedAttnParams {
+  const void* q;
+  const void* kv;
+  const int32_t* qo_indptr;
+  const int32_t* page_indptr;
+  const int32_t* page_indices;
+  const int32_t* last_page_len;
+  const uint64_t* mask_bits;
+  int mask_words;
+  void* out;
+  const int32_t* group_indptr;
+  const int32_t* shared_pages;
+  int batch, groups;
+  int Hq, Hkv, g, D, page_len, max_pages;
+  float scale;             // of the scores
+};
+
+// Tokens of request b's cache and, of those, the ones before its query rows.
+__device__ __forceinline__ int kv_tokens(const SharedAttnParams& p, int b) {
+  const int n = p.page_indptr[b + 1] - p.page_indptr[b];
+  return n > 0 ? (n - 1) * p.page_len + p.last_page_len[b] : 0;
+}
+
+// The pages of group gi that its rows attend together: shared_pages[gi], but none
+// that holds a query row's own token or lies past a member's table.  A whole warp
+// calls it; every lane returns the result.
+__device__ __forceinline__ int group_shared_pages(const SharedAttnParams& p, int gi) {
+  const int lane = threadIdx.x & 31;
+  int s = p.shared_pages[gi];
+  for (int b = p.group_indptr[gi] + lane; b < p.group_indptr[gi + 1]; b += 32) {
+    const int n = p.qo_indptr[b + 1] - p.qo_indptr[b];
+    if (n <= 0) continue;                               // no rows: nothing to attend
+    s = min(s, max(0, kv_tokens(p, b) - n) / p.page_len);
+  }
+  return max(0, __reduce_min_sync(0xffffffffu, s));
+}
+
+// The group that holds request b.
+__device__ __forceinline__ int group_of(const SharedAttnParams& p, int b) {
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.group_indptr[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace pts

@@ -601,6 +601,66 @@ def tree_attention(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: torch.Ten
     return out
 
 
+def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: torch.Tensor, page_indptr: torch.Tensor,
+                          page_indices: torch.Tensor, last_page_len: torch.Tensor, mask_bits: Optional[torch.Tensor],
+                          max_qo_len: int, max_kv_len: int, group_indptr: torch.Tensor, shared_pages: torch.Tensor,
+                          max_own_len: Optional[int] = None, sm_scale: Optional[float] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``tree_attention`` for requests that share leading pages, which are read once
+    for all rows of a group instead of once per request: requests group_indptr[g] ..
+    group_indptr[g + 1] (int32 [G + 1], all requests in order) hold the same first
+    ``shared_pages[g]`` pages (int32 [G]; cut to the pages before every member's rows).
+    ``cache_extend`` gives these tensors for forked sequences.  ``max_own_len`` bounds
+    the tokens after the shared pages, where the caller knows it; it and
+    ``max_kv_len`` only choose the schedule."""
+    dev = q.device
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on a CUDA device (this path has no CPU implementation)")
+    if q.dtype not in (torch.bfloat16, torch.float32) or kv_layer.dtype != q.dtype:
+        raise ValueError("tree attention takes bf16 or fp32 queries and a cache of the same type")
+    if q.dim() != 3 or kv_layer.dim() != 5 or kv_layer.shape[1] != 2 or kv_layer.shape[4] != q.shape[2]:
+        raise ValueError("q must be [T, Hq, D] and kv_layer [max_pages, 2, page_len, Hkv, D] with the same D")
+    if not q.is_contiguous() or not kv_layer.is_contiguous():
+        raise ValueError("q and kv_layer must be contiguous")
+    if kv_layer.device != dev:
+        raise ValueError("all tensors must be on the same device")
+    T, Hq, D = q.shape
+    P, _, pl, Hkv, _ = kv_layer.shape
+    B = _cache_ints("qo_indptr", qo_indptr, dev).numel() - 1
+    G = _cache_ints("shared_pages", shared_pages, dev).numel()
+    _cache_ints("page_indptr", page_indptr, dev, B + 1)
+    _cache_ints("page_indices", page_indices, dev)
+    _cache_ints("last_page_len", last_page_len, dev, B)
+    _cache_ints("group_indptr", group_indptr, dev, G + 1)
+    words = 1
+    if mask_bits is not None:
+        if mask_bits.dtype != torch.int64 or mask_bits.dim() != 2 or not mask_bits.is_contiguous() or \
+                mask_bits.shape[0] < T or mask_bits.device != dev:
+            raise ValueError("mask_bits must be a contiguous int64 [T, mask_words] tensor on the same device")
+        words = mask_bits.shape[1]
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor like q")
+    own = int(max_own_len) if max_own_len is not None else 0
+    es = q.element_size()
+    lib = _lib.lib()
+    with _on(dev):
+        nbytes = lib.pts_tree_attn_shared_workspace_size(B, G, T, int(max_qo_len), int(max_kv_len), own, Hq, Hkv, D, pl,
+                                                         es)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+        err = workspace(dev, "attn_shared", 256)
+        _lib.call("pts_tree_attn_run_shared", q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(),
+                  page_indptr.data_ptr(), page_indices.data_ptr(), last_page_len.data_ptr(),
+                  mask_bits.data_ptr() if mask_bits is not None else None, words, group_indptr.data_ptr(),
+                  shared_pages.data_ptr(), G, out.data_ptr(), B, T, int(max_qo_len), int(max_kv_len), own, Hq, Hkv, D,
+                  pl, P, float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D), es, ws.data_ptr(), ws.numel(),
+                  err.data_ptr(), _stream(dev))
+    if _CHECK_ATTENTION:
+        check_attention(dev)
+    return out
+
+
 # PTS_B200_CHECK=1: read the attention kernels' error word after every call
 # (synchronises the stream; for debugging).
 _CHECK_ATTENTION = os.environ.get("PTS_B200_CHECK", "0") not in ("", "0")
@@ -610,9 +670,12 @@ def check_attention(device: Optional[torch.device] = None) -> None:
     """Raise if an attention launch on the current stream gave up waiting
     (pts_tree_attn_check: synchronises the stream, then clears the error)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    ws = workspace(dev, "attn", 256)
     status = C.c_int(0)
-    _lib.call("pts_tree_attn_check", ws.data_ptr(), C.addressof(status), _stream(dev))
+    for kind in ("attn", "attn_shared"):
+        ws = workspace(dev, kind, 256)
+        _lib.call("pts_tree_attn_check", ws.data_ptr(), C.addressof(status), _stream(dev))
+        if status.value != 0:
+            break
     if status.value != 0:
         raise RuntimeError(f"tree attention gave up waiting (error {status.value}); its output is not valid")
 
