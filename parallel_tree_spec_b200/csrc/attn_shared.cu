@@ -317,12 +317,12 @@ using namespace pts;
 extern "C" size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups, int total_q, int max_qo_len,
                                                       int max_kv_len, int max_own_len, int num_qo_heads,
                                                       int num_kv_heads, int head_dim, int page_len, int elem_bytes) {
-  (void)max_own_len;
-  (void)page_len;
-  (void)elem_bytes;
   if (batch <= 0 || num_groups <= 0 || total_q <= 0 || max_qo_len <= 0 || max_kv_len <= 0 || num_qo_heads <= 0 ||
       num_kv_heads <= 0 || num_qo_heads % num_kv_heads || head_dim <= 0)
     return 0;
+  if (prefix_attn_supports(head_dim, page_len, elem_bytes))
+    return prefix_attn_workspace(batch, num_groups, total_q, max_qo_len, max_kv_len, max_own_len, num_qo_heads,
+                                 num_kv_heads, head_dim);
   return make_plan(batch, num_groups, total_q, max_qo_len, max_kv_len, num_qo_heads, num_kv_heads, head_dim).bytes;
 }
 
@@ -357,7 +357,6 @@ extern "C" int pts_tree_attn_run_shared(const void* q, const void* kv_layer, con
                                                           elem_bytes);
   if (!workspace || workspace_bytes < need)
     return set_error(PTS_ERR_CAPACITY, "workspace of %zu bytes (%zu needed)", workspace_bytes, need);
-  (void)error;
   SharedAttnParams a{};
   a.q = q;
   a.kv = kv_layer;
@@ -379,6 +378,8 @@ extern "C" int pts_tree_attn_run_shared(const void* q, const void* kv_layer, con
   a.page_len = page_len;
   a.max_pages = max_pages;
   a.scale = sm_scale;
+  if (prefix_attn_supports(head_dim, page_len, elem_bytes))
+    return prefix_attn_launch(a, total_q, max_qo_len, max_kv_len, max_own_len, workspace, error, (cudaStream_t)stream);
   const Plan pl = make_plan(batch, num_groups, total_q, max_qo_len, max_kv_len, num_qo_heads, num_kv_heads, head_dim);
   const int64_t gx = (int64_t)pl.group_tiles + (int64_t)batch * pl.request_tiles;
   if (gx > 2147483647ll) return set_error(PTS_ERR_CAPACITY, "grid too large");

@@ -62,4 +62,11 @@ __device__ __forceinline__ int group_of(const SharedAttnParams& p, int b) {
   return lo;
 }
 
+// attn_prefix.cu: bf16, head_dim 64 or 128, pages of whole 16-token runs.
+bool prefix_attn_supports(int head_dim, int page_len, int elem_bytes);
+size_t prefix_attn_workspace(int batch, int groups, int total_q, int max_qo_len, int max_kv_len, int max_own_len,
+                             int Hq, int Hkv, int D);
+int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, int max_kv_len, int max_own_len,
+                       void* workspace, int32_t* error, cudaStream_t stream);
+
 }  // namespace pts
