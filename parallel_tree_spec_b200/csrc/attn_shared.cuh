@@ -14,6 +14,15 @@
 
 namespace pts {
 
+// n / d by multiplication: exact for n * d < 2^32 (the launcher checks its n).
+struct FastDiv {
+  uint32_t d, m;           // m = ceil(2^32 / d)
+  __host__ __device__ __forceinline__ FastDiv() {}
+  __host__ explicit FastDiv(uint32_t divisor)
+      : d(divisor), m(divisor > 1 ? (uint32_t)((0x100000000ull + divisor - 1) / divisor) : 0u) {}
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, m); }
+};
+
 struct SharedAttnParams {
   const void* q;
   const void* kv;
