@@ -31,21 +31,23 @@ namespace {
 using namespace sm100;
 
 constexpr int kBlock = 128;               // tokens per block
-constexpr int kRun = 16;                  // tokens per TMA copy
+constexpr int kRun = 16;                  // tokens of one value product; pages are whole runs
 constexpr int kRuns = kBlock / kRun;
 constexpr int kTileRows = 256;
 constexpr int kThreads = 384;             // warps 0 TMA, 1 MMA, 2-3 plan, 4-7 and 8-11 softmax
 constexpr int kMaxSplits = 32;
-constexpr int kPlanSmem = 48;             // groups whose plan fits in shared memory
+constexpr int kPlanSmem = 40;             // groups whose plan fits in shared memory
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
 
-// A block's K (or V) in shared memory: 16-token runs of [half][16 tokens][64 dims], each
-// half 2 KB of 128-byte-swizzled rows, so that one TMA copy brings a whole run.
+// A block's K (or V) in shared memory: [8-token group][64-dim half][8 tokens][64 dims],
+// 128-byte-swizzled rows.  One TMA copy brings a page's tokens (up to a block) with both
+// halves, and the groups of a half lie evenly apart, as the matrix descriptors want.
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
-  static constexpr uint32_t kRunBytes = kHalves * kRun * 128;
+  static constexpr uint32_t kGroupBytes = kHalves * 1024;
+  static constexpr uint32_t kRunBytes = 2 * kGroupBytes;
   static constexpr uint32_t kSlotBytes = kRuns * kRunBytes;     // K or V of a block; Q of a stream
   static constexpr uint32_t kQHalfBytes = 128 * 128;            // Q: [half][128 rows][64 dims]
   static constexpr int kSlots = D == 128 ? 5 : 8;
@@ -60,6 +62,8 @@ static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared
 struct GroupPlan {
   int pages;      // shared pages
   int rows;       // query rows per KV head
+  int tok0;       // the group's first token
+  int table;      // where the page table of its first request with rows starts
   int first;      // first work item
   int splits;     // block ranges per (row tile, KV head)
 };
@@ -86,6 +90,7 @@ static_assert(sizeof(Bars) <= 1280, "barrier block");
 struct PrefixParams {
   SharedAttnParams a;
   FastDiv div_g;
+  int copy_tokens;          // tokens per TMA copy: the power of two in page_len, at most a block
   int page_shift;           // log2(page_len), or -1
   float scale_log2;
   int max_items;            // parts in the workspace
@@ -107,6 +112,16 @@ __device__ __forceinline__ void give_up(const PrefixParams& p, int code) {
 }
 
 __device__ __forceinline__ int blocks_of(int pages, int page_len) { return (pages * page_len + kBlock - 1) / kBlock; }
+__device__ __forceinline__ int tiles_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
+
+// a / b for 0 <= a < 2^24, 0 < b < 2^24 (the quotient by floats is off by one at most):
+// the planning is a chain of these, and the compiler's integer division is a longer one.
+__device__ __forceinline__ int small_div(int a, int b) {
+  int q = (int)__fdividef((float)a, (float)b);
+  const int r = a - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+__device__ __forceinline__ int ceil_div(int a, int b) { return small_div(a + b - 1, b); }
 
 __device__ __noinline__ bool find_item(const PrefixParams& p, const Bars& bars, const GroupPlan* plan, int i,
                                        Item& it) {
@@ -118,16 +133,11 @@ __device__ __noinline__ bool find_item(const PrefixParams& p, const Bars& bars, 
     else hi = mid;
   }
   const GroupPlan g = plan[lo];
-  const int tiles = (g.rows + kTileRows - 1) / kTileRows;
-  int b = p.a.group_indptr[lo];                         // the group's first request with rows
-  it.tok0 = p.a.qo_indptr[b];
-  while (p.a.qo_indptr[b + 1] == it.tok0) ++b;
-  it.table = p.a.page_indptr[b];
-  unsigned u = i - g.first;
-  const unsigned split = u % (unsigned)g.splits;
-  u /= (unsigned)g.splits;
-  it.h = u / (unsigned)tiles;
-  it.row0 = u % (unsigned)tiles * kTileRows;
+  const int u = small_div(i - g.first, g.splits), split = i - g.first - u * g.splits;
+  it.tok0 = g.tok0;
+  it.table = g.table;
+  it.h = small_div(u, tiles_of(g.rows));
+  it.row0 = (u - it.h * tiles_of(g.rows)) * kTileRows;
   it.rows = min(kTileRows, g.rows - it.row0);
   it.tokens = g.pages * p.a.page_len;
   it.ja = split * bars.chunk;
@@ -142,38 +152,37 @@ __device__ __noinline__ bool find_item(const PrefixParams& p, const Bars& bars, 
 __device__ __forceinline__ void plan_groups(const PrefixParams& p, GroupPlan* plan, int w) {
   const SharedAttnParams& a = p.a;
   for (int g = w; g < a.groups; g += 3) {
-    const int pages = group_shared_pages(a, g);
-    const int rows = (a.qo_indptr[a.group_indptr[g + 1]] - a.qo_indptr[a.group_indptr[g]]) * a.g;
-    if ((threadIdx.x & 31) == 0) plan[g] = GroupPlan{rows > 0 ? pages : 0, rows, 0, 0};
+    int lead;
+    const int pages = group_shared_pages(a, g, &lead);
+    const int b0 = a.group_indptr[g], b1 = a.group_indptr[g + 1];
+    const int tok0 = a.qo_indptr[b0], rows = (a.qo_indptr[b1] - tok0) * a.g;
+    if ((threadIdx.x & 31) == 0)
+      plan[g] = GroupPlan{rows > 0 ? pages : 0, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0};
   }
 }
 
 __device__ __forceinline__ void plan_ranges(const PrefixParams& p, Bars& bars, GroupPlan* plan) {
   const SharedAttnParams& a = p.a;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, ctas = gridDim.x;
   int longest = 1;
   for (int g = lane; g < a.groups; g += 32) longest = max(longest, blocks_of(plan[g].pages, a.page_len));
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const unsigned c = (unsigned)(longest + lane) / (unsigned)(lane + 1);
-  unsigned items = 0;
-  for (int g = 0; g < a.groups; ++g) {
-    const unsigned nb = blocks_of(plan[g].pages, a.page_len);
-    items += (unsigned)((plan[g].rows + kTileRows - 1) / kTileRows) * a.Hkv * ((nb + c - 1) / c);
-  }
+  const int c = ceil_div(longest, lane + 1);
+  int items = 0;
+  for (int g = 0; g < a.groups; ++g)
+    items += tiles_of(plan[g].rows) * a.Hkv * ceil_div(blocks_of(plan[g].pages, a.page_len), c);
   unsigned cost = 0xffffffffu;
-  if (lane == 0 || (lane < longest && items <= (unsigned)p.max_items))
-    cost = (items + gridDim.x - 1) / gridDim.x * (2 * c + 3);
+  if (lane == 0 || (lane < longest && items <= p.max_items)) cost = (unsigned)ceil_div(items, ctas) * (2 * c + 3);
   const unsigned win = __reduce_min_sync(0xffffffffu, cost);
   // equal costs: the longer ranges (fewer parts)
-  const unsigned chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0u);
+  const int chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0);
   int run = 0;
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
-    int n = 0;
+    int n = 0, splits = 0;
     if (g < a.groups) {
-      const int splits = (int)((unsigned)(blocks_of(plan[g].pages, a.page_len) + chunk - 1) / chunk);
-      n = (plan[g].rows + kTileRows - 1) / kTileRows * a.Hkv * splits;
-      plan[g].splits = splits;
+      splits = ceil_div(blocks_of(plan[g].pages, a.page_len), chunk);
+      n = tiles_of(plan[g].rows) * a.Hkv * splits;
     }
     int incl = n;
 #pragma unroll
@@ -182,17 +191,18 @@ __device__ __forceinline__ void plan_ranges(const PrefixParams& p, Bars& bars, G
       if (lane >= o) incl += y;
     }
     if (g < a.groups) {
+      plan[g].splits = splits;
       plan[g].first = run + incl - n;
       if (blockIdx.x == 0) p.plan[g] = plan[g];
     }
     run += __shfl_sync(0xffffffffu, incl, 31);
   }
-  __syncwarp();
   if (lane == 0) {
     bars.chunk = chunk;
     bars.total = min(run, p.max_items);
-    find_item(p, bars, plan, blockIdx.x, bars.first);
   }
+  __syncwarp();
+  if (lane == 0) find_item(p, bars, plan, blockIdx.x, bars.first);
 }
 
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
@@ -305,17 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc_fence_after();
         }
-        // column c: token 16 * ((c & 63) / 8) + c % 8 + 8 * (c / 64) of the block (the
-        // score products take the runs' first eight tokens, then their last eight)
         uint32_t s[2][64];
         tmem_ld32_x2(s_tm, s[0]);
         tmem_ld32_x2(s_tm + 64, s[1]);
         tmem_ld_wait();
-        const int left = it.tokens - (it.ja + (two ? x : 2 * x + t)) * kBlock;   // whole runs
+        const int left = it.tokens - (it.ja + (two ? x : 2 * x + t)) * kBlock;
         if (left < kBlock) {
 #pragma unroll
           for (int c = 0; c < kBlock; ++c)
-            if ((c & 63) / 8 >= left / kRun) s[c / 64][c % 64] = __float_as_uint(-INFINITY);
+            if (c >= left) s[c / 64][c % 64] = __float_as_uint(-INFINITY);
         }
         float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
 #pragma unroll
@@ -336,15 +344,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float sub = m == -INFINITY ? 0.0f : m;
         const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), nm2 = f2(-sub, -sub);
         uint64_t l0 = f2(0.0f, 0.0f), l1 = l0;
-        // P in token order: run r's 16 tokens are its columns of both halves
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t pk[32];
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
-            const int run = part * 4 + c / 16, u = c % 16, col = run * 8 + u % 8;
             float y0, y1;
-            f2_split(ffma2(f2(__uint_as_float(s[u / 8][col]), __uint_as_float(s[u / 8][col + 1])), sc2, nm2), y0, y1);
+            f2_split(ffma2(f2(__uint_as_float(s[part][c]), __uint_as_float(s[part][c + 1])), sc2, nm2), y0, y1);
             y0 = fast_exp2(y0);
             y1 = fast_exp2(y1);
             if (c & 2) l1 = fadd2(l1, f2(y0, y1));
@@ -423,9 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();                                    // the plan is complete
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
-      // Lane r < 8 brings 16-token run r.  The page of load x + 4 is fetched while load
-      // x is issued (unrolled by four, so that no register that a fetch is still
+      // Lane r brings the r-th copy of a block.  The page of load x + 4 is fetched while
+      // load x is issued (unrolled by four, so that no register that a fetch is still
       // filling is moved).
+      const int copies = kBlock / p.copy_tokens;
       bool ok = true;
       int pushed = 0;                                   // copies into the ring so far
       Item it = bars.first;
@@ -446,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             is_v = x == 2 * n - 1 || !(x & 1);
             j = x == 2 * n - 1 ? n - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
           }
-          tok = (it.ja + j) * kBlock + (lane & 7) * kRun;
+          tok = (it.ja + j) * kBlock + (lane & (copies - 1)) * p.copy_tokens;
         };
         auto fetch = [&](int x) -> int {
           bool is_v;
@@ -464,9 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (page < 0 || page >= a.max_pages) page = a.max_pages;  // past the pool: zero fill
           if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], S::kSlotBytes);
           __syncwarp();
-          if (lane < kRuns)
-            tma_load_5d(smem + S::kOffRing + s * S::kSlotBytes + lane * S::kRunBytes, &kv_map, &bars.full[s], 0,
-                        tok - p.page_of(tok) * a.page_len, 0, it.h, 2 * page + (is_v ? 1 : 0));
+          if (lane < copies)
+            tma_load_5d(smem + S::kOffRing + s * S::kSlotBytes + lane * (p.copy_tokens / 8) * S::kGroupBytes, &kv_map,
+                        &bars.full[s], 0, 0, it.h * S::kHalves, (tok - p.page_of(tok) * a.page_len) / 8,
+                        2 * page + (is_v ? 1 : 0));
           __syncwarp();
           ++pushed;
         };
@@ -494,13 +502,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer, one thread
       if (elect_one()) {
-        const uint32_t id_qk = idesc_bf16_f32(128, 64, 0, 0);
+        const uint32_t id_qk = idesc_bf16_f32(128, kBlock, 0, 0);
         const uint32_t id_pv = idesc_bf16_f32(128, D, 0, 1);
-        // K: eight-token groups 2 KB * halves apart; V: a run's two groups 1 KB apart,
-        // its halves 2 KB
+        // eight-token groups kGroupBytes apart, a group's halves 1 KB
         const uint64_t q0 = smem_desc(smem_u32(smem + S::kOffQ), 16, 1024, kSwizzle128B);
-        const uint64_t k0 = smem_desc(smem_u32(smem + S::kOffRing), 16, S::kRunBytes, kSwizzle128B);
-        const uint64_t v0 = smem_desc(smem_u32(smem + S::kOffRing), kRun * 128, 1024, kSwizzle128B);
+        const uint64_t k0 = smem_desc(smem_u32(smem + S::kOffRing), 16, S::kGroupBytes, kSwizzle128B);
+        const uint64_t v0 = smem_desc(smem_u32(smem + S::kOffRing), 1024, S::kGroupBytes, kSwizzle128B);
         bool ok = true, issued = false;
         int base = 0, items = 0, steps[2] = {0, 0};     // ring positions before this item; items and blocks done
         auto wait = [&](uint64_t* bar, int parity, int code) {
@@ -536,12 +543,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint64_t qd = q0 + (uint64_t)((two ? t * S::kSlotBytes : 0u) >> 4);
               const uint64_t kd = k0 + (uint64_t)((slot * S::kSlotBytes) >> 4);
 #pragma unroll
-              for (int part = 0; part < 2; ++part)
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                  mma_bf16_ss(tmem + kColS + 128 * t + 64 * part,
-                              qd + (uint64_t)(((k / 4) * S::kQHalfBytes + (k % 4) * 32) >> 4),
-                              kd + (uint64_t)((part * 1024 + (k / 4) * kRun * 128 + (k % 4) * 32) >> 4), id_qk, k > 0);
+              for (int k = 0; k < D / 16; ++k)
+                mma_bf16_ss(tmem + kColS + 128 * t, qd + (uint64_t)(((k / 4) * S::kQHalfBytes + (k % 4) * 32) >> 4),
+                            kd + (uint64_t)(((k / 4) * 1024 + (k % 4) * 32) >> 4), id_qk, k > 0);
               mma_commit(&bars.s_full[t]);
               if (!two || t == 1) mma_commit(&bars.empty[slot]);
               issued = true;
@@ -639,6 +643,7 @@ __device__ __forceinline__ void join_rows(const PrefixParams& p, const GroupPlan
            (in & 127) * 4;
   };
   const int most = 2 * g.splits + own_parts;
+#pragma unroll 4
   for (int e = threadIdx.x; e < most * ROWS; e += kOwnThreads) {
     const int k = e / ROWS, r = e % ROWS;
     float m = -INFINITY, l = 0.0f;
@@ -680,15 +685,20 @@ __device__ __forceinline__ void join_rows(const PrefixParams& p, const GroupPlan
     int shared;
     const float* s = part_of(r, 0, shared) + quad * 512;
     const int64_t step = shared == g.splits ? kPart : kHalf;
-#pragma unroll 8
-    for (int k = 0; k < shared; ++k) {
-      const float x = w[k * ROWS + r];
-      if (x != 0.0f) {                                  // a part of no columns has no O
-        const float4 v = __ldcg((const float4*)(s + k * step));
-        o0 = fmaf(x, v.x, o0);
-        o1 = fmaf(x, v.y, o1);
-        o2 = fmaf(x, v.z, o2);
-        o3 = fmaf(x, v.w, o3);
+    for (int k0 = 0; k0 < shared; k0 += 8) {
+      float4 v[8];                                      // eight loads in flight
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k0 + u < shared) v[u] = __ldcg((const float4*)(s + (k0 + u) * step));
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float x = k0 + u < shared ? w[(k0 + u) * ROWS + r] : 0.0f;
+        if (x != 0.0f) {                                // a part of no columns has no O
+          o0 = fmaf(x, v[u].x, o0);
+          o1 = fmaf(x, v[u].y, o1);
+          o2 = fmaf(x, v[u].z, o2);
+          o3 = fmaf(x, v[u].w, o3);
+        }
       }
     }
 #pragma unroll 2
@@ -1067,11 +1077,11 @@ template <int D>
 int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int total_q, cudaStream_t stream) {
   const SharedAttnParams& a = p.a;
   CUtensorMap map;
-  // (dim of a half, token, half, head, 2 page + K/V)
-  const cuuint64_t dims[5] = {64, (cuuint64_t)a.page_len, D / 64, (cuuint64_t)a.Hkv, (cuuint64_t)a.max_pages * 2};
-  const cuuint64_t strides[4] = {(cuuint64_t)a.Hkv * D * 2, 128, (cuuint64_t)D * 2,
-                                 (cuuint64_t)a.page_len * a.Hkv * D * 2};
-  const cuuint32_t box[5] = {64, (cuuint32_t)kRun, D / 64, 1, 1};
+  // (dim of a half, token of a group, head and half, group, 2 page + K/V)
+  const cuuint64_t tok = (cuuint64_t)a.Hkv * D * 2;
+  const cuuint64_t dims[5] = {64, 8, (cuuint64_t)a.Hkv * (D / 64), (cuuint64_t)a.page_len / 8, (cuuint64_t)a.max_pages * 2};
+  const cuuint64_t strides[4] = {tok, 128, 8 * tok, a.page_len * tok};
+  const cuuint32_t box[5] = {64, 8, D / 64, (cuuint32_t)p.copy_tokens / 8, 1};
   if (int rc = encode_tiled_bf16_sw128(&map, 5, a.kv, dims, strides, box)) return rc;
   if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem)) return rc;
   PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, map));
@@ -1105,6 +1115,8 @@ int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, i
   PrefixParams p{};
   p.a = a;
   p.div_g = FastDiv((uint32_t)a.g);
+  p.copy_tokens = kRun;
+  while (p.copy_tokens < kBlock && a.page_len % (2 * p.copy_tokens) == 0) p.copy_tokens *= 2;
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a.page_len == 1 << s) p.page_shift = s;

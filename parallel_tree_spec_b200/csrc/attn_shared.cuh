@@ -48,15 +48,21 @@ __device__ __forceinline__ int kv_tokens(const SharedAttnParams& p, int b) {
 
 // The pages of group gi that its rows attend together: shared_pages[gi], but none
 // that holds a query row's own token or lies past a member's table.  A whole warp
-// calls it; every lane returns the result.
-__device__ __forceinline__ int group_shared_pages(const SharedAttnParams& p, int gi) {
+// calls it; every lane returns the result.  `lead` (nullable) receives the group's first
+// request with rows, or the one past its last.
+__device__ __forceinline__ int group_shared_pages(const SharedAttnParams& p, int gi, int* lead = nullptr) {
   const int lane = threadIdx.x & 31;
-  int s = p.shared_pages[gi];
-  for (int b = p.group_indptr[gi] + lane; b < p.group_indptr[gi + 1]; b += 32) {
-    const int n = p.qo_indptr[b + 1] - p.qo_indptr[b];
-    if (n <= 0) continue;                               // no rows: nothing to attend
-    s = min(s, max(0, kv_tokens(p, b) - n) / p.page_len);
+  const int b0 = p.group_indptr[gi], b1 = p.group_indptr[gi + 1];
+  int s = p.shared_pages[gi], first = b1;
+#pragma unroll 4
+  for (int b = b0 + lane; b < b1; b += 32) {
+    const int n = p.qo_indptr[b + 1] - p.qo_indptr[b], before = kv_tokens(p, b) - n;
+    if (n > 0) {                                        // no rows: nothing to attend
+      s = min(s, before > 0 ? before / p.page_len : 0);
+      first = min(first, b);
+    }
   }
+  if (lead) *lead = __reduce_min_sync(0xffffffffu, first);
   return max(0, __reduce_min_sync(0xffffffffu, s));
 }
 
