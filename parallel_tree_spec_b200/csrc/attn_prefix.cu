@@ -1,23 +1,24 @@
 // Tree attention for requests that share leading pages, bf16 with head_dim 64 or 128
-// and pages of whole 16-token runs, on the tensor cores.  Two launches:
+// and pages of whole 16-token runs, on the tensor cores.  Three launches:
 //
-// prefix_attn_kernel: the shared columns, once for all rows of a group.  A group's
-//   rows -- (token, query head of the KV head's group), its requests one after the
-//   other -- are cut into tiles of 256; a work item is a row tile, a KV head and a
-//   range of 128-token blocks.  Two streams of S = Q K^T, P = e^(S - m), O += P V run
-//   in a CTA so that the tensor cores compute one's products while the other's
-//   exponentials run: stream t holds rows 128 t .. 128 t + 127 of the tile, or, for
-//   tiles of up to 128 rows (decoding a few dozen sequences), the same rows and every
-//   second block.  tcgen05 with S and O in TMEM, P written back over S as the A operand
-//   of the value product; K/V by TMA, a 16-token run at a time, into a ring; one
-//   thread per row, so the softmax needs no shuffles.  Each item leaves one part per
-//   row (fp32 O, m, l).
-// own_attn_kernel: each request's own columns with its tree mask, then the join with
-//   the shared parts.  A request has few rows (1 to 16 when decoding), far below the
-//   tensor cores' 128-row tiles, and each of its K/V bytes is used by those rows only:
-//   it is bound by HBM, so mma.sync m16n8k16 fed by cp.async is enough, and many small
-//   CTAs per SM keep the loads in flight.  It starts while the first kernel runs
-//   out (programmatic dependent launch) and waits for it before the join only.
+// plan_own_kernel: CTA 0 makes the plan of the second launch (which lengths are on the
+//   device only): the column sets -- each group's shared columns, each request's own
+//   -- with their rows and tokens, cut into work items.  The other CTAs, when requests
+//   have at most 16 query rows per KV head (decoding), compute the requests' own
+//   columns: so few rows fill an eighth of a 128-row tensor-core tile at most, and the
+//   K/V bytes serve those rows only, so HBM is the bound and mma.sync m16n8k16 on
+//   transposed products, fed by TMA through a small ring per warp, is enough.
+// prefix_attn_kernel: the work items, one at a time per CTA (persistent, claimed from a
+//   counter): a tile of 256 query rows -- (token, query head of the KV head's group),
+//   a group's requests one after the other -- a KV head and a range of 128-token blocks.
+//   Shared columns are read once for all rows of a group; own columns take the tree
+//   mask.  Two streams of S = Q K^T, P = e^(S - m), O += P V run in a CTA so that the
+//   tensor cores compute one's products while the other's exponentials run: stream t
+//   holds rows 128 t .. 128 t + 127 of the tile, or, for tiles of up to 128 rows, the same
+//   rows and every second block.  tcgen05 with S and O in TMEM, P written back over S as
+//   the A operand of the value product; K/V by TMA into a ring; one thread per row, so
+//   the softmax needs no shuffles.  Each item leaves one part per row (fp32 O, m, l).
+// join_parts_kernel: joins every row's parts and writes the output.
 //
 // Scores are kept in units of log2: x = s * scale * log2(e), e^(s - m) = 2^(x - m').
 #include <algorithm>
@@ -34,13 +35,15 @@ constexpr int kBlock = 128;               // tokens per block
 constexpr int kRun = 16;                  // tokens of one value product; pages are whole runs
 constexpr int kRuns = kBlock / kRun;
 constexpr int kTileRows = 256;
-constexpr int kThreads = 384;             // warps 0 TMA, 1 MMA, 2-3 plan, 4-7 and 8-11 softmax
-constexpr int kMaxSplits = 32;
-constexpr int kPlanSmem = 40;             // groups whose plan fits in shared memory
+constexpr int kThreads = 384;             // warps 0 TMA, 1 MMA, 2-3 masked values, 4-7 and 8-11 softmax
+constexpr int kMaxSplits = 32;            // block ranges of a column set
+constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in the first kernel
+constexpr int kFewRows = 16;              // rows per KV head up to which the first kernel takes them
+constexpr int kMaxTreeWords = PTS_MAX_TREE_NODES / 32;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
 
-// A block's K (or V) in shared memory: [8-token group][64-dim half][8 tokens][64 dims],
+// K (or V) in shared memory: [8-token group][64-dim half][8 tokens][64 dims],
 // 128-byte-swizzled rows.  One TMA copy brings a page's tokens (up to a block) with both
 // halves, and the groups of a half lie evenly apart, as the matrix descriptors want.
 template <int D>
@@ -54,38 +57,48 @@ struct Shape {
   static constexpr uint32_t kOffQ = 0;
   static constexpr uint32_t kOffRing = 2 * kSlotBytes;
   static constexpr uint32_t kOffBars = kOffRing + kSlots * kSlotBytes;
-  static constexpr uint32_t kSmem = kOffBars + 1280 + 1024;     // barriers, plan; alignment slack
+  static constexpr uint32_t kSmem = kOffBars + 1536 + 1024;     // barriers; alignment slack
   static constexpr int kPartFloats = 2 * 128 * (D + 2);         // one item's part: two streams' rows
 };
 static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared memory above 227 KB");
 
-struct GroupPlan {
-  int pages;      // shared pages
+// A column set: entries 0 .. groups - 1 are the groups' shared columns, groups + b the
+// own columns of request b (where they are work items).
+struct Entry {
+  int tokens;     // columns
+  int prefix;     // of those, the ones that every row sees; from there on the tree mask
   int rows;       // query rows per KV head
-  int tok0;       // the group's first token
-  int table;      // where the page table of its first request with rows starts
+  int tok0;       // first token of the rows
+  int table;      // where its page table starts
   int first;      // first work item
   int splits;     // block ranges per (row tile, KV head)
+  int pages;      // a group: its shared pages
 };
 
-// One work item.
-struct Item {
-  int h, tok0, table;       // KV head; first token of the group; its page table
-  int rows, row0;           // rows of the tile: row0 .. of the group's rows per KV head
-  int ja, jb, tokens;       // blocks; tokens of the shared columns
+struct __align__(16) Item {
+  int tokens, prefix, rows, tok0;         // of the entry; rows of the tile
+  int table, row0, h, own;                // row0: first row of the tile; own: takes the tree mask
+  int ja, jb, pad0, pad1;                 // blocks
 };
 
-struct __align__(8) Bars {
+struct PlanHead {
+  int total, next;          // work items; the next one that nobody has claimed
+};
+
+struct __align__(16) Bars {
+  Item items[2];            // by the parity of the CTA's item count
+  int index[2];             // their numbers, or -1: no more
+  uint64_t item_full[2], item_free[2];
   uint64_t q_ready;         // both warpgroups: done with the last item, this one's rows stored
   uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_full[2];
+  uint64_t s_full[2], p_full[2][2];       // P of a stream: its first and second 64 columns
   uint64_t o_full, drain;
   uint32_t tmem;
-  int chunk, total;         // blocks per range, work items
-  Item first;               // this CTA's first item
-  GroupPlan plan[kPlanSmem];
+  // masked value blocks so far: in shared memory; gone over by warps 2 and 3
+  volatile int arrived, cleaned[2];
+  uint32_t odd[4][2][kMaxTreeWords];      // by item count mod 4 and warp: tree slots with infinities or NaN in V
 };
-static_assert(sizeof(Bars) <= 1280, "barrier block");
+static_assert(sizeof(Bars) <= 1536, "barrier block");
 
 struct PrefixParams {
   SharedAttnParams a;
@@ -93,14 +106,18 @@ struct PrefixParams {
   int copy_tokens;          // tokens per TMA copy: the power of two in page_len, at most a block
   int page_shift;           // log2(page_len), or -1
   float scale_log2;
-  int max_items;            // parts in the workspace
-  float* parts;
-  GroupPlan* plan;          // [groups], for the second kernel
-  GroupPlan* cta_plan;      // [CTAs][groups] when the groups do not fit in shared memory
   int* error;
   long long wait_limit;
-  // own columns
-  int own_splits, request_tiles;
+  // plan
+  int ctas;                 // of the second kernel
+  int max_items;            // parts in the workspace
+  int own_items;            // own columns are work items
+  PlanHead* head;
+  Entry* entries;
+  Item* items;
+  float* parts;
+  // own columns in the first kernel
+  int own_tiles, own_splits;
   float* own_o;             // [T * Hq][own_splits][D]
   float2* own_ml;           // [T * Hq][own_splits]
 
@@ -111,108 +128,427 @@ __device__ __forceinline__ void give_up(const PrefixParams& p, int code) {
   if (p.error) atomicExch(p.error, code);
 }
 
-__device__ __forceinline__ int blocks_of(int pages, int page_len) { return (pages * page_len + kBlock - 1) / kBlock; }
+__device__ __forceinline__ int blocks_of(int tokens) { return (tokens + kBlock - 1) / kBlock; }
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
 
-// a / b for 0 <= a < 2^24, 0 < b < 2^24 (the quotient by floats is off by one at most):
-// the planning is a chain of these, and the compiler's integer division is a longer one.
-__device__ __forceinline__ int small_div(int a, int b) {
-  int q = (int)__fdividef((float)a, (float)b);
-  const int r = a - q * b;
-  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
-}
-__device__ __forceinline__ int ceil_div(int a, int b) { return small_div(a + b - 1, b); }
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
 
-__device__ __noinline__ bool find_item(const PrefixParams& p, const Bars& bars, const GroupPlan* plan, int i,
-                                       Item& it) {
-  if (i >= bars.total) return false;
-  int lo = 0, hi = p.a.groups;                          // the last group whose first item is <= i
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (plan[mid].first <= i) lo = mid;
-    else hi = mid;
+// Which of columns c0 .. c0 + 63 row `node` (token tok of the queries) sees (bit i: column
+// c0 + i): those before `prefix`, then tree slots by the row's mask, or up to its own
+// without masks; none from `len` on.
+__device__ __noinline__ uint64_t seen_columns(const SharedAttnParams& a, int tok, int node, int c0, int prefix,
+                                              int len) {
+  uint64_t v = low_bits(min(prefix, len) - c0);
+  const int first = max(prefix, c0), end = min(len, c0 + 64);   // tree columns of the 64
+  if (first < end) {
+    const int slot = first - prefix;
+    uint64_t bits;
+    if (!a.mask_bits) {
+      bits = low_bits(node - slot + 1);
+    } else {
+      const uint64_t* mask = a.mask_bits + (int64_t)tok * a.mask_words;
+      const int w = slot >> 6, sh = slot & 63;
+      const uint64_t lo = w < a.mask_words ? __ldg(mask + w) : 0ull;
+      const uint64_t hi = sh && w + 1 < a.mask_words ? __ldg(mask + w + 1) : 0ull;
+      bits = sh ? (lo >> sh) | (hi << (64 - sh)) : lo;
+    }
+    v |= (bits & low_bits(end - first)) << (first - c0);
   }
-  const GroupPlan g = plan[lo];
-  const int u = small_div(i - g.first, g.splits), split = i - g.first - u * g.splits;
-  it.tok0 = g.tok0;
-  it.table = g.table;
-  it.h = small_div(u, tiles_of(g.rows));
-  it.row0 = (u - it.h * tiles_of(g.rows)) * kTileRows;
-  it.rows = min(kTileRows, g.rows - it.row0);
-  it.tokens = g.pages * p.a.page_len;
-  it.ja = split * bars.chunk;
-  it.jb = min((it.tokens + kBlock - 1) / kBlock, it.ja + bars.chunk);
-  return true;
+  return v;
 }
 
-// Every CTA makes the plan for itself (warps 0, 2 and 3): each group's shared pages and
-// rows, then the length of a block range.  With c blocks per range the launch takes
-// about ceil(items / CTAs) * (c + 1.5) block times (an item's start and end cost about
-// one and a half blocks); lane k tries ranges of ceil(longest / (k + 1)) blocks.
-__device__ __forceinline__ void plan_groups(const PrefixParams& p, GroupPlan* plan, int w) {
+// One of two packed bf16 values is infinite or NaN.
+__device__ __forceinline__ bool odd2(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// ---------------------------------------------------------------- first kernel
+constexpr int kOwnThreads = 128;
+constexpr int kOwnStages = 2;
+
+// The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
+// and end cost about one and a half), and the launch about the larger of the total over
+// the CTAs and the large items' rounds; the cheapest of up to 32 ranges of
+// ceil(longest / k) blocks is taken.  On one CTA, beside the own columns' CTAs.
+__device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
   const SharedAttnParams& a = p.a;
-  for (int g = w; g < a.groups; g += 3) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* sums = (int*)smem;                               // [3][32]: items, large items, blocks
+  int* red = sums + 96;                                 // [4]; chunk at red[4]; running item count at red[5]
+  for (int g = warp; g < a.groups; g += kOwnThreads / 32) {
     int lead;
     const int pages = group_shared_pages(a, g, &lead);
     const int b0 = a.group_indptr[g], b1 = a.group_indptr[g + 1];
     const int tok0 = a.qo_indptr[b0], rows = (a.qo_indptr[b1] - tok0) * a.g;
-    if ((threadIdx.x & 31) == 0)
-      plan[g] = GroupPlan{rows > 0 ? pages : 0, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0};
+    if (lane == 0) {
+      const int tokens = rows > 0 ? pages * a.page_len : 0;
+      p.entries[g] = Entry{tokens, tokens, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0, rows > 0 ? pages : 0};
+    }
   }
-}
-
-__device__ __forceinline__ void plan_ranges(const PrefixParams& p, Bars& bars, GroupPlan* plan) {
-  const SharedAttnParams& a = p.a;
-  const int lane = threadIdx.x & 31, ctas = gridDim.x;
+  for (int i = tid; i < 96; i += kOwnThreads) sums[i] = 0;
+  __syncthreads();
+  const int entries = a.groups + (p.own_items ? a.batch : 0);
   int longest = 1;
-  for (int g = lane; g < a.groups; g += 32) longest = max(longest, blocks_of(plan[g].pages, a.page_len));
+  if (p.own_items) {
+    for (int b = tid; b < a.batch; b += kOwnThreads) {
+      const int tok0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - tok0, pages = p.entries[group_of(a, b)].pages;
+      const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0;
+      p.entries[a.groups + b] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
+      longest = max(longest, blocks_of(len));
+    }
+  }
+  for (int g = tid; g < a.groups; g += kOwnThreads) longest = max(longest, blocks_of(p.entries[g].tokens));
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const int c = ceil_div(longest, lane + 1);
-  int items = 0;
-  for (int g = 0; g < a.groups; ++g)
-    items += tiles_of(plan[g].rows) * a.Hkv * ceil_div(blocks_of(plan[g].pages, a.page_len), c);
-  unsigned cost = 0xffffffffu;
-  if (lane == 0 || (lane < longest && items <= p.max_items)) cost = (unsigned)ceil_div(items, ctas) * (2 * c + 3);
-  const unsigned win = __reduce_min_sync(0xffffffffu, cost);
-  // equal costs: the longer ranges (fewer parts)
-  const int chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0);
-  int run = 0;
-  for (int g0 = 0; g0 < a.groups; g0 += 32) {
-    const int g = g0 + lane;
-    int n = 0, splits = 0;
-    if (g < a.groups) {
-      splits = ceil_div(blocks_of(plan[g].pages, a.page_len), chunk);
-      n = tiles_of(plan[g].rows) * a.Hkv * splits;
+  if (lane == 0) red[warp] = longest;
+  __syncthreads();
+  longest = max(max(red[0], red[1]), max(red[2], red[3]));
+  const int tries = min(kMaxSplits, longest);
+  for (int e = tid; e < entries; e += kOwnThreads) {
+    const Entry x = p.entries[e];
+    const int units = tiles_of(x.rows) * a.Hkv, nb = blocks_of(x.tokens);
+    if (units == 0 || nb == 0) continue;
+    for (int k = 0; k < tries; ++k) {
+      const int c = (longest + k) / (k + 1), full = nb / c, rest = nb - full * c;
+      atomicAdd(&sums[k], units * (full + (rest > 0)));
+      atomicAdd(&sums[32 + k], units * (full + (2 * rest >= c && rest > 0)));
     }
-    int incl = n;
+    atomicAdd(&sums[64], units * nb);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int c = (longest + lane) / (lane + 1), items = sums[lane], large = sums[32 + lane], blocks = sums[64];
+    unsigned cost = 0xffffffffu;
+    if (lane == 0 || (lane < tries && items <= p.max_items))
+      cost = (unsigned)max((2ll * blocks + 3ll * items) / p.ctas, (long long)((large + p.ctas - 1) / p.ctas) * (2 * c + 3));
+    const unsigned win = __reduce_min_sync(0xffffffffu, cost);
+    const int chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0);   // equal costs: fewer parts
+    if (lane == 0) red[4] = chunk;
+  }
+  __syncthreads();
+  const int chunk = red[4];
+  // the entries' first items, warp 0 over all entries in order
+  if (warp == 0) {
+    int run = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0, splits = 0;
+      if (e < entries) {
+        splits = (blocks_of(p.entries[e].tokens) + chunk - 1) / chunk;
+        n = tiles_of(p.entries[e].rows) * a.Hkv * splits;
+      }
+      int incl = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (e < entries) {
+        p.entries[e].splits = splits;
+        p.entries[e].first = run + incl - n;
+      }
+      run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (g < a.groups) {
-      plan[g].splits = splits;
-      plan[g].first = run + incl - n;
-      if (blockIdx.x == 0) p.plan[g] = plan[g];
+    if (lane == 0) {
+      red[5] = min(run, p.max_items);
+      *p.head = PlanHead{min(run, p.max_items), p.ctas};
     }
-    run += __shfl_sync(0xffffffffu, incl, 31);
   }
-  if (lane == 0) {
-    bars.chunk = chunk;
-    bars.total = min(run, p.max_items);
+  __syncthreads();
+  const int total = red[5];
+  for (int i = tid; i < total; i += kOwnThreads) {
+    int lo = 0, hi = entries;                           // the last entry whose first item is <= i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.entries[mid].first <= i) lo = mid;
+      else hi = mid;
+    }
+    const Entry x = p.entries[lo];
+    const int u = (i - x.first) / x.splits, split = i - x.first - u * x.splits, tiles = tiles_of(x.rows);
+    const int h = u / tiles, row0 = (u - h * tiles) * kTileRows;
+    p.items[i] = Item{x.tokens, x.prefix, min(kTileRows, x.rows - row0), x.tok0, x.table, row0, h, lo >= a.groups,
+                      split * chunk, min(blocks_of(x.tokens), (split + 1) * chunk), 0, 0};
   }
-  __syncwarp();
-  if (lane == 0) find_item(p, bars, plan, blockIdx.x, bars.first);
 }
 
+// The own columns of a request with at most 8 NR rows.  Each of the four warps takes
+// every fourth 16-token run through a ring of its own and computes
+//   S^T = K Q^T (16 tokens x 8 rows per product), O^T += V^T P^T,
+// P^T handed to the second product by movmatrix; the four warps' O, m and l are added up
+// at the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
+// in use, and the 8 columns are query rows: half the products of the plain form at 8
+// rows or fewer.
+template <int D, int NR>
+__global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParams p,
+                                                               const __grid_constant__ CUtensorMap run_map) {
+  using S = Shape<D>;
+  constexpr int kRows = 8 * NR;
+  constexpr uint32_t kStage = 2 * S::kRunBytes, kWarp = kOwnStages * kStage;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[4][kOwnStages];
+  __shared__ float2 ml[4][kRows];
+  const SharedAttnParams& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  if (lane < kOwnStages) mbar_init(&full[warp][lane], 1);
+  fence_mbar_init();
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) make_plan(p, smem);
+    return;
+  }
+  const int b = (blockIdx.x - 1) / p.own_tiles, row0 = (blockIdx.x - 1 - b * p.own_tiles) * kRows, h = blockIdx.y;
+  const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
+  if (row0 >= total_rows) return;
+  const int rows = min(kRows, total_rows - row0);
+  const int shared = group_shared_pages(a, group_of(a, b));
+  const int32_t* table = a.page_indices + a.page_indptr[b] + shared;
+  const int len = max(0, kv_tokens(a, b) - shared * a.page_len), prefix = len - n_tok;
+  const int n_runs = (len + kRun - 1) / kRun;
+  const int r0 = (int)((int64_t)n_runs * blockIdx.z / p.own_splits);
+  const int r1 = (int)((int64_t)n_runs * (blockIdx.z + 1) / p.own_splits);
+  const int mine = max(0, (r1 - r0 - warp + 3) / 4);    // this warp's runs r0 + warp + 4 i
+  const uint32_t ring = smem_u32(smem) + warp * kWarp;
+
+  // the pages of this warp's runs 32 w .. 32 w + 31, one per lane
+  auto window = [&](int w) -> int {
+    const int tok = (r0 + warp + 4 * (32 * w + lane)) * kRun;
+    const int page = 32 * w + lane < mine ? __ldg(table + p.page_of(tok)) : -1;
+    return page >= 0 && page < a.max_pages ? page : a.max_pages;     // past the pool: zero fill
+  };
+  int page_now = window(0), page_next = mine > 32 ? window(1) : 0;
+  auto load = [&](int i) {
+    if ((i & 31) == 0 && i > 0) {
+      page_now = page_next;
+      page_next = i + 32 < mine ? window((i >> 5) + 1) : 0;
+    }
+    const int page = __shfl_sync(0xffffffffu, page_now, i & 31);
+    if (lane == 0) {
+      const int tok = (r0 + warp + 4 * i) * kRun, group = (tok - p.page_of(tok) * a.page_len) / 8;
+      uint64_t* bar = &full[warp][i % kOwnStages];
+      uint8_t* dst = smem + warp * kWarp + (i % kOwnStages) * kStage;
+      mbar_arrive_expect_tx(bar, kStage);
+      tma_load_5d(dst, &run_map, bar, 0, 0, h * S::kHalves, group, 2 * page);
+      tma_load_5d(dst + S::kRunBytes, &run_map, bar, 0, 0, h * S::kHalves, group, 2 * page + 1);
+    }
+    __syncwarp();
+  };
+  int loaded = 0;
+  for (; loaded < min(kOwnStages, mine); ++loaded) load(loaded);
+
+  // Q^T as the B operand: column gq of tile n is row 8 n + gq; rows past the request's are 0
+  uint32_t qb[NR][D / 16][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = 8 * n + gq, R = row0 + r, tk = p.div_g.div(R);
+    const bool valid = r < rows;
+    const uint16_t* q =
+        (const uint16_t*)a.q + ((int64_t)(tok0 + (valid ? tk : 0)) * a.Hq + h * a.g + (valid ? R - tk * a.g : 0)) * D + 2 * tq;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      qb[n][k][0] = valid ? __ldg((const uint32_t*)(q + 16 * k)) : 0u;
+      qb[n][k][1] = valid ? __ldg((const uint32_t*)(q + 16 * k + 8)) : 0u;
+    }
+  }
+  // this lane's softmax rows: 8 n + 2 tq + {0, 1}
+  float o[NR][D / 16][4], m[NR][2], l[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.0f;
+  }
+  const int mi = lane >> 3, rr = lane & 7;
+  bool ok = true;
+  int i = 0;
+  for (; i < mine; ++i) {
+    const uint32_t kb = ring + (i % kOwnStages) * kStage, vb = kb + S::kRunBytes;
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1, p.wait_limit));
+    if (!ok) break;
+    const int c0 = (r0 + warp + 4 * i) * kRun;          // own column of the run's first token
+    float s[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t x[4];                                    // K: tokens 8 (mi & 1) + rr, dims 16 k + 8 (mi >> 1)
+      const int ch = 2 * k + (mi >> 1);
+      ldmatrix_x4(kb + (mi & 1) * S::kGroupBytes + (ch >> 3) * 1024 + rr * 128 + (((ch & 7) ^ rr) << 4), x[0], x[1], x[2],
+                  x[3]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma_m16n8k16(s[n], x, qb[n][k][0], qb[n][k][1]);
+    }
+    // element e: token gq + 8 (e >> 1), row 2 tq + (e & 1)
+    const bool masked = c0 + kRun > prefix;             // tree slots or the end in this run
+    bool grow = false;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      uint32_t seen[2] = {0xffffu, 0xffffu};
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 8 * n + 2 * tq + j, node = p.div_g.div(row0 + r);
+          seen[j] = r < rows ? (uint32_t)seen_columns(a, tok0 + node, node, c0, prefix, len) : 0u;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool see = (seen[e & 1] >> (gq + 8 * (e >> 1))) & 1u;
+        s[n][e] = see ? s[n][e] * p.scale_log2 : -INFINITY;
+        grow |= s[n][e] > m[n][e & 1] + kRescale;
+      }
+    }
+    // the subtracted max moves only when some score exceeds it by more than 2^8
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = fmaxf(s[n][j], s[n][2 + j]);
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float nm = fmaxf(m[n][j], top);
+          const float f = nm == -INFINITY ? 1.0f : fast_exp2(m[n][j] - nm);
+          m[n][j] = nm;
+          l[n][j] *= f;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            o[n][d][j] *= f;
+            o[n][d][2 + j] *= f;
+          }
+        }
+    }
+    uint32_t pb[NR][2];
+    float e[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float base = m[n][k & 1] == -INFINITY ? 0.0f : m[n][k & 1];
+        e[n][k] = fast_exp2(s[n][k] - base);
+        l[n][k & 1] += e[n][k];
+      }
+      pb[n][0] = movmatrix_trans(pack_bf16x2(e[n][0], e[n][1]));
+      pb[n][1] = movmatrix_trans(pack_bf16x2(e[n][2], e[n][3]));
+    }
+    // Values in places that no row sees, or that only some rows see, may be infinite or NaN,
+    // which 0 * v does not cancel: slots from the length on are zeroed, and a run that
+    // holds such values is added up value by value.
+    bool odd = false;
+    if (masked) {
+      for (int x = lane; x < kRun * D / 8; x += 32) {
+        const int tok = x / (D / 8), ch = x % (D / 8);
+        const uint32_t at = vb + (tok >> 3) * S::kGroupBytes + (ch >> 3) * 1024 + (tok & 7) * 128 + (((ch & 7) ^ (tok & 7)) << 4);
+        if (c0 + tok >= len) {
+          st_shared_v4(at, 0u, 0u, 0u, 0u);
+        } else {
+          const uint4 v = ld_shared_v4(at);
+          odd |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
+        }
+      }
+      odd = __any_sync(0xffffffffu, odd) && n_tok > 1;
+      __syncwarp();
+    }
+    if (!odd) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t x[4];                                  // V^T: dims 16 d + 8 (mi & 1), tokens 8 (mi >> 1) + rr
+        const int ch = 2 * d + (mi & 1);
+        ldmatrix_x4_trans(vb + (mi >> 1) * S::kGroupBytes + (ch >> 3) * 1024 + rr * 128 + (((ch & 7) ^ rr) << 4), x[0],
+                          x[1], x[2], x[3]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) mma_m16n8k16(o[n][d], x, pb[n][0], pb[n][1]);
+      }
+    } else {
+      for (int u = 0; u < kRun; ++u) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const int from = (u & 7) * 4 + tq;
+          const float p0 = __shfl_sync(0xffffffffu, u < 8 ? e[n][0] : e[n][2], from);
+          const float p1 = __shfl_sync(0xffffffffu, u < 8 ? e[n][1] : e[n][3], from);
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {      // dim 16 d + gq + 8 half
+              const int ch = 2 * d + half;
+              uint16_t w;
+              asm volatile("ld.shared.u16 %0, [%1];"
+                           : "=h"(w)
+                           : "r"(vb + (u >> 3) * S::kGroupBytes + (ch >> 3) * 1024 + (u & 7) * 128 +
+                                 (((ch & 7) ^ (u & 7)) << 4) + 2 * gq));
+              const float v = bf16_bits_to_float(w);
+              if (p0 != 0.0f) o[n][d][2 * half] = fmaf(p0, v, o[n][d][2 * half]);
+              if (p1 != 0.0f) o[n][d][2 * half + 1] = fmaf(p1, v, o[n][d][2 * half + 1]);
+            }
+        }
+      }
+    }
+    __syncwarp();
+    if (loaded < mine) load(loaded++);
+  }
+  if (!ok) {
+    if (lane == 0) give_up(p, 81);
+    for (int x = i; x < loaded; ++x) mbar_wait(&full[warp][x % kOwnStages], (x / kOwnStages) & 1);
+  }
+  __syncthreads();
+  float* os = (float*)smem;                             // [4][kRows][D + 4]
+  constexpr int kStride = D + 4;
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum = l[n][j];
+#pragma unroll
+      for (int off = 4; off <= 16; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      const int r = 8 * n + 2 * tq + j;
+      if (gq == 0) ml[warp][r] = make_float2(m[n][j], sum);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        os[(warp * kRows + r) * kStride + 16 * d + gq] = o[n][d][j];
+        os[(warp * kRows + r) * kStride + 16 * d + gq + 8] = o[n][d][2 + j];
+      }
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < rows * (D / 4); e += kOwnThreads) {
+    const int r = e / (D / 4), quad = e % (D / 4), R = row0 + r, tk = p.div_g.div(R);
+    const float M = fmaxf(fmaxf(ml[0][r].x, ml[1][r].x), fmaxf(ml[2][r].x, ml[3][r].x));
+    const float base = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(ml[w][r].x - base);
+      const float4 v = *(const float4*)(os + (w * kRows + r) * kStride + quad * 4);
+      L = fmaf(f, ml[w][r].y, L);
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    }
+    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g, part = row * p.own_splits + blockIdx.z;
+    *(float4*)(p.own_o + part * D + quad * 4) = acc;
+    if (quad == 0) p.own_ml[part] = make_float2(M, L);
+  }
+}
+
+template <int D, int NR>
+constexpr size_t own_smem() {
+  constexpr size_t ring = (size_t)4 * kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)4 * 8 * NR * (D + 4) * 4;
+  return (ring > o ? ring : o) + 1024;
+}
+
+// --------------------------------------------------------------- second kernel
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
 // every block at once: K0 V0 K1 V1 ..; two block streams start with both streams' keys:
 // K0 K1 V0 K2 V1 K3 ..
 __device__ __forceinline__ int ring_k(bool two, int i) { return two ? 2 * i : i < 2 ? i : 2 * i - 1; }
 __device__ __forceinline__ int ring_v(bool two, int i, int n) { return two ? 2 * i + 1 : i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
 
-__device__ __forceinline__ void bar_sync(int id, int count) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+// Block j of an own item holds columns that some rows do not see.
+__device__ __forceinline__ bool masked_block(const Item& it, int j) {
+  return it.own && (it.ja + j + 1) * kBlock > it.prefix;
 }
 
 template <int D>
@@ -224,20 +560,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   Bars& bars = *reinterpret_cast<Bars*>(smem + S::kOffBars);
   const SharedAttnParams& a = p.a;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  GroupPlan* plan = a.groups <= kPlanSmem ? bars.plan : p.cta_plan + (int64_t)blockIdx.x * a.groups;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars.q_ready, 8);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars.item_full[t], 1);
+      mbar_init(&bars.item_free[t], 11);                // 8 softmax warps, 2 value warps, the MMA thread
       mbar_init(&bars.s_full[t], 1);
-      mbar_init(&bars.p_full[t], 4);
+      mbar_init(&bars.p_full[t][0], 4);
+      mbar_init(&bars.p_full[t][1], 4);
     }
+    mbar_init(&bars.q_ready, 8);
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(&bars.full[s], 1);
       mbar_init(&bars.empty[s], 1);
     }
     mbar_init(&bars.o_full, 1);
     mbar_init(&bars.drain, 1);
+    bars.arrived = bars.cleaned[0] = bars.cleaned[1] = 0;
     fence_mbar_init();
     tma_prefetch_desc(&kv_map);
   }
@@ -249,15 +588,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  if (warp < 4) {
-    pdl_wait();
-    pdl_trigger();                                      // the second kernel's own part needs nothing from this one
-  }
-  if (warp == 0 || warp == 2 || warp == 3) {
-    plan_groups(p, plan, warp == 0 ? 0 : warp - 1);
-    bar_sync(1, 96);
-    if (warp == 2) plan_ranges(p, bars, plan);
-  }
+
+  // Item number k of this CTA, for the warps that do not hand it out: waits until it is
+  // there and copies it; false when there are no more (or the wait ran out).
+  auto next_item = [&](int k, Item& it) -> bool {
+    if (!mbar_wait(&bars.item_full[k & 1], (k >> 1) & 1, p.wait_limit)) {
+      give_up(p, 41);
+      return false;
+    }
+    const int i = bars.index[k & 1];
+    it = bars.items[k & 1];
+    return i >= 0;
+  };
 
   if (warp >= 4) {
     // ------------------------------------------------------------ softmax
@@ -266,18 +608,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tm = tmem + lane_base + kColS + 128 * t, o_tm = tmem + lane_base + kColO + D * t;
     bool ok = true;
-    int steps = 0, items = 0;
+    int steps = 0;
     // The first round is a rehearsal, while the plan is made: one pass of the block
     // code over whatever the TMEM holds, with nothing waited for, signalled or kept.
     // It brings the loop's instructions (some 10 KB) into the SM's caches, which cost the
-    // first real block about 5000 cycles otherwise, twice a later block's time.
-    bool rehearse = true;
+    // first real block about 3500 cycles otherwise.
     Item it;
-    it.rows = it.tokens = it.ja = it.row0 = it.h = it.tok0 = 0;
+    it.rows = it.tokens = it.ja = it.row0 = it.h = it.tok0 = it.prefix = it.own = 0;
     it.jb = 1;
-    for (int i = blockIdx.x;;) {
+    for (int k = -1;; ++k) {
+      const bool rehearse = k < 0;
+      int index = 0;
+      if (!rehearse) {
+        ok = __all_sync(0xffffffffu, next_item(k, it));
+        if (!ok) break;
+        index = bars.index[k & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.item_free[k & 1]);
+      }
       const bool two = it.rows > 128;
-      const int n = it.jb - it.ja, count = rehearse ? 1 : two ? n : (n + 1 - t) / 2;
+      const int n = it.jb - it.ja, count = two ? n : (n + 1 - t) / 2;
       const int my0 = two ? 128 * t : 0;                // this stream's first row of the tile
       if (!rehearse) {
         if (two || t == 0) {
@@ -290,17 +640,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k0 = 0; k0 < kLoads; k0 += 8) {
             uint4 v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int r = quarter * 32 + (k0 + k) * kPer + lane / kChunks, R = it.row0 + my0 + r;
+            for (int j = 0; j < 8; ++j) {
+              const int r = quarter * 32 + (k0 + j) * kPer + lane / kChunks, R = it.row0 + my0 + r;
               const int tk = p.div_g.div(R);
-              v[k] = make_uint4(0, 0, 0, 0);
-              if (my0 + r < it.rows) v[k] = __ldg((const uint4*)(q + ((int64_t)tk * a.Hq + (R - tk * a.g)) * D));
+              v[j] = make_uint4(0, 0, 0, 0);
+              if (my0 + r < it.rows) v[j] = __ldg((const uint4*)(q + ((int64_t)tk * a.Hq + (R - tk * a.g)) * D));
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int r = quarter * 32 + (k0 + k) * kPer + lane / kChunks;
-              st_shared_v4(qb + (uint32_t)r * 128u + (uint32_t)(((chunk & 7) ^ (r & 7)) << 4), v[k].x, v[k].y, v[k].z,
-                           v[k].w);
+            for (int j = 0; j < 8; ++j) {
+              const int r = quarter * 32 + (k0 + j) * kPer + lane / kChunks;
+              st_shared_v4(qb + (uint32_t)r * 128u + (uint32_t)(((chunk & 7) ^ (r & 7)) << 4), v[j].x, v[j].y, v[j].z,
+                           v[j].w);
             }
           }
           fence_proxy_async_smem();
@@ -308,6 +658,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_ready);
       }
+      const bool valid = my0 + r_local < it.rows;
+      const int node = p.div_g.div(it.row0 + my0 + r_local);
       float m = -INFINITY, l = 0.0f;
       for (int x = 0; x < count; ++x) {
         if (!rehearse) {
@@ -319,11 +671,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32_x2(s_tm, s[0]);
         tmem_ld32_x2(s_tm + 64, s[1]);
         tmem_ld_wait();
-        const int left = it.tokens - (it.ja + (two ? x : 2 * x + t)) * kBlock;
-        if (left < kBlock) {
+        const int c0 = (it.ja + (two ? x : 2 * x + t)) * kBlock;
+        if (c0 + kBlock > it.prefix) {
+          uint32_t seen[4] = {0u, 0u, 0u, 0u};
+          if (valid) {
+            const uint64_t lo = seen_columns(a, it.tok0 + node, node, c0, it.prefix, it.tokens);
+            const uint64_t hi = seen_columns(a, it.tok0 + node, node, c0 + 64, it.prefix, it.tokens);
+            seen[0] = (uint32_t)lo;
+            seen[1] = (uint32_t)(lo >> 32);
+            seen[2] = (uint32_t)hi;
+            seen[3] = (uint32_t)(hi >> 32);
+          }
 #pragma unroll
           for (int c = 0; c < kBlock; ++c)
-            if (c >= left) s[c / 64][c % 64] = __float_as_uint(-INFINITY);
+            if (!((seen[c / 32] >> (c % 32)) & 1u)) s[c / 64][c % 64] = __float_as_uint(-INFINITY);
         }
         float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
 #pragma unroll
@@ -341,9 +702,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= alpha;
           m = top;
         }
+        if (x > 0 && __any_sync(0xffffffffu, need)) {
+          // O's last update was issued before these scores, whose commit covers it
+          for (int cb = 0; cb < D / 32; ++cb) {
+            uint32_t o[32];
+            tmem_ld32(o_tm + 32 * cb, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            tmem_st32(o_tm + 32 * cb, o);
+          }
+        }
         const float sub = m == -INFINITY ? 0.0f : m;
         const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), nm2 = f2(-sub, -sub);
         uint64_t l0 = f2(0.0f, 0.0f), l1 = l0;
+        // P's two halves are handed over one by one: the first one's product runs during
+        // the second one's exponentials
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t pk[32];
@@ -358,56 +732,56 @@ __global__ void __launch_bounds__(kThreads, 1)
             pk[c / 2] = pack_bf16x2(y0, y1);
           }
           tmem_st32(s_tm + 32 * part, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (!rehearse && lane == 0) mbar_arrive(&bars.p_full[t][part]);
         }
         float a0, a1;
         f2_split(fadd2(l0, l1), a0, a1);
         l += a0 + a1;
-        if (x > 0 && __any_sync(0xffffffffu, need)) {
-          // O's last update was issued before these scores, whose commit covers it
-          for (int cb = 0; cb < D / 32; ++cb) {
-            uint32_t o[32];
-            tmem_ld32(o_tm + 32 * cb, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-            tmem_st32(o_tm + 32 * cb, o);
-          }
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (!rehearse) {
-          if (lane == 0) mbar_arrive(&bars.p_full[t]);
-          ++steps;
-        }
+        if (!rehearse) ++steps;
       }
       if (!ok) {
         if (lane == 0) give_up(p, 71);
         break;
       }
-      if (rehearse) {
-        rehearse = false;
-        pdl_wait();
-        pdl_trigger();
-        __syncthreads();                                // the plan is complete
-        if (i >= bars.total) break;
-        it = bars.first;
-        continue;
-      }
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full, items & 1, p.wait_limit));
+      if (rehearse) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full, k & 1, p.wait_limit));
       if (!ok) {
         if (lane == 0) give_up(p, 72);
         break;
       }
       tc_fence_after();
       // the part: O as [column quad][row] so that a warp stores 512 contiguous bytes
-      float* part = p.parts + (int64_t)i * S::kPartFloats + t * (S::kPartFloats / 2);
-      const bool valid = my0 + r_local < it.rows;
+      float* part = p.parts + (int64_t)index * S::kPartFloats + t * (S::kPartFloats / 2);
 #pragma unroll 1
       for (int cb = 0; cb < D / 32; ++cb) {
         uint32_t o[32];
         tmem_ld32(o_tm + 32 * cb, o);
         tmem_ld_wait();
+        if (it.own) {
+          // tree slots whose infinite or NaN values were taken out of V: the rows that
+          // see them get them
+          for (int w = 0; w < kMaxTreeWords; ++w) {
+            uint32_t bits = bars.odd[k & 3][0][w] | bars.odd[k & 3][1][w];
+            for (; bits; bits &= bits - 1) {
+              const int slot = 32 * w + __ffs(bits) - 1, col = it.prefix + slot, blk = col / kBlock;
+              if (!valid || blk < it.ja || blk >= it.jb || (!two && ((blk - it.ja) & 1) != t)) continue;
+              if (!(seen_columns(a, it.tok0 + node, node, col & ~63, it.prefix, it.tokens) >> (col & 63) & 1ull)) continue;
+              const int pg = p.page_of(col), page = a.page_indices[it.table + pg];
+              if (page < 0 || page >= a.max_pages) continue;
+              const uint16_t* v = (const uint16_t*)a.kv +
+                                  (((int64_t)page * 2 + 1) * a.page_len + (col - pg * a.page_len)) * a.Hkv * D +
+                                  (int64_t)it.h * D + 32 * cb;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const float y = bf16_bits_to_float(v[c]);
+                if (!(fabsf(y) < INFINITY)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
+              }
+            }
+          }
+        }
         if (valid) {
 #pragma unroll
           for (int qd = 0; qd < 8; ++qd)
@@ -421,149 +795,245 @@ __global__ void __launch_bounds__(kThreads, 1)
         part[128 * D + r_local] = m;
         part[128 * D + 128 + r_local] = l;
       }
-      ++items;
-      i += gridDim.x;
-      if (!find_item(p, bars, plan, i, it)) break;
     }
-  } else {
-    __syncthreads();                                    // the plan is complete
-    if (warp == 0) {
-      // ------------------------------------------------------------ TMA producer
-      // Lane r brings the r-th copy of a block.  The page of load x + 4 is fetched while
-      // load x is issued (unrolled by four, so that no register that a fetch is still
-      // filling is moved).
-      const int copies = kBlock / p.copy_tokens;
-      bool ok = true;
-      int pushed = 0;                                   // copies into the ring so far
-      Item it = bars.first;
-      for (int i = blockIdx.x; ok && i < bars.total;) {
-        const bool two = it.rows > 128;
-        const int n = it.jb - it.ja;
-        const int32_t* table = a.page_indices + it.table;
-        // the x-th load: K or V, and this lane's token of it
-        auto what = [&](int x, bool& is_v, int& tok) {
-          int j;
-          if (two) {                                    // K0 V0 K1 V1 ..
-            is_v = x & 1;
-            j = x >> 1;
-          } else if (x < min(2, n)) {                   // K0 K1 V0 K2 V1 .. , the last two V
-            is_v = false;
-            j = x;
-          } else {
-            is_v = x == 2 * n - 1 || !(x & 1);
-            j = x == 2 * n - 1 ? n - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
-          }
-          tok = (it.ja + j) * kBlock + (lane & (copies - 1)) * p.copy_tokens;
-        };
-        auto fetch = [&](int x) -> int {
-          bool is_v;
-          int tok;
-          what(x, is_v, tok);
-          return x < 2 * n && tok < it.tokens ? __ldg(table + p.page_of(tok)) : -1;
-        };
-        auto push = [&](int x, int page) {
-          bool is_v;
-          int tok;
-          what(x, is_v, tok);
-          const int s = pushed % S::kSlots;
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ((pushed / S::kSlots) + 1) & 1, p.wait_limit));
-          if (!ok) return;
-          if (page < 0 || page >= a.max_pages) page = a.max_pages;  // past the pool: zero fill
-          if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], S::kSlotBytes);
-          __syncwarp();
-          if (lane < copies)
-            tma_load_5d(smem + S::kOffRing + s * S::kSlotBytes + lane * (p.copy_tokens / 8) * S::kGroupBytes, &kv_map,
-                        &bars.full[s], 0, 0, it.h * S::kHalves, (tok - p.page_of(tok) * a.page_len) / 8,
-                        2 * page + (is_v ? 1 : 0));
-          __syncwarp();
-          ++pushed;
-        };
-        int p0 = fetch(0), p1 = fetch(1), p2 = fetch(2), p3 = fetch(3);
-        for (int x = 0; ok && x < 2 * n; x += 4) {
-          push(x, p0);
-          p0 = fetch(x + 4);
-          if (!ok || x + 1 >= 2 * n) break;
-          push(x + 1, p1);
-          p1 = fetch(x + 5);
-          if (!ok || x + 2 >= 2 * n) break;
-          push(x + 2, p2);
-          p2 = fetch(x + 6);
-          if (!ok || x + 3 >= 2 * n) break;
-          push(x + 3, p3);
-          p3 = fetch(x + 7);
-        }
-        i += gridDim.x;
-        if (!find_item(p, bars, plan, i, it)) break;
-      }
-      if (!ok && lane == 0) give_up(p, 51);
-      // the copies in flight must land before the CTA can exit
-      for (int x = max(0, pushed - S::kSlots); x < pushed; ++x)
-        mbar_wait(&bars.full[x % S::kSlots], (x / S::kSlots) & 1);
-    } else if (warp == 1) {
-      // ------------------------------------------------------------ MMA issuer, one thread
-      if (elect_one()) {
-        const uint32_t id_qk = idesc_bf16_f32(128, kBlock, 0, 0);
-        const uint32_t id_pv = idesc_bf16_f32(128, D, 0, 1);
-        // eight-token groups kGroupBytes apart, a group's halves 1 KB
-        const uint64_t q0 = smem_desc(smem_u32(smem + S::kOffQ), 16, 1024, kSwizzle128B);
-        const uint64_t k0 = smem_desc(smem_u32(smem + S::kOffRing), 16, S::kGroupBytes, kSwizzle128B);
-        const uint64_t v0 = smem_desc(smem_u32(smem + S::kOffRing), 1024, S::kGroupBytes, kSwizzle128B);
-        bool ok = true, issued = false;
-        int base = 0, items = 0, steps[2] = {0, 0};     // ring positions before this item; items and blocks done
-        auto wait = [&](uint64_t* bar, int parity, int code) {
-          ok = ok && mbar_wait(bar, parity & 1, p.wait_limit);
-          if (!ok) give_up(p, code);
-          tc_fence_after();
-          return ok;
-        };
-        Item it = bars.first;
-        for (int i = blockIdx.x; ok && i < bars.total;) {
-          const bool two = it.rows > 128;
-          const int n = it.jb - it.ja;
-          const int count[2] = {two ? n : (n + 1) / 2, two ? n : n / 2};
-          if (!wait(&bars.q_ready, items, 61)) break;
-          // step 2 x + t: O += P V of stream t's block x - 1, then S = Q K^T of its block x
-          for (int st = 0; ok && st < 2 * (count[0] + 1); ++st) {
-            const int t = st & 1, x = st >> 1;
-            if (x > count[t]) continue;
-            if (x > 0) {
-              const int pos = base + ring_v(two, two ? x - 1 : 2 * (x - 1) + t, n), slot = pos % S::kSlots;
-              if (!wait(&bars.full[slot], pos / S::kSlots, 63) || !wait(&bars.p_full[t], steps[t], 64)) break;
-              ++steps[t];
-              const uint64_t vd = v0 + (uint64_t)((slot * S::kSlotBytes) >> 4);
-#pragma unroll
-              for (int k = 0; k < kRuns; ++k)
-                mma_bf16_ts(tmem + kColO + D * t, tmem + kColS + 128 * t + 8 * k,
-                            vd + (uint64_t)((k * S::kRunBytes) >> 4), id_pv, (x > 1 || k > 0) ? 1u : 0u);
-              if (!two || t == 1) mma_commit(&bars.empty[slot]);
-            }
-            if (x < count[t]) {
-              const int pos = base + ring_k(two, two ? x : 2 * x + t), slot = pos % S::kSlots;
-              if (!wait(&bars.full[slot], pos / S::kSlots, 65)) break;
-              const uint64_t qd = q0 + (uint64_t)((two ? t * S::kSlotBytes : 0u) >> 4);
-              const uint64_t kd = k0 + (uint64_t)((slot * S::kSlotBytes) >> 4);
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k)
-                mma_bf16_ss(tmem + kColS + 128 * t, qd + (uint64_t)(((k / 4) * S::kQHalfBytes + (k % 4) * 32) >> 4),
-                            kd + (uint64_t)(((k / 4) * 1024 + (k % 4) * 32) >> 4), id_qk, k > 0);
-              mma_commit(&bars.s_full[t]);
-              if (!two || t == 1) mma_commit(&bars.empty[slot]);
-              issued = true;
-            }
-          }
-          if (ok) mma_commit(&bars.o_full);
-          base += 2 * n;
-          ++items;
-          i += gridDim.x;
-          if (!find_item(p, bars, plan, i, it)) break;
-        }
-        if (issued) {
-          mma_commit(&bars.drain);
-          mbar_wait(&bars.drain, 0);
-        }
+  } else if (warp == 0) {
+    // ------------------------------------------------------------ items and TMA producer
+    // Item k + 1 is claimed and read while item k loads.  Lane r brings the r-th copy of a
+    // block.  The page of load x + 4 is fetched while load x is issued (unrolled by four,
+    // so that no register that a fetch is still filling is moved).
+    pdl_wait();
+    pdl_trigger();
+    const int total = *(volatile int*)&p.head->total;
+    const int copies = kBlock / p.copy_tokens;
+    bool ok = true;
+    int pushed = 0, mine = blockIdx.x;                  // copies into the ring so far; this item's number
+    for (int k = 0; ok; ++k) {
+      const bool more = mine < total;
+      Item it;
+      if (more) it = p.items[mine];
+      int claim = 0;
+      if (lane == 0 && more) claim = atomicAdd(&p.head->next, 1);
+      // the slot's last item, k - 2, has been copied by everyone
+      ok = k < 2 || __all_sync(0xffffffffu, mbar_wait(&bars.item_free[k & 1], ((k >> 1) + 1) & 1, p.wait_limit));
+      if (!ok) break;
+      if (lane == 0) {
+        bars.index[k & 1] = more ? mine : -1;
+        if (more) bars.items[k & 1] = it;
+        mbar_arrive(&bars.item_full[k & 1]);
       }
       __syncwarp();
+      if (!more) break;
+      const bool two = it.rows > 128;
+      const int n = it.jb - it.ja;
+      const int32_t* table = a.page_indices + it.table;
+      // the x-th load: K or V, and this lane's token of it
+      auto what = [&](int x, bool& is_v, int& tok) {
+        int j;
+        if (two) {                                      // K0 V0 K1 V1 ..
+          is_v = x & 1;
+          j = x >> 1;
+        } else if (x < min(2, n)) {                     // K0 K1 V0 K2 V1 .. , the last two V
+          is_v = false;
+          j = x;
+        } else {
+          is_v = x == 2 * n - 1 || !(x & 1);
+          j = x == 2 * n - 1 ? n - 1 : is_v ? (x - 2) / 2 : (x + 1) / 2;
+        }
+        tok = (it.ja + j) * kBlock + (lane & (copies - 1)) * p.copy_tokens;
+      };
+      auto fetch = [&](int x) -> int {
+        bool is_v;
+        int tok;
+        what(x, is_v, tok);
+        return x < 2 * n && tok < it.tokens ? __ldg(table + p.page_of(tok)) : -1;
+      };
+      auto push = [&](int x, int page) {
+        bool is_v;
+        int tok;
+        what(x, is_v, tok);
+        const int s = pushed % S::kSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], ((pushed / S::kSlots) + 1) & 1, p.wait_limit));
+        if (!ok) return;
+        if (page < 0 || page >= a.max_pages) page = a.max_pages;    // past the pool: zero fill
+        if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], S::kSlotBytes);
+        __syncwarp();
+        if (lane < copies)
+          tma_load_5d(smem + S::kOffRing + s * S::kSlotBytes + lane * (p.copy_tokens / 8) * S::kGroupBytes, &kv_map,
+                      &bars.full[s], 0, 0, it.h * S::kHalves, (tok - p.page_of(tok) * a.page_len) / 8,
+                      2 * page + (is_v ? 1 : 0));
+        __syncwarp();
+        ++pushed;
+      };
+      int p0 = fetch(0), p1 = fetch(1), p2 = fetch(2), p3 = fetch(3);
+      for (int x = 0; ok && x < 2 * n; x += 4) {
+        push(x, p0);
+        p0 = fetch(x + 4);
+        if (!ok || x + 1 >= 2 * n) break;
+        push(x + 1, p1);
+        p1 = fetch(x + 5);
+        if (!ok || x + 2 >= 2 * n) break;
+        push(x + 2, p2);
+        p2 = fetch(x + 6);
+        if (!ok || x + 3 >= 2 * n) break;
+        push(x + 3, p3);
+        p3 = fetch(x + 7);
+      }
+      mine = __shfl_sync(0xffffffffu, claim, 0);
     }
+    if (!ok && lane == 0) give_up(p, 51);
+    // the copies in flight must land before the CTA can exit
+    for (int x = max(0, pushed - S::kSlots); x < pushed; ++x)
+      mbar_wait(&bars.full[x % S::kSlots], (x / S::kSlots) & 1);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer, one thread
+    if (elect_one()) {
+      const uint32_t id_qk = idesc_bf16_f32(128, kBlock, 0, 0);
+      const uint32_t id_pv = idesc_bf16_f32(128, D, 0, 1);
+      // eight-token groups kGroupBytes apart, a group's halves 1 KB
+      const uint64_t q0 = smem_desc(smem_u32(smem + S::kOffQ), 16, 1024, kSwizzle128B);
+      const uint64_t k0 = smem_desc(smem_u32(smem + S::kOffRing), 16, S::kGroupBytes, kSwizzle128B);
+      const uint64_t v0 = smem_desc(smem_u32(smem + S::kOffRing), 1024, S::kGroupBytes, kSwizzle128B);
+      bool ok = true, issued = false;
+      int base = 0, steps0 = 0, steps1 = 0;             // ring positions before this item; blocks done
+      int arrived = 0, passed = 0;                      // masked value blocks announced; used up
+      auto wait = [&](uint64_t* bar, int parity, int code) {
+        ok = ok && mbar_wait(bar, parity & 1, p.wait_limit);
+        if (!ok) give_up(p, code);
+        return ok;
+      };
+      Item it;
+      for (int k = 0; ok && next_item(k, it); ++k) {
+        mbar_arrive(&bars.item_free[k & 1]);
+        const bool two = it.rows > 128;
+        const int n = it.jb - it.ja;
+        const int count0 = two ? n : (n + 1) / 2, count1 = two ? n : n / 2;
+        if (!wait(&bars.q_ready, k, 61)) break;
+        // step 2 x + t: O += P V of stream t's block x - 1, then S = Q K^T of its block x
+        for (int st = 0; ok && st < 2 * (count0 + 1); ++st) {
+          const int t = st & 1, x = st >> 1, count = t ? count1 : count0;
+          if (x > count) continue;
+          const int kpos = base + ring_k(two, two ? x : 2 * x + t), kslot = kpos % S::kSlots;
+          // K of the next scores first: it is there long before P is
+          if (x < count && !wait(&bars.full[kslot], kpos / S::kSlots, 65)) break;
+          if (x > 0) {
+            const int blk = two ? x - 1 : 2 * (x - 1) + t;
+            const int pos = base + ring_v(two, blk, n), slot = pos % S::kSlots;
+            if (!wait(&bars.full[slot], pos / S::kSlots, 63)) break;
+            if (masked_block(it, blk)) {
+              // warps 2 and 3 have gone over the block's values
+              const long long since = clock64();
+              while (bars.cleaned[0] <= passed || bars.cleaned[1] <= passed)
+                if (clock64() - since > p.wait_limit) {
+                  ok = false;
+                  break;
+                }
+              if (!ok) {
+                give_up(p, 66);
+                break;
+              }
+              if (!two || t == 1) ++passed;
+            }
+            const uint64_t vd = v0 + (uint64_t)((slot * S::kSlotBytes) >> 4);
+            const int ph = (t ? steps1++ : steps0++) & 1;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              if (!wait(&bars.p_full[t][part], ph, 64)) break;
+              tc_fence_after();
+#pragma unroll
+              for (int j = part * kRuns / 2; j < (part + 1) * kRuns / 2; ++j)
+                mma_bf16_ts(tmem + kColO + D * t, tmem + kColS + 128 * t + 8 * j,
+                            vd + (uint64_t)((j * S::kRunBytes) >> 4), id_pv, (x > 1 || j > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
+            if (!two || t == 1) mma_commit(&bars.empty[slot]);
+          }
+          if (x < count) {
+            tc_fence_after();
+            const uint64_t qd = q0 + (uint64_t)((two ? t * S::kSlotBytes : 0u) >> 4);
+            const uint64_t kd = k0 + (uint64_t)((kslot * S::kSlotBytes) >> 4);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+              mma_bf16_ss(tmem + kColS + 128 * t, qd + (uint64_t)(((j / 4) * S::kQHalfBytes + (j % 4) * 32) >> 4),
+                          kd + (uint64_t)(((j / 4) * 1024 + (j % 4) * 32) >> 4), id_qk, j > 0);
+            mma_commit(&bars.s_full[t]);
+            if (!two || t == 1) mma_commit(&bars.empty[kslot]);
+            issued = true;
+            const int blk = two ? x : 2 * x + t;
+            if (masked_block(it, blk) && (!two || t == 0)) {
+              // its values come right behind the keys: warps 2 and 3 may start on them
+              const int pos = base + ring_v(two, blk, n);
+              if (!wait(&bars.full[pos % S::kSlots], pos / S::kSlots, 67)) break;
+              __threadfence_block();
+              bars.arrived = ++arrived;
+            }
+          }
+        }
+        if (ok) mma_commit(&bars.o_full);
+        base += 2 * n;
+      }
+      if (issued) {
+        mma_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ values of masked slots
+    // A masked probability is 0, and 0 * v is 0 only for finite v.  Warps 2 and 3 each go
+    // over half the tokens of an own item's masked value blocks while the scores' softmax
+    // runs: slots from the length on (the rest of a page) are zeroed, and so are infinite
+    // or NaN values of tree slots, which are noted for the rows that do see them.
+    const int half = warp - 2;
+    bool ok = true;
+    int base = 0, done = 0;                             // ring positions before this item; masked blocks so far
+    Item it;
+    for (int k = 0; ok; ++k) {
+      if (!__all_sync(0xffffffffu, next_item(k, it))) break;
+      uint32_t* odd = bars.odd[k & 3][half];
+      odd[lane] = 0u;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.item_free[k & 1]);
+      const bool two = it.rows > 128;
+      const int n = it.jb - it.ja;
+      for (int j = it.own ? max(0, max(it.prefix, 0) / kBlock - it.ja) : n; ok && j < n; ++j) {
+        const int c0 = (it.ja + j) * kBlock, pos = base + ring_v(two, j, n), slot = pos % S::kSlots;
+        // the MMA thread has seen the block arrive; it is not overwritten before this
+        // warp has passed it, so the barrier's phase is this block's
+        const long long since = clock64();
+        while (bars.arrived <= done && ok) ok = clock64() - since <= p.wait_limit;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars.full[slot], (pos / S::kSlots) & 1, p.wait_limit));
+        if (!ok) break;
+        const uint32_t vb = smem_u32(smem + S::kOffRing + slot * S::kSlotBytes);
+        const int first = max(half * 64, it.prefix - c0);         // tokens before it are the prefix
+        for (int x = first * (D / 8) + lane; x < (half + 1) * 64 * (D / 8); x += 32) {
+          const int tok = x / (D / 8), ch = x % (D / 8);
+          const uint32_t at =
+              vb + (tok >> 3) * S::kGroupBytes + (ch >> 3) * 1024 + (tok & 7) * 128 + (((ch & 7) ^ (tok & 7)) << 4);
+          if (c0 + tok >= it.tokens) {
+            st_shared_v4(at, 0u, 0u, 0u, 0u);
+          } else {
+            const uint4 v = ld_shared_v4(at);
+            const int tree = c0 + tok - it.prefix;      // causal rows past the notes keep the value as it is
+            if ((odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w)) && tree < 32 * kMaxTreeWords) {
+              auto fix = [](uint32_t w) {
+                if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+                if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+                return w;
+              };
+              st_shared_v4(at, fix(v.x), fix(v.y), fix(v.z), fix(v.w));
+              atomicOr(&odd[tree >> 5], 1u << (tree & 31));
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __threadfence_block();
+        __syncwarp();
+        ++done;
+        if (lane == 0) bars.cleaned[half] = done;
+      }
+      base += 2 * n;
+    }
+    if (!ok && lane == 0) give_up(p, 91);
   }
   tc_fence_before();
   __syncthreads();
@@ -573,452 +1043,126 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// --------------------------------------------------------------- own columns
-constexpr int kOwnThreads = 128;
-constexpr int kOwnTile = 32;              // tokens staged at a time
-constexpr int kOwnStages = 3;
-constexpr int kMaxOwnSplits = 32;
+// ---------------------------------------------------------------- third kernel
+// A CTA joins 16 rows of a request and KV head: the parts of its group's shared columns,
+// and those of its own.  First every part's m and l come in at once, then a thread per
+// row turns them into weights e^(m - M) / L, then each thread sums one column quad of one
+// row: four rows and eight quads per warp, so that both the parts ([quad][row]) and the
+// output are touched in 64-byte pieces.
+constexpr int kJoinRows = 16;
+constexpr int kMaxParts = 4 * kMaxSplits;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;                         // 0: the 16 bytes are zeroed
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
-
-// Which of own columns c0 .. c0 + 63 row `node` sees (bit i: column c0 + i): those
-// before `prefix`, then tree slots by the row's mask, or up to its own without masks.
-__device__ __forceinline__ uint64_t seen_columns(const SharedAttnParams& a, const uint64_t* mask, int node, int c0,
-                                                 int prefix, int len) {
-  uint64_t v = low_bits(min(prefix, len) - c0);
-  const int first = max(prefix, c0);                    // first tree column of the 64
-  if (first < min(len, c0 + 64)) {
-    const int slot = first - prefix;
-    uint64_t bits;
-    if (!a.mask_bits) {
-      bits = low_bits(node - slot + 1);
-    } else {
-      const int w = slot >> 6, sh = slot & 63;
-      const uint64_t lo = w < a.mask_words ? __ldg(mask + w) : 0ull;
-      const uint64_t hi = sh && w + 1 < a.mask_words ? __ldg(mask + w + 1) : 0ull;
-      bits = sh ? (lo >> sh) | (hi << (64 - sh)) : lo;
-    }
-    v |= (bits & low_bits(min(len, c0 + 64) - first)) << (first - c0);
-  }
-  return v;
-}
-
-// Joins rows 0 .. n - 1 (request rows row0 ..) of request b and KV head h: their own
-// parts, and the shared parts of their group.  Own part k of row r: O at own_o + k *
-// o_part + r * o_row, (m, l) at own_ml + k * ml_part + r * ml_row.  `w` and `lw` hold
-// [kMaxParts][ROWS] floats.  First every part's m and l come in at once, then a thread
-// per row turns them into weights e^(m - M) / L, then each thread sums one column quad of
-// one row: four rows and eight quads per warp, so that both the parts ([quad][row]) and
-// the output are touched in 64-byte pieces.
-constexpr int kMaxParts = 2 * kMaxSplits + kMaxOwnSplits;
-
-template <int D, int ROWS>
-__device__ __forceinline__ void join_rows(const PrefixParams& p, const GroupPlan& g, int gi, int b, int h, int row0,
-                                          int n, const float* own_o, int64_t o_part, int64_t o_row,
-                                          const float2* own_ml, int64_t ml_part, int64_t ml_row, int own_parts,
-                                          float* w, float* lw) {
+template <int D>
+__global__ void __launch_bounds__(128) join_parts_kernel(const PrefixParams p, int row_tiles) {
   const SharedAttnParams& a = p.a;
   constexpr int kPart = Shape<D>::kPartFloats, kHalf = kPart / 2;
-  const int tok0 = a.qo_indptr[b];
-  const int in_group = (tok0 - a.qo_indptr[a.group_indptr[gi]]) * a.g + row0;
-  const int tiles = (g.rows + kTileRows - 1) / kTileRows;
-  // row r's shared part k: stream k & 1 of range k / 2 where two block streams shared
-  // the rows, else its row half's stream of range k
-  const float* first = p.parts + ((int64_t)g.first + (int64_t)h * tiles * g.splits) * kPart;
-  auto part_of = [&](int r, int k, int& shared) -> const float* {
-    const int rg = in_group + r, tile = rg / kTileRows, in = rg % kTileRows;
-    const bool two = g.rows - tile * kTileRows > 128;
-    shared = two ? g.splits : 2 * g.splits;
-    return first + (int64_t)tile * g.splits * kPart + (two ? (int64_t)k * kPart + (in >> 7) * kHalf : (int64_t)k * kHalf) +
-           (in & 127) * 4;
-  };
-  const int most = 2 * g.splits + own_parts;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < most * ROWS; e += kOwnThreads) {
-    const int k = e / ROWS, r = e % ROWS;
-    float m = -INFINITY, l = 0.0f;
-    if (r < n) {
-      int shared;
-      const float* s = part_of(r, k, shared);
-      if (k < shared) {
-        const float* ml = s - ((in_group + r) % 128) * 4 + 128 * D + (in_group + r) % 128;
-        m = __ldcg(ml);
-        l = __ldcg(ml + 128);
-      } else if (k - shared < own_parts) {
-        const float2 x = own_ml[(k - shared) * ml_part + r * ml_row];
-        m = x.x;
-        l = x.y;
-      }
+  __shared__ float w[kMaxParts][kJoinRows], lw[kMaxParts][kJoinRows];
+  __shared__ const float* src[2][kJoinRows];            // first part's O of the shared and the own columns
+  __shared__ int64_t step[2][kJoinRows];                // floats from part to part
+  __shared__ int cnt[2][kJoinRows];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / row_tiles, row0 = (blockIdx.x - b * row_tiles) * kJoinRows, h = blockIdx.y;
+  const int tok0 = a.qo_indptr[b], total_rows = (a.qo_indptr[b + 1] - tok0) * a.g;
+  if (row0 >= total_rows) return;
+  const int n = min(kJoinRows, total_rows - row0);
+  // where the parts of row R are: thread (set, row).  A stored part is [quad][128 rows] with
+  // m and l behind, two streams per item; the first kernel's are [quad] with (m, l) apart.
+  if (threadIdx.x < 2 * kJoinRows) {
+    const int set = threadIdx.x / kJoinRows, r = threadIdx.x % kJoinRows, R = row0 + r;
+    if (set == 1 && !p.own_items) {
+      const int tk = p.div_g.div(R);
+      const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g;
+      src[1][r] = p.own_o + row * p.own_splits * D;
+      step[1][r] = D;
+      cnt[1][r] = r < n ? p.own_splits : 0;
+    } else {
+      const Entry e = p.entries[set == 0 ? group_of(a, b) : a.groups + b];
+      const int in_entry = (tok0 - e.tok0) * a.g + R, tile = in_entry / kTileRows, in = in_entry % kTileRows;
+      const bool two = e.rows - tile * kTileRows > 128;
+      src[set][r] = p.parts + ((int64_t)e.first + ((int64_t)h * tiles_of(e.rows) + tile) * e.splits) * kPart +
+                    (two ? (in >> 7) * kHalf : 0) + (in & 127) * 4;
+      step[set][r] = two ? kPart : kHalf;
+      cnt[set][r] = r < n ? (two ? e.splits : 2 * e.splits) : 0;
     }
-    w[e] = m;
-    lw[e] = l;
   }
   __syncthreads();
-  for (int r = threadIdx.x; r < ROWS; r += kOwnThreads) {
+  const int most = max(cnt[0][0], cnt[0][n - 1]) + max(cnt[1][0], cnt[1][n - 1]);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < most * kJoinRows; e += 128) {
+    const int r = e % kJoinRows, k = e / kJoinRows, shared = cnt[0][r];
+    float m = -INFINITY, l = 0.0f;
+    if (k < shared + cnt[1][r]) {
+      const int set = k >= shared, i = set ? k - shared : k;
+      if (set && !p.own_items) {
+        const float2 x = __ldcg(p.own_ml + (src[1][r] - p.own_o) / D + i);
+        m = x.x;
+        l = x.y;
+      } else {
+        // (row & 127) * 4 floats into the part: m is 128 D + row & 127 floats in
+        const int64_t at = (src[set][r] - p.parts) % kHalf;
+        const float* part = src[set][r] - at + i * step[set][r];
+        m = __ldcg(part + 128 * D + at / 4);
+        l = __ldcg(part + 128 * D + 128 + at / 4);
+      }
+    }
+    w[k][r] = m;
+    lw[k][r] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < kJoinRows) {
+    const int r = threadIdx.x;
     float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < most; ++k) M = fmaxf(M, w[k * ROWS + r]);
+    for (int k = 0; k < most; ++k) M = fmaxf(M, w[k][r]);
     const float base = M == -INFINITY ? 0.0f : M;
     for (int k = 0; k < most; ++k) {
-      const float x = fast_exp2(w[k * ROWS + r] - base);
-      L = fmaf(x, lw[k * ROWS + r], L);
-      w[k * ROWS + r] = x;
+      const float x = fast_exp2(w[k][r] - base);
+      L = fmaf(x, lw[k][r], L);
+      w[k][r] = x;
     }
-    lw[r] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;    // nothing seen: 0
+    lw[0][r] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L; // nothing seen: 0
   }
   __syncthreads();
   const int units = (n + 3) / 4 * D;
-  for (int idx = threadIdx.x; idx < units; idx += kOwnThreads) {
+  for (int idx = threadIdx.x; idx < units; idx += 128) {
     const int lo = idx & 31, hi = idx >> 5;
     const int r = (hi / (D / 32)) * 4 + (lo & 3), quad = (hi % (D / 32)) * 8 + (lo >> 2);
     if (r >= n) continue;
     float o0 = 0.0f, o1 = 0.0f, o2 = 0.0f, o3 = 0.0f;
-    int shared;
-    const float* s = part_of(r, 0, shared) + quad * 512;
-    const int64_t step = shared == g.splits ? kPart : kHalf;
-    for (int k0 = 0; k0 < shared; k0 += 8) {
-      float4 v[8];                                      // eight loads in flight
+    int k = 0;
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (k0 + u < shared) v[u] = __ldcg((const float4*)(s + (k0 + u) * step));
+    for (int set = 0; set < 2; ++set) {
+      const float* s = src[set][r] + (set && !p.own_items ? quad * 4 : quad * 512);
+      const int64_t d = step[set][r];
+      const int c = cnt[set][r];
+      for (int k0 = 0; k0 < c; k0 += 8) {
+        float4 v[8];                                    // eight loads in flight
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float x = k0 + u < shared ? w[(k0 + u) * ROWS + r] : 0.0f;
-        if (x != 0.0f) {                                // a part of no columns has no O
-          o0 = fmaf(x, v[u].x, o0);
-          o1 = fmaf(x, v[u].y, o1);
-          o2 = fmaf(x, v[u].z, o2);
-          o3 = fmaf(x, v[u].w, o3);
+        for (int u = 0; u < 8; ++u)
+          if (k0 + u < c) v[u] = __ldcg((const float4*)(s + (k0 + u) * d));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float x = k0 + u < c ? w[k + k0 + u][r] : 0.0f;
+          if (x != 0.0f) {                              // a part of no columns has no O
+            o0 = fmaf(x, v[u].x, o0);
+            o1 = fmaf(x, v[u].y, o1);
+            o2 = fmaf(x, v[u].z, o2);
+            o3 = fmaf(x, v[u].w, o3);
+          }
         }
       }
+      k += c;
     }
-#pragma unroll 2
-    for (int k = 0; k < own_parts; ++k) {
-      const float x = w[(shared + k) * ROWS + r];
-      if (x != 0.0f) {
-        const float4 v = *(const float4*)(own_o + k * o_part + r * o_row + quad * 4);
-        o0 = fmaf(x, v.x, o0);
-        o1 = fmaf(x, v.y, o1);
-        o2 = fmaf(x, v.z, o2);
-        o3 = fmaf(x, v.w, o3);
-      }
-    }
-    const float inv = lw[r];
+    const float inv = lw[0][r];
     const int R = row0 + r, tk = p.div_g.div(R);
     *(uint2*)((uint16_t*)a.out + ((int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g) * D + quad * 4) =
         make_uint2(pack_bf16x2(o0 * inv, o1 * inv), pack_bf16x2(o2 * inv, o3 * inv));
   }
 }
 
-// Shared memory of own_attn_kernel: the stages, or O and the weights of the join.
-template <int D, int WR>
-constexpr size_t own_smem() {
-  constexpr int WT = WR == 1 ? 2 : 1, kRows = 16 * WR;
-  constexpr size_t stages = (size_t)kOwnStages * 2 * kOwnTile * D * 2;
-  constexpr size_t join = ((size_t)WT * kRows * D + 2 * (2 * kMaxSplits + WT) * kRows) * 4;
-  return stages > join ? stages : join;
-}
-
-// 16 WR rows of a request per CTA.  The four warps are WR row groups x WT token groups x
-// WD halves of the output dimensions: with few rows the tokens and dimensions are split
-// instead (the scores are then computed twice, which costs nothing next to the loads),
-// so that a thread's O stays at 32 registers and four CTAs fit an SM.
-template <int D, int WR>
-__global__ void __launch_bounds__(kOwnThreads, WR == 4 ? 3 : 4) own_attn_kernel(const PrefixParams p) {
-  constexpr int WD = WR == 4 ? 1 : 2, WT = 4 / (WR * WD), kRows = 16 * WR, kChunks = D / 8, kRowBytes = D * 2;
-  constexpr int NC = kOwnTile / WT / 16;                // 16-token chunks of a warp
-  constexpr int DW = D / WD;                            // its output dimensions
-  constexpr uint32_t kTileBytes = kOwnTile * kRowBytes; // K or V
-  extern __shared__ __align__(16) uint8_t stage[];
-  __shared__ float2 ml[WT][kRows];
-  const SharedAttnParams& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  const int wr = warp % WR, wt = warp / WR % WT, wd = warp / (WR * WT);
-  const int b = blockIdx.x / p.request_tiles, row0 = (blockIdx.x - b * p.request_tiles) * kRows, h = blockIdx.y;
-  const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
-  pdl_trigger();
-  if (row0 >= total_rows) {
-    pdl_wait();                                         // no CTA ends before the first kernel has: what follows may
-    return;                                             // wait for this one alone
-  }
-  const int rows = min(kRows, total_rows - row0);
-  const int gi = group_of(a, b);
-  const int shared = group_shared_pages(a, gi);
-  const int32_t* table = a.page_indices + a.page_indptr[b] + shared;
-  const int len = max(0, kv_tokens(a, b) - shared * a.page_len), prefix = len - n_tok;
-  const int n_tiles = (len + kOwnTile - 1) / kOwnTile;
-  const int j0 = (int)((int64_t)n_tiles * blockIdx.z / p.own_splits);
-  const int j1 = (int)((int64_t)n_tiles * (blockIdx.z + 1) / p.own_splits);
-  const uint32_t smem0 = smem_u32(stage);
-  const int64_t tok_elems = (int64_t)a.Hkv * D;
-  const uint16_t* kv = (const uint16_t*)a.kv + (int64_t)h * D;
-
-  // Where 16-token runs 32 w .. 32 w + 31 start (lane i: run 32 w + i), in elements of the
-  // pool's head h; -1: not in the pool.
-  auto window = [&](int w) -> int64_t {
-    const int tok = (32 * w + lane) * 16;
-    if (tok >= len) return -1;
-    const int pg = p.page_of(tok), page = __ldg(table + pg);
-    if (page < 0 || page >= a.max_pages) return -1;
-    return ((int64_t)page * 2 * a.page_len + (tok - pg * a.page_len)) * tok_elems;
-  };
-  constexpr int kTilesPerWindow = 32 * 16 / kOwnTile;
-  int win = j0 / kTilesPerWindow;
-  int64_t at = window(win), at_next = window(win + 1);
-  auto load_tile = [&](int j) {
-    if (j / kTilesPerWindow != win) {
-      ++win;
-      at = at_next;
-      at_next = window(win + 1);
-    }
-    const uint32_t buf = smem0 + (j % kOwnStages) * 2 * kTileBytes;
-#pragma unroll
-    for (int e0 = 0; e0 < kOwnTile * kChunks; e0 += kOwnThreads) {
-      const int e = e0 + threadIdx.x, t = e / kChunks, c = e % kChunks;
-      const int64_t run = __shfl_sync(0xffffffffu, at, (j * (kOwnTile / 16) + t / 16) & 31);
-      const bool valid = run >= 0 && j * kOwnTile + t < len;
-      const uint16_t* src = valid ? kv + run + (t & 15) * tok_elems + c * 8 : kv;
-      const uint32_t dst = buf + t * kRowBytes + ((c ^ (t & 7)) << 4);
-      cp_async16(dst, src, valid);
-      cp_async16(dst + kTileBytes, valid ? src + a.page_len * tok_elems : src, valid);
-    }
-    cp_async_commit();
-  };
-  static_assert(kOwnThreads / kChunks <= 16, "the lanes of a warp load one run at a time");
-
-  for (int s = 0; s < kOwnStages - 1; ++s) {
-    if (j0 + s < j1) load_tile(j0 + s);
-    else cp_async_commit();
-  }
-  // the warp's 16 query rows as A fragments; rows past the request's are zero
-  uint32_t qa[D / 16][4];
-  int node[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = wr * 16 + gq + 8 * i, R = row0 + r;
-    const bool valid = r < rows;
-    node[i] = valid ? p.div_g.div(R) : 0;
-    const uint16_t* q =
-        (const uint16_t*)a.q + ((int64_t)(tok0 + node[i]) * a.Hq + h * a.g + (valid ? R - node[i] * a.g : 0)) * D + 2 * tq;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      qa[k][i] = valid ? __ldg((const uint32_t*)(q + 16 * k)) : 0u;
-      qa[k][2 + i] = valid ? __ldg((const uint32_t*)(q + 16 * k + 8)) : 0u;
-    }
-  }
-  float o[DW / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < DW / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  const int mi = lane >> 3, rr = lane & 7;
-
-  for (int j = j0; j < j1; ++j) {
-    if (j + kOwnStages - 1 < j1) load_tile(j + kOwnStages - 1);
-    else cp_async_commit();
-    cp_async_wait<kOwnStages - 1>();
-    __syncthreads();
-    const uint32_t kb = smem0 + (j % kOwnStages) * 2 * kTileBytes, vb = kb + kTileBytes;
-    const int c0 = j * kOwnTile, t0 = wt * (kOwnTile / WT);
-    float s[NC][2][4];
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[c][e >> 2][e & 3] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int t = t0 + 16 * c + rr + 8 * (mi >> 1);
-        uint32_t r0, r1, r2, r3;
-        ldmatrix_x4(kb + t * kRowBytes + (((2 * k + (mi & 1)) ^ (t & 7)) << 4), r0, r1, r2, r3);
-        mma_m16n8k16(s[c][0], qa[k], r0, r1);
-        mma_m16n8k16(s[c][1], qa[k], r2, r3);
-      }
-    const bool masked = c0 + kOwnTile > prefix;         // tree slots or the end in this tile
-    uint32_t seen[2] = {~0u, ~0u};
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        seen[i] = seen_columns(a, a.mask_bits ? a.mask_bits + (int64_t)(tok0 + node[i]) * a.mask_words : nullptr,
-                               node[i], c0, prefix, len);
-    }
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& x = s[c][e >> 2][e & 3];
-        const int i = (e >> 1) & 1, col = t0 + 16 * c + 8 * (e >> 2) + 2 * tq + (e & 1);
-        x = (seen[i] >> col) & 1u ? x * p.scale_log2 : -INFINITY;
-        top[i] = fmaxf(top[i], x);
-      }
-    float keep[2], sub[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      const float nm = fmaxf(m[i], top[i]);
-      sub[i] = nm == -INFINITY ? 0.0f : nm;
-      keep[i] = fast_exp2(m[i] - sub[i]);
-      m[i] = nm;
-      l[i] *= keep[i];
-    }
-#pragma unroll
-    for (int i = 0; i < DW / 8; ++i) {
-      o[i][0] *= keep[0];
-      o[i][1] *= keep[0];
-      o[i][2] *= keep[1];
-      o[i][3] *= keep[1];
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& x = s[c][e >> 2][e & 3];
-        x = fast_exp2(x - sub[(e >> 1) & 1]);
-        l[(e >> 1) & 1] += x;
-      }
-    // Values that 0 * v does not cancel, in a tile where rows see different slots: only
-    // the rows that see them may take them.
-    bool odd = false;
-    if (masked && n_tok > 1) {
-      for (int e = threadIdx.x; e < kOwnTile * kChunks; e += kOwnThreads) {
-        const uint4 v = ld_shared_v4(vb + e * 16);
-        auto bad = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
-        odd |= bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
-      }
-      odd = __syncthreads_or(odd);
-    }
-    if (!odd) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const uint32_t pa[4] = {pack_bf16x2(s[c][0][0], s[c][0][1]), pack_bf16x2(s[c][0][2], s[c][0][3]),
-                                pack_bf16x2(s[c][1][0], s[c][1][1]), pack_bf16x2(s[c][1][2], s[c][1][3])};
-#pragma unroll
-        for (int d = 0; d < DW / 16; ++d) {
-          const int t = t0 + 16 * c + rr + 8 * (mi & 1), ch = wd * (DW / 8) + 2 * d + (mi >> 1);
-          uint32_t r0, r1, r2, r3;
-          ldmatrix_x4_trans(vb + t * kRowBytes + ((ch ^ (t & 7)) << 4), r0, r1, r2, r3);
-          mma_m16n8k16(o[2 * d], pa, r0, r1);
-          mma_m16n8k16(o[2 * d + 1], pa, r2, r3);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int u = 0; u < 16; ++u) {                  // token u of the 16: its lane of the quad, its element
-          const float p0 = __shfl_sync(0xffffffffu, s[c][u >> 3][u & 1], (lane & ~3) | ((u & 7) >> 1));
-          const float p1 = __shfl_sync(0xffffffffu, s[c][u >> 3][2 + (u & 1)], (lane & ~3) | ((u & 7) >> 1));
-          const int t = t0 + 16 * c + u;
-#pragma unroll
-          for (int d = 0; d < DW / 8; ++d) {
-            uint32_t w;
-            asm volatile("ld.shared.b32 %0, [%1];"
-                         : "=r"(w)
-                         : "r"(vb + t * kRowBytes + (((wd * (DW / 8) + d) ^ (t & 7)) << 4) + 4 * tq));
-            const float v0 = bf16_bits_to_float(w & 0xffffu), v1 = bf16_bits_to_float(w >> 16);
-            if (p0 != 0.0f) {
-              o[d][0] = fmaf(p0, v0, o[d][0]);
-              o[d][1] = fmaf(p0, v1, o[d][1]);
-            }
-            if (p1 != 0.0f) {
-              o[d][2] = fmaf(p1, v0, o[d][2]);
-              o[d][3] = fmaf(p1, v1, o[d][3]);
-            }
-          }
-        }
-    }
-    __syncthreads();                                    // the stage may be loaded again
-  }
-  cp_async_wait<0>();
-  __syncthreads();
-  float* os = (float*)stage;                            // [WT][rows][D]
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    const int r = wr * 16 + gq + 8 * i;
-    if (tq == 0 && wd == 0) ml[wt][r] = make_float2(m[i], l[i]);
-#pragma unroll
-    for (int d = 0; d < DW / 8; ++d)
-      *(float2*)(os + (wt * kRows + r) * D + wd * DW + 8 * d + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-  }
-  __syncthreads();
-  if (p.own_splits > 1) {
-    // a slice of the own columns: one part per row for the join kernel
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kOwnThreads) {
-      const int r = e / (D / 4), quad = e % (D / 4), R = row0 + r, tk = p.div_g.div(R);
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WT; ++w) M = fmaxf(M, ml[w][r].x);
-      const float sub = M == -INFINITY ? 0.0f : M;
-      float L = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < WT; ++w) {
-        const float f = fast_exp2(ml[w][r].x - sub);
-        if (f == 0.0f) continue;
-        const float4 v = *(const float4*)(os + (w * kRows + r) * D + quad * 4);
-        L = fmaf(f, ml[w][r].y, L);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
-      }
-      const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g, part = row * p.own_splits + blockIdx.z;
-      *(float4*)(p.own_o + part * D + quad * 4) = acc;
-      if (quad == 0) p.own_ml[part] = make_float2(M, L);
-    }
-    pdl_wait();
-    return;
-  }
-  // the weights go behind O in the stage
-  constexpr int kOFloats = WT * kRows * D, kWeights = (2 * kMaxSplits + WT) * kRows;
-  static_assert((kOFloats + 2 * kWeights) * 4 <= own_smem<D, WR>(), "the join's arrays");
-  pdl_wait();                                           // the shared parts are complete
-  join_rows<D, kRows>(p, p.plan[gi], gi, b, h, row0, rows, os, kRows * D, D, &ml[0][0], kRows, 1, WT, os + kOFloats,
-                      os + kOFloats + kWeights);
-}
-
-// After own_attn_kernel with several slices: one CTA per (request row, KV head) joins a
-// token's heads.
-template <int D>
-__global__ void __launch_bounds__(kOwnThreads) join_parts_kernel(const PrefixParams p) {
-  const SharedAttnParams& a = p.a;
-  constexpr int kRows = 16;
-  __shared__ float w[kMaxParts * kRows], lw[kMaxParts * kRows];
-  pdl_trigger();
-  pdl_wait();
-  const int tok = blockIdx.x, h = blockIdx.y;
-  if (tok >= a.qo_indptr[a.batch]) return;
-  int lo = 0, hi = a.batch;                             // the request of the token
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.qo_indptr[mid] <= tok) lo = mid;
-    else hi = mid;
-  }
-  const int gi = group_of(a, lo), node = tok - a.qo_indptr[lo];
-  for (int r0 = 0; r0 < a.g; r0 += kRows) {
-    const int64_t row = (int64_t)tok * a.Hq + h * a.g + r0;
-    join_rows<D, kRows>(p, p.plan[gi], gi, lo, h, node * a.g + r0, min(kRows, a.g - r0), p.own_o + row * p.own_splits * D,
-                        D, (int64_t)p.own_splits * D, p.own_ml + row * p.own_splits, 1, p.own_splits, p.own_splits, w,
-                        lw);
-    __syncthreads();
-  }
-}
-
 struct PrefixPlan {
-  int own_rows, request_tiles, own_splits, max_items, ctas;
-  size_t plan, cta_plan, parts, own_ml, own_o, bytes;
+  int few, own_rows, own_tiles, own_splits, max_items, ctas;
+  size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
 int sm_count() {
@@ -1036,17 +1180,19 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   PrefixPlan f;
   const int g = Hq / Hkv;
   const int64_t rows = (int64_t)max_qo_len * g;
-  f.own_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  f.request_tiles = (int)((rows + f.own_rows - 1) / f.own_rows);
+  f.few = rows <= kFewRows;
+  f.own_rows = rows <= 8 ? 8 : 16;
+  f.own_tiles = f.few ? 1 : 0;
   f.ctas = sm_count();
-  // own columns: about four CTAs per SM, each with four tiles at least
-  const int64_t ctas = (int64_t)batch * f.request_tiles * Hkv;
+  // own columns in the first kernel: about three CTAs per SM, each warp with two runs at least
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
-  f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({4ll * f.ctas / std::max<int64_t>(ctas, 1),
-                                                              (own + 4 * kOwnTile - 1) / (4 * kOwnTile),
-                                                              kMaxOwnSplits}));
-  const int64_t units = (((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups) * Hkv;
-  f.max_items = (int)std::min<int64_t>(units + 2 * f.ctas, 1 << 30);
+  f.own_splits = 1;
+  if (f.few)
+    f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({3ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
+                                                                (own + 8 * kRun - 1) / (8 * kRun), kMaxOwnSplits}));
+  int64_t units = ((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups;
+  if (!f.few) units += ((int64_t)total_q * g + kTileRows - 1) / kTileRows + batch;
+  f.max_items = (int)std::min<int64_t>(units * Hkv + 2 * f.ctas, 1 << 28);
   const int part = D == 128 ? Shape<128>::kPartFloats : Shape<64>::kPartFloats;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -1054,42 +1200,48 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
     at = align_up(at + n, 256);
     return o;
   };
-  f.plan = take(sizeof(GroupPlan) * groups);
-  f.cta_plan = take(groups > kPlanSmem ? sizeof(GroupPlan) * groups * f.ctas : 0);
+  f.head = take(sizeof(PlanHead));
+  f.entries = take(sizeof(Entry) * (groups + (f.few ? 0 : batch)));
+  f.items = take(sizeof(Item) * f.max_items);
   f.parts = take((size_t)f.max_items * part * sizeof(float));
-  const size_t own_parts = f.own_splits > 1 ? (size_t)total_q * Hq * f.own_splits : 0;
+  const size_t own_parts = f.few ? (size_t)total_q * Hq * f.own_splits : 0;
   f.own_ml = take(own_parts * sizeof(float2));
   f.own_o = take(own_parts * D * sizeof(float));
   f.bytes = at;
   return f;
 }
 
-template <int D, int WR>
-int launch_own(const PrefixParams& p, cudaStream_t stream) {
-  constexpr size_t smem = own_smem<D, WR>();
-  if (int rc = ensure_smem_attr((const void*)own_attn_kernel<D, WR>, smem)) return rc;
-  PTS_CUDA_TRY(launch_pdl(own_attn_kernel<D, WR>, dim3(p.a.batch * p.request_tiles, p.a.Hkv, p.own_splits),
-                          dim3(kOwnThreads), smem, stream, p));
-  return launch_status("own_attn_kernel");
-}
-
 template <int D>
-int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int total_q, cudaStream_t stream) {
-  const SharedAttnParams& a = p.a;
-  CUtensorMap map;
+int encode_kv(CUtensorMap* map, const SharedAttnParams& a, int copy_tokens) {
   // (dim of a half, token of a group, head and half, group, 2 page + K/V)
   const cuuint64_t tok = (cuuint64_t)a.Hkv * D * 2;
   const cuuint64_t dims[5] = {64, 8, (cuuint64_t)a.Hkv * (D / 64), (cuuint64_t)a.page_len / 8, (cuuint64_t)a.max_pages * 2};
   const cuuint64_t strides[4] = {tok, 128, 8 * tok, a.page_len * tok};
-  const cuuint32_t box[5] = {64, 8, D / 64, (cuuint32_t)p.copy_tokens / 8, 1};
-  if (int rc = encode_tiled_bf16_sw128(&map, 5, a.kv, dims, strides, box)) return rc;
+  const cuuint32_t box[5] = {64, 8, D / 64, (cuuint32_t)copy_tokens / 8, 1};
+  return encode_tiled_bf16_sw128(map, 5, a.kv, dims, strides, box);
+}
+
+template <int D, int NR>
+int launch_own(const PrefixParams& p, int few, const CUtensorMap& map, cudaStream_t stream) {
+  constexpr size_t smem = own_smem<D, NR>();
+  if (int rc = ensure_smem_attr((const void*)plan_own_kernel<D, NR>, smem)) return rc;
+  const dim3 grid = few ? dim3(1 + p.a.batch * p.own_tiles, p.a.Hkv, p.own_splits) : dim3(1);
+  PTS_CUDA_TRY(launch_pdl(plan_own_kernel<D, NR>, grid, dim3(kOwnThreads), smem, stream, p, map));
+  return launch_status("plan_own_kernel");
+}
+
+template <int D>
+int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cudaStream_t stream) {
+  CUtensorMap run_map, block_map;
+  if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
+  if (int rc = encode_kv<D>(&block_map, p.a, p.copy_tokens)) return rc;
+  if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, f.few, run_map, stream) : launch_own<D, 2>(p, f.few, run_map, stream))
+    return rc;
   if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem)) return rc;
-  PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, map));
+  PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
   if (int rc = launch_status("prefix_attn_kernel")) return rc;
-  int rc = f.own_rows == 16 ? launch_own<D, 1>(p, stream) : f.own_rows == 32 ? launch_own<D, 2>(p, stream)
-                                                                            : launch_own<D, 4>(p, stream);
-  if (rc || p.own_splits == 1) return rc;
-  PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(total_q, a.Hkv), dim3(kOwnThreads), 0, stream, p));
+  const int row_tiles = (int)(((int64_t)max_qo_len * p.a.g + kJoinRows - 1) / kJoinRows);
+  PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(128), 0, stream, p, row_tiles));
   return launch_status("join_parts_kernel");
 }
 
@@ -1107,7 +1259,7 @@ size_t prefix_attn_workspace(int batch, int groups, int total_q, int max_qo_len,
 int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, int max_kv_len, int max_own_len,
                        void* workspace, int32_t* error, cudaStream_t stream) {
   const PrefixPlan f = plan_prefix(a.batch, a.groups, total_q, max_qo_len, max_kv_len, max_own_len, a.Hq, a.Hkv, a.D);
-  if ((int64_t)a.batch * ((int64_t)max_qo_len * a.g / 16 + 1) > 2147483647ll)
+  if ((int64_t)a.batch * ((int64_t)max_qo_len * a.g / kJoinRows + 1) > 2147483647ll)
     return set_error(PTS_ERR_CAPACITY, "grid too large");
   if ((int64_t)total_q * a.g * a.g > 0xffffffffll)
     return set_error(PTS_ERR_CAPACITY, "%d query rows are too many", total_q);
@@ -1121,17 +1273,20 @@ int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, i
   for (int s = 0; s < 31; ++s)
     if (a.page_len == 1 << s) p.page_shift = s;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.max_items = f.max_items;
-  p.parts = (float*)(ws + f.parts);
-  p.plan = (GroupPlan*)(ws + f.plan);
-  p.cta_plan = (GroupPlan*)(ws + f.cta_plan);
   p.error = error;
   p.wait_limit = wait_limit_cycles();
+  p.ctas = f.ctas;
+  p.max_items = f.max_items;
+  p.own_items = !f.few;
+  p.head = (PlanHead*)(ws + f.head);
+  p.entries = (Entry*)(ws + f.entries);
+  p.items = (Item*)(ws + f.items);
+  p.parts = (float*)(ws + f.parts);
+  p.own_tiles = f.own_tiles;
   p.own_splits = f.own_splits;
-  p.request_tiles = f.request_tiles;
   p.own_o = (float*)(ws + f.own_o);
   p.own_ml = (float2*)(ws + f.own_ml);
-  return a.D == 128 ? launch_prefix<128>(p, f, total_q, stream) : launch_prefix<64>(p, f, total_q, stream);
+  return a.D == 128 ? launch_prefix<128>(p, f, max_qo_len, stream) : launch_prefix<64>(p, f, max_qo_len, stream);
 }
 
 }  // namespace pts
