@@ -93,6 +93,7 @@ struct __align__(16) Bars {
   uint64_t full[8], empty[8];
   uint64_t s_full[2], p_full[2][2];       // P of a stream: its first and second 64 columns
   uint64_t o_full, drain;
+  uint64_t merge[2];        // two block streams: stream t's m and l are in TMEM
   uint32_t tmem;
   // masked value blocks so far: in shared memory; gone over by warps 2 and 3
   volatile int arrived, cleaned[2];
@@ -131,6 +132,14 @@ __device__ __forceinline__ void give_up(const PrefixParams& p, int code) {
 __device__ __forceinline__ int blocks_of(int tokens) { return (tokens + kBlock - 1) / kBlock; }
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
 
+// a / b for 0 <= a < 2^24, 0 < b < 2^24 (the quotient by floats is off by one at most):
+// the planning is a chain of these, and the compiler's integer division is a longer one.
+__device__ __forceinline__ int small_div(int a, int b) {
+  const int q = (int)__fdividef((float)a, (float)b), r = a - q * b;
+  return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+__device__ __forceinline__ int ceil_div(int a, int b) { return small_div(a + b - 1, b); }
+
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
 
 // Which of columns c0 .. c0 + 63 row `node` (token tok of the queries) sees (bit i: column
@@ -163,8 +172,9 @@ __device__ __forceinline__ bool odd2(uint32_t w) {
 }
 
 // ---------------------------------------------------------------- first kernel
-constexpr int kOwnThreads = 128;
+constexpr int kMaxOwnWarps = 4;
 constexpr int kOwnStages = 2;
+constexpr int kPlanCache = 512;           // entries whose shapes the plan keeps in shared memory
 
 // The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
 // and end cost about one and a half), and the launch about the larger of the total over
@@ -173,9 +183,12 @@ constexpr int kOwnStages = 2;
 __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
   const SharedAttnParams& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int* sums = (int*)smem;                               // [3][32]: items, large items, blocks
-  int* red = sums + 96;                                 // [4]; chunk at red[4]; running item count at red[5]
-  for (int g = warp; g < a.groups; g += kOwnThreads / 32) {
+  const int warps = blockDim.x >> 5, threads = blockDim.x;
+  int* sums = (int*)smem;                               // [2][32]: items, large items
+  int* red = sums + 64;                                 // longest, blocks, chunk, total
+  int2* shape = (int2*)(red + 4);                       // (units, blocks) of the first kPlanCache entries
+  for (int i = tid; i < 68; i += threads) sums[i] = 0;
+  for (int g = warp; g < a.groups; g += warps) {
     int lead;
     const int pages = group_shared_pages(a, g, &lead);
     const int b0 = a.group_indptr[g], b1 = a.group_indptr[g + 1];
@@ -183,49 +196,66 @@ __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
     if (lane == 0) {
       const int tokens = rows > 0 ? pages * a.page_len : 0;
       p.entries[g] = Entry{tokens, tokens, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0, rows > 0 ? pages : 0};
+      if (g < kPlanCache) shape[g] = make_int2(tiles_of(rows) * a.Hkv, blocks_of(tokens));
     }
   }
-  for (int i = tid; i < 96; i += kOwnThreads) sums[i] = 0;
   __syncthreads();
   const int entries = a.groups + (p.own_items ? a.batch : 0);
-  int longest = 1;
   if (p.own_items) {
-    for (int b = tid; b < a.batch; b += kOwnThreads) {
+    for (int b = tid; b < a.batch; b += threads) {
       const int tok0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - tok0, pages = p.entries[group_of(a, b)].pages;
-      const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0;
-      p.entries[a.groups + b] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
-      longest = max(longest, blocks_of(len));
+      const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0, e = a.groups + b;
+      p.entries[e] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
+      if (e < kPlanCache) shape[e] = make_int2(tiles_of(n * a.g) * a.Hkv, blocks_of(len));
     }
+    __syncthreads();
   }
-  for (int g = tid; g < a.groups; g += kOwnThreads) longest = max(longest, blocks_of(p.entries[g].tokens));
+  auto shape_of = [&](int e) -> int2 {
+    if (e < kPlanCache) return shape[e];
+    return make_int2(tiles_of(p.entries[e].rows) * a.Hkv, blocks_of(p.entries[e].tokens));
+  };
+  int longest = 1, blocks = 0;
+  for (int e = tid; e < entries; e += threads) {
+    const int2 x = shape_of(e);
+    longest = max(longest, x.x ? x.y : 0);
+    blocks += x.x * x.y;
+  }
   longest = __reduce_max_sync(0xffffffffu, longest);
-  if (lane == 0) red[warp] = longest;
+  blocks = __reduce_add_sync(0xffffffffu, blocks);
+  if (lane == 0) {
+    atomicMax(&red[0], longest);
+    atomicAdd(&red[1], blocks);
+  }
   __syncthreads();
-  longest = max(max(red[0], red[1]), max(red[2], red[3]));
-  const int tries = min(kMaxSplits, longest);
-  for (int e = tid; e < entries; e += kOwnThreads) {
-    const Entry x = p.entries[e];
-    const int units = tiles_of(x.rows) * a.Hkv, nb = blocks_of(x.tokens);
-    if (units == 0 || nb == 0) continue;
-    for (int k = 0; k < tries; ++k) {
-      const int c = (longest + k) / (k + 1), full = nb / c, rest = nb - full * c;
-      atomicAdd(&sums[k], units * (full + (rest > 0)));
-      atomicAdd(&sums[32 + k], units * (full + (2 * rest >= c && rest > 0)));
+  longest = red[0];
+  blocks = red[1];
+  {
+    // lane k: ranges of c blocks; each warp takes every warps-th entry
+    const int c = ceil_div(longest, lane + 1);
+    int items = 0, large = 0;
+#pragma unroll 2
+    for (int e = warp; e < entries; e += warps) {
+      const int2 x = shape_of(e);
+      const int full = small_div(x.y, c), rest = x.y - full * c;
+      items += x.x * (full + (rest > 0));
+      large += x.x * (full + (2 * rest >= c && rest > 0));
     }
-    atomicAdd(&sums[64], units * nb);
+    atomicAdd(&sums[lane], items);
+    atomicAdd(&sums[32 + lane], large);
   }
   __syncthreads();
   if (warp == 0) {
-    const int c = (longest + lane) / (lane + 1), items = sums[lane], large = sums[32 + lane], blocks = sums[64];
+    const int c = ceil_div(longest, lane + 1), items = sums[lane], large = sums[32 + lane];
     unsigned cost = 0xffffffffu;
-    if (lane == 0 || (lane < tries && items <= p.max_items))
-      cost = (unsigned)max((2ll * blocks + 3ll * items) / p.ctas, (long long)((large + p.ctas - 1) / p.ctas) * (2 * c + 3));
+    if (lane == 0 || (lane < longest && items <= p.max_items))
+      cost = (unsigned)max(small_div(min(2 * blocks + 3 * items, (1 << 24) - 1), p.ctas),
+                           small_div(min(large, 1 << 20) + p.ctas - 1, p.ctas) * (2 * c + 3));
     const unsigned win = __reduce_min_sync(0xffffffffu, cost);
     const int chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0);   // equal costs: fewer parts
-    if (lane == 0) red[4] = chunk;
+    if (lane == 0) red[2] = chunk;
   }
   __syncthreads();
-  const int chunk = red[4];
+  const int chunk = red[2];
   // the entries' first items, warp 0 over all entries in order
   if (warp == 0) {
     int run = 0;
@@ -233,8 +263,9 @@ __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
       const int e = e0 + lane;
       int n = 0, splits = 0;
       if (e < entries) {
-        splits = (blocks_of(p.entries[e].tokens) + chunk - 1) / chunk;
-        n = tiles_of(p.entries[e].rows) * a.Hkv * splits;
+        const int2 x = shape_of(e);
+        splits = ceil_div(x.y, chunk);
+        n = x.x * splits;
       }
       int incl = n;
 #pragma unroll
@@ -249,13 +280,13 @@ __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
     if (lane == 0) {
-      red[5] = min(run, p.max_items);
+      red[3] = min(run, p.max_items);
       *p.head = PlanHead{min(run, p.max_items), p.ctas};
     }
   }
   __syncthreads();
-  const int total = red[5];
-  for (int i = tid; i < total; i += kOwnThreads) {
+  const int total = red[3];
+  for (int i = tid; i < total; i += threads) {
     int lo = 0, hi = entries;                           // the last entry whose first item is <= i
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -263,32 +294,34 @@ __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
       else hi = mid;
     }
     const Entry x = p.entries[lo];
-    const int u = (i - x.first) / x.splits, split = i - x.first - u * x.splits, tiles = tiles_of(x.rows);
-    const int h = u / tiles, row0 = (u - h * tiles) * kTileRows;
+    const int u = small_div(i - x.first, x.splits), split = i - x.first - u * x.splits, tiles = tiles_of(x.rows);
+    const int h = small_div(u, tiles), row0 = (u - h * tiles) * kTileRows;
     p.items[i] = Item{x.tokens, x.prefix, min(kTileRows, x.rows - row0), x.tok0, x.table, row0, h, lo >= a.groups,
                       split * chunk, min(blocks_of(x.tokens), (split + 1) * chunk), 0, 0};
   }
 }
 
-// The own columns of a request with at most 8 NR rows.  Each of the four warps takes
-// every fourth 16-token run through a ring of its own and computes
+// The own columns of a request with at most 8 NR rows.  The CTA's warps (two to four, as
+// fill the SMs in one round) take its 16-token runs in turn, each through a ring of its
+// own, and compute
 //   S^T = K Q^T (16 tokens x 8 rows per product), O^T += V^T P^T,
-// P^T handed to the second product by movmatrix; the four warps' O, m and l are added up
-// at the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
+// P^T handed to the second product by movmatrix; the warps' O, m and l are added up at
+// the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
 // in use, and the 8 columns are query rows: half the products of the plain form at 8
 // rows or fewer.
 template <int D, int NR>
-__global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParams p,
+__global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const PrefixParams p,
                                                                const __grid_constant__ CUtensorMap run_map) {
   using S = Shape<D>;
   constexpr int kRows = 8 * NR;
   constexpr uint32_t kStage = 2 * S::kRunBytes, kWarp = kOwnStages * kStage;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[4][kOwnStages];
-  __shared__ float2 ml[4][kRows];
+  __shared__ uint64_t full[kMaxOwnWarps][kOwnStages];
+  __shared__ float2 ml[kMaxOwnWarps][kRows];
   const SharedAttnParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int warps = blockDim.x >> 5;
   if (lane < kOwnStages) mbar_init(&full[warp][lane], 1);
   fence_mbar_init();
   __syncwarp();
@@ -308,12 +341,12 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
   const int n_runs = (len + kRun - 1) / kRun;
   const int r0 = (int)((int64_t)n_runs * blockIdx.z / p.own_splits);
   const int r1 = (int)((int64_t)n_runs * (blockIdx.z + 1) / p.own_splits);
-  const int mine = max(0, (r1 - r0 - warp + 3) / 4);    // this warp's runs r0 + warp + 4 i
+  const int mine = r1 - r0 > warp ? ceil_div(r1 - r0 - warp, warps) : 0;   // this warp's runs r0 + warp + warps i
   const uint32_t ring = smem_u32(smem) + warp * kWarp;
 
   // the pages of this warp's runs 32 w .. 32 w + 31, one per lane
   auto window = [&](int w) -> int {
-    const int tok = (r0 + warp + 4 * (32 * w + lane)) * kRun;
+    const int tok = (r0 + warp + warps * (32 * w + lane)) * kRun;
     const int page = 32 * w + lane < mine ? __ldg(table + p.page_of(tok)) : -1;
     return page >= 0 && page < a.max_pages ? page : a.max_pages;     // past the pool: zero fill
   };
@@ -325,7 +358,7 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
     }
     const int page = __shfl_sync(0xffffffffu, page_now, i & 31);
     if (lane == 0) {
-      const int tok = (r0 + warp + 4 * i) * kRun, group = (tok - p.page_of(tok) * a.page_len) / 8;
+      const int tok = (r0 + warp + warps * i) * kRun, group = (tok - p.page_of(tok) * a.page_len) / 8;
       uint64_t* bar = &full[warp][i % kOwnStages];
       uint8_t* dst = smem + warp * kWarp + (i % kOwnStages) * kStage;
       mbar_arrive_expect_tx(bar, kStage);
@@ -367,7 +400,7 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
     const uint32_t kb = ring + (i % kOwnStages) * kStage, vb = kb + S::kRunBytes;
     ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1, p.wait_limit));
     if (!ok) break;
-    const int c0 = (r0 + warp + 4 * i) * kRun;          // own column of the run's first token
+    const int c0 = (r0 + warp + warps * i) * kRun;      // own column of the run's first token
     float s[NR][4];
 #pragma unroll
     for (int n = 0; n < NR; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
@@ -493,7 +526,7 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
     for (int x = i; x < loaded; ++x) mbar_wait(&full[warp][x % kOwnStages], (x / kOwnStages) & 1);
   }
   __syncthreads();
-  float* os = (float*)smem;                             // [4][kRows][D + 4]
+  float* os = (float*)smem;                             // [warps][kRows][D + 4]
   constexpr int kStride = D + 4;
 #pragma unroll
   for (int n = 0; n < NR; ++n)
@@ -511,14 +544,14 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
       }
     }
   __syncthreads();
-  for (int e = threadIdx.x; e < rows * (D / 4); e += kOwnThreads) {
+  for (int e = threadIdx.x; e < rows * (D / 4); e += blockDim.x) {
     const int r = e / (D / 4), quad = e % (D / 4), R = row0 + r, tk = p.div_g.div(R);
-    const float M = fmaxf(fmaxf(ml[0][r].x, ml[1][r].x), fmaxf(ml[2][r].x, ml[3][r].x));
+    float M = -INFINITY;
+    for (int w = 0; w < warps; ++w) M = fmaxf(M, ml[w][r].x);
     const float base = M == -INFINITY ? 0.0f : M;
     float L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const float f = fast_exp2(ml[w][r].x - base);
       const float4 v = *(const float4*)(os + (w * kRows + r) * kStride + quad * 4);
       L = fmaf(f, ml[w][r].y, L);
@@ -533,11 +566,13 @@ __global__ void __launch_bounds__(kOwnThreads) plan_own_kernel(const PrefixParam
   }
 }
 
+// Shared memory per warp: its ring, later its O; the plan's CTA needs less.
 template <int D, int NR>
 constexpr size_t own_smem() {
-  constexpr size_t ring = (size_t)4 * kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)4 * 8 * NR * (D + 4) * 4;
-  return (ring > o ? ring : o) + 1024;
+  constexpr size_t ring = (size_t)kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)8 * NR * (D + 4) * 4;
+  return ring > o ? ring : o;
 }
+static_assert(2 * own_smem<64, 1>() >= (64 + 4) * 4 + kPlanCache * 8, "the plan's arrays");
 
 // --------------------------------------------------------------- second kernel
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
@@ -568,6 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.s_full[t], 1);
       mbar_init(&bars.p_full[t][0], 4);
       mbar_init(&bars.p_full[t][1], 4);
+      mbar_init(&bars.merge[t], 4);
     }
     mbar_init(&bars.q_ready, 8);
     for (int s = 0; s < S::kSlots; ++s) {
@@ -608,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tm = tmem + lane_base + kColS + 128 * t, o_tm = tmem + lane_base + kColO + D * t;
     bool ok = true;
-    int steps = 0;
+    int steps = 0, merges = 0;
     // The first round is a rehearsal, while the plan is made: one pass of the block
     // code over whatever the TMEM holds, with nothing waited for, signalled or kept.
     // It brings the loop's instructions (some 10 KB) into the SM's caches, which cost the
@@ -637,21 +673,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int chunk = lane % kChunks;
           const uint32_t qb = smem_u32(smem + S::kOffQ + (two ? t : 0) * S::kSlotBytes) + (chunk / 8) * S::kQHalfBytes;
           const uint16_t* q = (const uint16_t*)a.q + ((int64_t)it.tok0 * a.Hq + it.h * a.g) * D + chunk * 8;
-          for (int k0 = 0; k0 < kLoads; k0 += 8) {
-            uint4 v[8];
+          uint4 v[kLoads];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = quarter * 32 + (k0 + j) * kPer + lane / kChunks, R = it.row0 + my0 + r;
-              const int tk = p.div_g.div(R);
-              v[j] = make_uint4(0, 0, 0, 0);
-              if (my0 + r < it.rows) v[j] = __ldg((const uint4*)(q + ((int64_t)tk * a.Hq + (R - tk * a.g)) * D));
-            }
+          for (int j = 0; j < kLoads; ++j) {
+            const int r = quarter * 32 + j * kPer + lane / kChunks, R = it.row0 + my0 + r;
+            const int tk = p.div_g.div(R);
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (my0 + r < it.rows) v[j] = __ldg((const uint4*)(q + ((int64_t)tk * a.Hq + (R - tk * a.g)) * D));
+          }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = quarter * 32 + (k0 + j) * kPer + lane / kChunks;
-              st_shared_v4(qb + (uint32_t)r * 128u + (uint32_t)(((chunk & 7) ^ (r & 7)) << 4), v[j].x, v[j].y, v[j].z,
-                           v[j].w);
-            }
+          for (int j = 0; j < kLoads; ++j) {
+            const int r = quarter * 32 + j * kPer + lane / kChunks;
+            st_shared_v4(qb + (uint32_t)r * 128u + (uint32_t)(((chunk & 7) ^ (r & 7)) << 4), v[j].x, v[j].y, v[j].z,
+                         v[j].w);
           }
           fence_proxy_async_smem();
         }
@@ -753,21 +787,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
+      // Two block streams hold the same rows: each warpgroup adds up half of the columns
+      // of both, with m and l exchanged through TMEM (a row is the same lane in both).
+      // The next item's products wait for both warpgroups' q_ready.
+      float mine = 1.0f, theirs = 0.0f;                 // weights of the two streams' O
+      if (!two) {
+        tmem_st2(s_tm, __float_as_uint(m), __float_as_uint(l));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.merge[t]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.merge[1 - t], merges & 1, p.wait_limit));
+        if (!ok) {
+          if (lane == 0) give_up(p, 73);
+          break;
+        }
+        ++merges;
+        tc_fence_after();
+        uint32_t u0, u1;
+        tmem_ld2(tmem + lane_base + kColS + 128 * (1 - t), u0, u1);
+        tmem_ld_wait();
+        const float m2 = __uint_as_float(u0), l2 = __uint_as_float(u1), M = fmaxf(m, m2);
+        const float base = M == -INFINITY ? 0.0f : M;
+        mine = fast_exp2(m - base);
+        theirs = fast_exp2(m2 - base);
+        l = mine * l + theirs * l2;
+        m = M;
+      }
+      // tree slots whose infinite or NaN values were taken out of V
+      const bool odd = it.own && __any_sync(0xffffffffu, (bars.odd[k & 3][0][lane] | bars.odd[k & 3][1][lane]) != 0u);
       // the part: O as [column quad][row] so that a warp stores 512 contiguous bytes
-      float* part = p.parts + (int64_t)index * S::kPartFloats + t * (S::kPartFloats / 2);
+      float* part = p.parts + (int64_t)index * S::kPartFloats + (two ? t * (S::kPartFloats / 2) : 0);
+      const int cb0 = two ? 0 : t * (D / 64), cb1 = two ? D / 32 : cb0 + D / 64;
 #pragma unroll 1
-      for (int cb = 0; cb < D / 32; ++cb) {
+      for (int cb = cb0; cb < cb1; ++cb) {
         uint32_t o[32];
         tmem_ld32(o_tm + 32 * cb, o);
+        if (!two) {
+          uint32_t o2[32];
+          tmem_ld32(tmem + lane_base + kColO + D * (1 - t) + 32 * cb, o2);
+          tmem_ld_wait();
+          // a stream that has had no block (weight 0) has no O
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float x = mine != 0.0f ? mine * __uint_as_float(o[c]) : 0.0f;
+            o[c] = __float_as_uint(theirs != 0.0f ? fmaf(theirs, __uint_as_float(o2[c]), x) : x);
+          }
+        }
         tmem_ld_wait();
-        if (it.own) {
-          // tree slots whose infinite or NaN values were taken out of V: the rows that
-          // see them get them
+        if (odd) {
+          // the rows that see them get them
           for (int w = 0; w < kMaxTreeWords; ++w) {
             uint32_t bits = bars.odd[k & 3][0][w] | bars.odd[k & 3][1][w];
             for (; bits; bits &= bits - 1) {
               const int slot = 32 * w + __ffs(bits) - 1, col = it.prefix + slot, blk = col / kBlock;
-              if (!valid || blk < it.ja || blk >= it.jb || (!two && ((blk - it.ja) & 1) != t)) continue;
+              if (!valid || blk < it.ja || blk >= it.jb) continue;
               if (!(seen_columns(a, it.tok0 + node, node, col & ~63, it.prefix, it.tokens) >> (col & 63) & 1ull)) continue;
               const int pg = p.page_of(col), page = a.page_indices[it.table + pg];
               if (page < 0 || page >= a.max_pages) continue;
@@ -791,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_fence_before();
-      if (valid) {
+      if (valid && (two || t == 0)) {
         part[128 * D + r_local] = m;
         part[128 * D + 128 + r_local] = l;
       }
@@ -803,14 +877,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // so that no register that a fetch is still filling is moved).
     pdl_wait();
     pdl_trigger();
-    const int total = *(volatile int*)&p.head->total;
+    const int total = __ldcg(&p.head->total);
     const int copies = kBlock / p.copy_tokens;
     bool ok = true;
     int pushed = 0, mine = blockIdx.x;                  // copies into the ring so far; this item's number
     for (int k = 0; ok; ++k) {
       const bool more = mine < total;
-      Item it;
-      if (more) it = p.items[mine];
+      const Item it = p.items[min(mine, p.max_items - 1)];   // (read beside the total, not after it)
       int claim = 0;
       if (lane == 0 && more) claim = atomicAdd(&p.head->next, 1);
       // the slot's last item, k - 2, has been copied by everyone
@@ -937,7 +1010,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int ph = (t ? steps1++ : steps0++) & 1;
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
-              if (!wait(&bars.p_full[t][part], ph, 64)) break;
+              ok = mbar_wait_spin(&bars.p_full[t][part], ph, p.wait_limit);
+              if (!ok) {
+                give_up(p, 64);
+                break;
+              }
               tc_fence_after();
 #pragma unroll
               for (int j = part * kRuns / 2; j < (part + 1) * kRuns / 2; ++j)
@@ -1045,123 +1122,142 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---------------------------------------------------------------- third kernel
 // A CTA joins 16 rows of a request and KV head: the parts of its group's shared columns,
-// and those of its own.  First every part's m and l come in at once, then a thread per
-// row turns them into weights e^(m - M) / L, then each thread sums one column quad of one
-// row: four rows and eight quads per warp, so that both the parts ([quad][row]) and the
-// output are touched in 64-byte pieces.
+// and those of its own.  Every part's m and l come in at once and become weights
+// e^(m - M); then the O values are summed, a thread per row and column quad: four rows and
+// eight quads per warp, so that both the parts ([quad][row]) and the output are touched in
+// 64-byte pieces.  With few rows the parts are split over the spare threads too.  Bound by
+// the latency of reading what other SMs have just written, so every load is issued
+// before the first is used.
 constexpr int kJoinRows = 16;
-constexpr int kMaxParts = 4 * kMaxSplits;
+constexpr int kJoinThreads = 256;
+constexpr int kMaxParts = 2 * kMaxSplits;
+static_assert(kMaxOwnSplits <= kMaxSplits, "");
 
 template <int D>
-__global__ void __launch_bounds__(128) join_parts_kernel(const PrefixParams p, int row_tiles) {
+__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const PrefixParams p, int row_tiles) {
   const SharedAttnParams& a = p.a;
   constexpr int kPart = Shape<D>::kPartFloats, kHalf = kPart / 2;
   __shared__ float w[kMaxParts][kJoinRows], lw[kMaxParts][kJoinRows];
   __shared__ const float* src[2][kJoinRows];            // first part's O of the shared and the own columns
-  __shared__ int64_t step[2][kJoinRows];                // floats from part to part
   __shared__ int cnt[2][kJoinRows];
+  __shared__ float inv[kJoinRows];
+  __shared__ float4 sum[kJoinThreads];
   pdl_trigger();
-  pdl_wait();
   const int b = blockIdx.x / row_tiles, row0 = (blockIdx.x - b * row_tiles) * kJoinRows, h = blockIdx.y;
-  const int tok0 = a.qo_indptr[b], total_rows = (a.qo_indptr[b + 1] - tok0) * a.g;
+  const int tok0 = a.qo_indptr[b], total_rows = (a.qo_indptr[b + 1] - tok0) * a.g, gi = group_of(a, b);
+  pdl_wait();                                           // (the lengths are no kernel's of this call)
   if (row0 >= total_rows) return;
   const int n = min(kJoinRows, total_rows - row0);
-  // where the parts of row R are: thread (set, row).  A stored part is [quad][128 rows] with
-  // m and l behind, two streams per item; the first kernel's are [quad] with (m, l) apart.
+  // Where row R's parts are: thread (set, row).  A stored part is [quad][128 rows] with m and
+  // l behind; the first kernel's are [quad] with (m, l) apart.
   if (threadIdx.x < 2 * kJoinRows) {
     const int set = threadIdx.x / kJoinRows, r = threadIdx.x % kJoinRows, R = row0 + r;
     if (set == 1 && !p.own_items) {
       const int tk = p.div_g.div(R);
       const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g;
       src[1][r] = p.own_o + row * p.own_splits * D;
-      step[1][r] = D;
-      cnt[1][r] = r < n ? p.own_splits : 0;
+      cnt[1][r] = p.own_splits;
     } else {
-      const Entry e = p.entries[set == 0 ? group_of(a, b) : a.groups + b];
+      const Entry e = p.entries[set == 0 ? gi : a.groups + b];
       const int in_entry = (tok0 - e.tok0) * a.g + R, tile = in_entry / kTileRows, in = in_entry % kTileRows;
-      const bool two = e.rows - tile * kTileRows > 128;
       src[set][r] = p.parts + ((int64_t)e.first + ((int64_t)h * tiles_of(e.rows) + tile) * e.splits) * kPart +
-                    (two ? (in >> 7) * kHalf : 0) + (in & 127) * 4;
-      step[set][r] = two ? kPart : kHalf;
-      cnt[set][r] = r < n ? (two ? e.splits : 2 * e.splits) : 0;
+                    (in >> 7) * kHalf + (in & 127) * 4;
+      cnt[set][r] = e.splits;
     }
   }
   __syncthreads();
-  const int most = max(cnt[0][0], cnt[0][n - 1]) + max(cnt[1][0], cnt[1][n - 1]);
+  const int shared = cnt[0][0], own = cnt[1][0], parts = shared + own;
+  const int64_t own_step = p.own_items ? kPart : D;
 #pragma unroll 4
-  for (int e = threadIdx.x; e < most * kJoinRows; e += 128) {
-    const int r = e % kJoinRows, k = e / kJoinRows, shared = cnt[0][r];
+  for (int e = threadIdx.x; e < parts * kJoinRows; e += kJoinThreads) {
+    const int r = e % kJoinRows, k = e / kJoinRows;
     float m = -INFINITY, l = 0.0f;
-    if (k < shared + cnt[1][r]) {
-      const int set = k >= shared, i = set ? k - shared : k;
-      if (set && !p.own_items) {
-        const float2 x = __ldcg(p.own_ml + (src[1][r] - p.own_o) / D + i);
+    if (r < n) {
+      if (k >= shared && !p.own_items) {
+        const float2 x = __ldcg(p.own_ml + (src[1][r] - p.own_o) / D + (k - shared));
         m = x.x;
         l = x.y;
       } else {
-        // (row & 127) * 4 floats into the part: m is 128 D + row & 127 floats in
-        const int64_t at = (src[set][r] - p.parts) % kHalf;
-        const float* part = src[set][r] - at + i * step[set][r];
-        m = __ldcg(part + 128 * D + at / 4);
-        l = __ldcg(part + 128 * D + 128 + at / 4);
+        // src is (row & 127) * 4 floats into the part: m is 128 D + row & 127 floats in
+        const int set = k >= shared, at = (int)((src[set][r] - p.parts) % kHalf);
+        const float* part = src[set][r] - at + at / 4 + 128 * D + (int64_t)(set ? k - shared : k) * kPart;
+        m = __ldcg(part);
+        l = __ldcg(part + 128);
       }
     }
     w[k][r] = m;
     lw[k][r] = l;
   }
   __syncthreads();
-  if (threadIdx.x < kJoinRows) {
-    const int r = threadIdx.x;
+  {
+    // sixteen threads per row
+    const int r = threadIdx.x / 16, j = threadIdx.x % 16;
     float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < most; ++k) M = fmaxf(M, w[k][r]);
+    for (int k = j; k < parts; k += 16) M = fmaxf(M, w[k][r]);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
     const float base = M == -INFINITY ? 0.0f : M;
-    for (int k = 0; k < most; ++k) {
+    for (int k = j; k < parts; k += 16) {
       const float x = fast_exp2(w[k][r] - base);
       L = fmaf(x, lw[k][r], L);
       w[k][r] = x;
     }
-    lw[0][r] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L; // nothing seen: 0
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    if (j == 0) inv[r] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;   // nothing seen: 0
   }
   __syncthreads();
-  const int units = (n + 3) / 4 * D;
-  for (int idx = threadIdx.x; idx < units; idx += 128) {
-    const int lo = idx & 31, hi = idx >> 5;
+  // units of four rows x eight quads per warp; `slices` threads share a unit's parts
+  const int units = (n + 3) / 4 * D, slices = max(1, kJoinThreads / units);
+  for (int idx = threadIdx.x; idx < units * slices; idx += kJoinThreads) {
+    const int unit = idx % units, slice = idx / units, lo = unit & 31, hi = unit >> 5;
     const int r = (hi / (D / 32)) * 4 + (lo & 3), quad = (hi % (D / 32)) * 8 + (lo >> 2);
-    if (r >= n) continue;
-    float o0 = 0.0f, o1 = 0.0f, o2 = 0.0f, o3 = 0.0f;
-    int k = 0;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < n) {
+      const float* s0 = src[0][r] + quad * 512;
+      const float* s1 = src[1][r] + (p.own_items ? quad * 512 : quad * 4);
+      for (int k0 = slice; k0 < parts; k0 += 12 * slices) {
+        float4 v[12];
 #pragma unroll
-    for (int set = 0; set < 2; ++set) {
-      const float* s = src[set][r] + (set && !p.own_items ? quad * 4 : quad * 512);
-      const int64_t d = step[set][r];
-      const int c = cnt[set][r];
-      for (int k0 = 0; k0 < c; k0 += 8) {
-        float4 v[8];                                    // eight loads in flight
+        for (int u = 0; u < 12; ++u) {
+          const int k = k0 + u * slices;
+          if (k < parts) v[u] = __ldcg((const float4*)(k < shared ? s0 + (int64_t)k * kPart : s1 + (k - shared) * own_step));
+        }
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (k0 + u < c) v[u] = __ldcg((const float4*)(s + (k0 + u) * d));
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float x = k0 + u < c ? w[k + k0 + u][r] : 0.0f;
+        for (int u = 0; u < 12; ++u) {
+          const int k = k0 + u * slices;
+          const float x = k < parts ? w[k][r] : 0.0f;
           if (x != 0.0f) {                              // a part of no columns has no O
-            o0 = fmaf(x, v[u].x, o0);
-            o1 = fmaf(x, v[u].y, o1);
-            o2 = fmaf(x, v[u].z, o2);
-            o3 = fmaf(x, v[u].w, o3);
+            o.x = fmaf(x, v[u].x, o.x);
+            o.y = fmaf(x, v[u].y, o.y);
+            o.z = fmaf(x, v[u].z, o.z);
+            o.w = fmaf(x, v[u].w, o.w);
           }
         }
       }
-      k += c;
     }
-    const float inv = lw[0][r];
+    if (slices > 1) {                                   // (then units * slices <= the CTA: one round)
+      sum[idx] = o;
+      __syncthreads();
+      if (slice > 0) return;
+      for (int i = 1; i < slices; ++i) {
+        const float4 v = sum[unit + i * units];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+      }
+    }
+    if (r >= n) continue;
+    const float f = inv[r];
     const int R = row0 + r, tk = p.div_g.div(R);
     *(uint2*)((uint16_t*)a.out + ((int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g) * D + quad * 4) =
-        make_uint2(pack_bf16x2(o0 * inv, o1 * inv), pack_bf16x2(o2 * inv, o3 * inv));
+        make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
   }
 }
 
 struct PrefixPlan {
-  int few, own_rows, own_tiles, own_splits, max_items, ctas;
+  int few, own_rows, own_tiles, own_splits, own_warps, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
@@ -1184,12 +1280,23 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   f.own_rows = rows <= 8 ? 8 : 16;
   f.own_tiles = f.few ? 1 : 0;
   f.ctas = sm_count();
-  // own columns in the first kernel: about three CTAs per SM, each warp with two runs at least
+  // Own columns in the first kernel: slices for about three CTAs of four warps per SM, each
+  // warp with two runs at least; where there are more (request, head) pairs than that,
+  // CTAs of three or two warps if they then all run at once.
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
   f.own_splits = 1;
-  if (f.few)
-    f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({3ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
-                                                                (own + 8 * kRun - 1) / (8 * kRun), kMaxOwnSplits}));
+  f.own_warps = kMaxOwnWarps;
+  if (f.few) {
+    const int64_t pairs = std::max<int64_t>((int64_t)batch * Hkv, 1);
+    f.own_splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>({3ll * f.ctas / pairs, (own + 8 * kRun - 1) / (8 * kRun), kMaxOwnSplits}));
+    const int per_warp = D == 128 ? (int)own_smem<128, 2>() : (int)own_smem<64, 2>();
+    for (int w = kMaxOwnWarps; w >= 2; --w)
+      if (pairs * f.own_splits <= (int64_t)f.ctas * ((227 * 1024) / (w * per_warp + 3 * 1024))) {
+        f.own_warps = w;
+        break;
+      }
+  }
   int64_t units = ((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups;
   if (!f.few) units += ((int64_t)total_q * g + kTileRows - 1) / kTileRows + batch;
   f.max_items = (int)std::min<int64_t>(units * Hkv + 2 * f.ctas, 1 << 28);
@@ -1222,11 +1329,11 @@ int encode_kv(CUtensorMap* map, const SharedAttnParams& a, int copy_tokens) {
 }
 
 template <int D, int NR>
-int launch_own(const PrefixParams& p, int few, const CUtensorMap& map, cudaStream_t stream) {
-  constexpr size_t smem = own_smem<D, NR>();
-  if (int rc = ensure_smem_attr((const void*)plan_own_kernel<D, NR>, smem)) return rc;
-  const dim3 grid = few ? dim3(1 + p.a.batch * p.own_tiles, p.a.Hkv, p.own_splits) : dim3(1);
-  PTS_CUDA_TRY(launch_pdl(plan_own_kernel<D, NR>, grid, dim3(kOwnThreads), smem, stream, p, map));
+int launch_own(const PrefixParams& p, const PrefixPlan& f, const CUtensorMap& map, cudaStream_t stream) {
+  const size_t smem = f.own_warps * own_smem<D, NR>() + 1024;
+  if (int rc = ensure_smem_attr((const void*)plan_own_kernel<D, NR>, kMaxOwnWarps * own_smem<D, NR>() + 1024)) return rc;
+  const dim3 grid = f.few ? dim3(1 + p.a.batch * p.own_tiles, p.a.Hkv, p.own_splits) : dim3(1);
+  PTS_CUDA_TRY(launch_pdl(plan_own_kernel<D, NR>, grid, dim3(32 * f.own_warps), smem, stream, p, map));
   return launch_status("plan_own_kernel");
 }
 
@@ -1235,13 +1342,14 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
   CUtensorMap run_map, block_map;
   if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
   if (int rc = encode_kv<D>(&block_map, p.a, p.copy_tokens)) return rc;
-  if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, f.few, run_map, stream) : launch_own<D, 2>(p, f.few, run_map, stream))
+  if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, f, run_map, stream) : launch_own<D, 2>(p, f, run_map, stream))
     return rc;
   if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem)) return rc;
   PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
   if (int rc = launch_status("prefix_attn_kernel")) return rc;
   const int row_tiles = (int)(((int64_t)max_qo_len * p.a.g + kJoinRows - 1) / kJoinRows);
-  PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(128), 0, stream, p, row_tiles));
+  PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(kJoinThreads), 0,
+                          stream, p, row_tiles));
   return launch_status("join_parts_kernel");
 }
 
