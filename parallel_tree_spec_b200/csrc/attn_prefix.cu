@@ -1,13 +1,9 @@
 // Tree attention for requests that share leading pages, bf16 with head_dim 64 or 128
-// and pages of whole 16-token runs, on the tensor cores.  Three launches:
+// and pages of whole 16-token runs, on the tensor cores.  Three or four launches:
 //
-// plan_own_kernel: CTA 0 makes the plan of the second launch (which lengths are on the
-//   device only): the column sets -- each group's shared columns, each request's own
-//   -- with their rows and tokens, cut into work items.  The other CTAs, when requests
-//   have at most 16 query rows per KV head (decoding), compute the requests' own
-//   columns: so few rows fill an eighth of a 128-row tensor-core tile at most, and the
-//   K/V bytes serve those rows only, so HBM is the bound and mma.sync m16n8k16 on
-//   transposed products, fed by TMA through a small ring per warp, is enough.
+// plan_kernel: one CTA makes the plan (which lengths are on the device only): the column
+//   sets -- each group's shared columns, each request's own -- with their rows and
+//   tokens, cut into work items.
 // prefix_attn_kernel: the work items, one at a time per CTA (persistent, claimed from a
 //   counter): a tile of 256 query rows -- (token, query head of the KV head's group),
 //   a group's requests one after the other -- a KV head and a range of 128-token blocks.
@@ -18,10 +14,18 @@
 //   rows and every second block.  tcgen05 with S and O in TMEM, P written back over S as
 //   the A operand of the value product; K/V by TMA into a ring; one thread per row, so
 //   the softmax needs no shuffles.  Each item leaves one part per row (fp32 O, m, l).
+// own_attn_kernel, when requests have at most 16 query rows per KV head (decoding): their
+//   own columns.  So few rows fill an eighth of a 128-row tensor-core tile at most, and
+//   the K/V bytes serve those rows only, so HBM is the bound and mma.sync m16n8k16 on
+//   transposed products, fed by TMA through a small ring per warp, is enough.  It is
+//   launched to run beside the second kernel, which is bound by its arithmetic: a CTA of
+//   two warps fits an SM next to that kernel's CTA (its ring and its registers are kept
+//   that small).
 // join_parts_kernel: joins every row's parts and writes the output.
 //
 // Scores are kept in units of log2: x = s * scale * log2(e), e^(s - m) = 2^(x - m').
 #include <algorithm>
+#include <atomic>
 
 #include "attn_shared.cuh"
 #include "sm100.cuh"
@@ -36,9 +40,14 @@ constexpr int kRun = 16;                  // tokens of one value product; pages 
 constexpr int kRuns = kBlock / kRun;
 constexpr int kTileRows = 256;
 constexpr int kThreads = 384;             // warps 0 TMA, 1 MMA, 2-3 masked values, 4-7 and 8-11 softmax
+// Registers: the block is launched with 128 a thread; warps 0-3 give some back and the
+// softmax warps take them.  The shares stay within the launch's total.
+constexpr int kLaunchRegs = 128, kHelperRegs = 48, kSoftmaxRegs = 168;
+constexpr int kBoundThreads = 512;        // the launch bound that gives 128 registers
+static_assert(128 * kHelperRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, "the split draws on the launch's registers");
 constexpr int kMaxSplits = 32;            // block ranges of a column set
-constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in the first kernel
-constexpr int kFewRows = 16;              // rows per KV head up to which the first kernel takes them
+constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in own_attn_kernel
+constexpr int kFewRows = 16;              // rows per KV head up to which own_attn_kernel takes them
 constexpr int kMaxTreeWords = PTS_MAX_TREE_NODES / 32;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -53,11 +62,11 @@ struct Shape {
   static constexpr uint32_t kRunBytes = 2 * kGroupBytes;
   static constexpr uint32_t kSlotBytes = kRuns * kRunBytes;     // K or V of a block; Q of a stream
   static constexpr uint32_t kQHalfBytes = 128 * 128;            // Q: [half][128 rows][64 dims]
-  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSlots = D == 128 ? 4 : 6;
   static constexpr uint32_t kOffQ = 0;
   static constexpr uint32_t kOffRing = 2 * kSlotBytes;
   static constexpr uint32_t kOffBars = kOffRing + kSlots * kSlotBytes;
-  static constexpr uint32_t kSmem = kOffBars + 1536 + 1024;     // barriers; alignment slack
+  static constexpr uint32_t kSmem = kOffBars + 1408;            // barriers
   static constexpr int kPartFloats = 2 * 128 * (D + 2);         // one item's part: two streams' rows
 };
 static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared memory above 227 KB");
@@ -99,7 +108,7 @@ struct __align__(16) Bars {
   volatile int arrived, cleaned[2];
   uint32_t odd[4][2][kMaxTreeWords];      // by item count mod 4 and warp: tree slots with infinities or NaN in V
 };
-static_assert(sizeof(Bars) <= 1536, "barrier block");
+static_assert(sizeof(Bars) <= 1408, "barrier block");
 
 struct PrefixParams {
   SharedAttnParams a;
@@ -110,15 +119,15 @@ struct PrefixParams {
   int* error;
   long long wait_limit;
   // plan
-  int ctas;                 // of the second kernel
+  int ctas;                 // of prefix_attn_kernel
   int max_items;            // parts in the workspace
   int own_items;            // own columns are work items
   PlanHead* head;
   Entry* entries;
   Item* items;
   float* parts;
-  // own columns in the first kernel
-  int own_tiles, own_splits;
+  // own columns in own_attn_kernel
+  int own_splits;
   float* own_o;             // [T * Hq][own_splits][D]
   float2* own_ml;           // [T * Hq][own_splits]
 
@@ -171,23 +180,26 @@ __device__ __forceinline__ bool odd2(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// ---------------------------------------------------------------- first kernel
-constexpr int kMaxOwnWarps = 4;
+// ------------------------------------------------------------------------- plan
+constexpr int kPlanThreads = 256;
+constexpr int kOwnWarps = 2;
 constexpr int kOwnStages = 2;
 constexpr int kPlanCache = 512;           // entries whose shapes the plan keeps in shared memory
 
 // The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
 // and end cost about one and a half), and the launch about the larger of the total over
 // the CTAs and the large items' rounds; the cheapest of up to 32 ranges of
-// ceil(longest / k) blocks is taken.  On one CTA, beside the own columns' CTAs.
-__device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
+// ceil(longest / k) blocks is taken.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p) {
+  __shared__ __align__(8) int sums[64 + 4 + 2 * kPlanCache];         // [2][32] items, large items; red; shapes
   const SharedAttnParams& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int warps = blockDim.x >> 5, threads = blockDim.x;
-  int* sums = (int*)smem;                               // [2][32]: items, large items
+  constexpr int warps = kPlanThreads / 32, threads = kPlanThreads;
+  pdl_wait();
+  pdl_trigger();
   int* red = sums + 64;                                 // longest, blocks, chunk, total
   int2* shape = (int2*)(red + 4);                       // (units, blocks) of the first kPlanCache entries
-  for (int i = tid; i < 68; i += threads) sums[i] = 0;
+  if (tid < 68) sums[tid] = 0;
   for (int g = warp; g < a.groups; g += warps) {
     int lead;
     const int pages = group_shared_pages(a, g, &lead);
@@ -301,47 +313,47 @@ __device__ void make_plan(const PrefixParams& p, uint8_t* smem) {
   }
 }
 
-// The own columns of a request with at most 8 NR rows.  The CTA's warps (two to four, as
-// fill the SMs in one round) take its 16-token runs in turn, each through a ring of its
-// own, and compute
+// ------------------------------------------------------------------ own columns
+// The own columns of a request with at most 8 NR rows.  The CTA's two warps take its
+// 16-token runs in turn, each through a ring of its own, and compute
 //   S^T = K Q^T (16 tokens x 8 rows per product), O^T += V^T P^T,
 // P^T handed to the second product by movmatrix; the warps' O, m and l are added up at
 // the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
 // in use, and the 8 columns are query rows: half the products of the plain form at 8
 // rows or fewer.
 template <int D, int NR>
-__global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const PrefixParams p,
-                                                               const __grid_constant__ CUtensorMap run_map) {
+__global__ void __launch_bounds__(32 * kOwnWarps, 7)
+    own_attn_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap run_map) {
   using S = Shape<D>;
   constexpr int kRows = 8 * NR;
   constexpr uint32_t kStage = 2 * S::kRunBytes, kWarp = kOwnStages * kStage;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[kMaxOwnWarps][kOwnStages];
-  __shared__ float2 ml[kMaxOwnWarps][kRows];
+  extern __shared__ __align__(1024) uint8_t smem[];      // the warps' rings; barriers and (m, l) behind
+  constexpr int warps = kOwnWarps;
+  uint64_t(*full)[kOwnStages] = (uint64_t(*)[kOwnStages])(smem + warps * kWarp);
+  float2(*ml)[kRows] = (float2(*)[kRows])(smem + warps * kWarp + sizeof(uint64_t) * warps * kOwnStages);
   const SharedAttnParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
-  const int warps = blockDim.x >> 5;
   if (lane < kOwnStages) mbar_init(&full[warp][lane], 1);
   fence_mbar_init();
   __syncwarp();
-  pdl_wait();
   pdl_trigger();
-  if (blockIdx.x == 0) {
-    if (blockIdx.y == 0 && blockIdx.z == 0) make_plan(p, smem);
+  // Nothing here depends on the two kernels before: what this one reads is not theirs, and
+  // everything before them had completed when they were launched.  It waits for them at the
+  // end, so that what follows may wait for this kernel alone.
+  const int b = blockIdx.x, h = blockIdx.y;
+  const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
+  if (total_rows <= 0) {
+    pdl_wait();
     return;
   }
-  const int b = (blockIdx.x - 1) / p.own_tiles, row0 = (blockIdx.x - 1 - b * p.own_tiles) * kRows, h = blockIdx.y;
-  const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
-  if (row0 >= total_rows) return;
-  const int rows = min(kRows, total_rows - row0);
+  const int rows = min(kRows, total_rows);
   const int shared = group_shared_pages(a, group_of(a, b));
   const int32_t* table = a.page_indices + a.page_indptr[b] + shared;
   const int len = max(0, kv_tokens(a, b) - shared * a.page_len), prefix = len - n_tok;
   const int n_runs = (len + kRun - 1) / kRun;
   const int r0 = (int)((int64_t)n_runs * blockIdx.z / p.own_splits);
   const int r1 = (int)((int64_t)n_runs * (blockIdx.z + 1) / p.own_splits);
-  const int mine = r1 - r0 > warp ? ceil_div(r1 - r0 - warp, warps) : 0;   // this warp's runs r0 + warp + warps i
+  const int mine = max(0, (r1 - r0 - warp + warps - 1) / warps);   // this warp's runs r0 + warp + warps i
   const uint32_t ring = smem_u32(smem) + warp * kWarp;
 
   // the pages of this warp's runs 32 w .. 32 w + 31, one per lane
@@ -374,10 +386,10 @@ __global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const Prefi
   uint32_t qb[NR][D / 16][2];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    const int r = 8 * n + gq, R = row0 + r, tk = p.div_g.div(R);
+    const int r = 8 * n + gq, tk = p.div_g.div(r);
     const bool valid = r < rows;
     const uint16_t* q =
-        (const uint16_t*)a.q + ((int64_t)(tok0 + (valid ? tk : 0)) * a.Hq + h * a.g + (valid ? R - tk * a.g : 0)) * D + 2 * tq;
+        (const uint16_t*)a.q + ((int64_t)(tok0 + (valid ? tk : 0)) * a.Hq + h * a.g + (valid ? r - tk * a.g : 0)) * D + 2 * tq;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       qb[n][k][0] = valid ? __ldg((const uint32_t*)(q + 16 * k)) : 0u;
@@ -422,7 +434,7 @@ __global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const Prefi
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int r = 8 * n + 2 * tq + j, node = p.div_g.div(row0 + r);
+          const int r = 8 * n + 2 * tq + j, node = p.div_g.div(r);
           seen[j] = r < rows ? (uint32_t)seen_columns(a, tok0 + node, node, c0, prefix, len) : 0u;
         }
       }
@@ -545,7 +557,7 @@ __global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const Prefi
     }
   __syncthreads();
   for (int e = threadIdx.x; e < rows * (D / 4); e += blockDim.x) {
-    const int r = e / (D / 4), quad = e % (D / 4), R = row0 + r, tk = p.div_g.div(R);
+    const int r = e / (D / 4), quad = e % (D / 4), tk = p.div_g.div(r);
     float M = -INFINITY;
     for (int w = 0; w < warps; ++w) M = fmaxf(M, ml[w][r].x);
     const float base = M == -INFINITY ? 0.0f : M;
@@ -560,21 +572,24 @@ __global__ void __launch_bounds__(32 * kMaxOwnWarps) plan_own_kernel(const Prefi
       acc.z = fmaf(f, v.z, acc.z);
       acc.w = fmaf(f, v.w, acc.w);
     }
-    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g, part = row * p.own_splits + blockIdx.z;
+    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + r - tk * a.g, part = row * p.own_splits + blockIdx.z;
     *(float4*)(p.own_o + part * D + quad * 4) = acc;
     if (quad == 0) p.own_ml[part] = make_float2(M, L);
   }
+  pdl_wait();
 }
 
-// Shared memory per warp: its ring, later its O; the plan's CTA needs less.
+// Shared memory of own_attn_kernel: the rings (later the warps' O), barriers, (m, l).
 template <int D, int NR>
 constexpr size_t own_smem() {
   constexpr size_t ring = (size_t)kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)8 * NR * (D + 4) * 4;
-  return ring > o ? ring : o;
+  static_assert(ring >= o, "the rings hold the warps' O");
+  return kOwnWarps * (ring + 8 * kOwnStages + 8 * 8 * NR);
 }
-static_assert(2 * own_smem<64, 1>() >= (64 + 4) * 4 + kPlanCache * 8, "the plan's arrays");
+// with prefix_attn_kernel's CTA beside it (and 1 KB that the system takes for each)
+static_assert(own_smem<128, 2>() + Shape<128>::kSmem + 2048 <= 228 * 1024, "both fit an SM");
 
-// --------------------------------------------------------------- second kernel
+// ------------------------------------------------------------------- work items
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
 // every block at once: K0 V0 K1 V1 ..; two block streams start with both streams' keys:
 // K0 K1 V0 K2 V1 K3 ..
@@ -587,14 +602,14 @@ __device__ __forceinline__ bool masked_block(const Item& it, int j) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kBoundThreads, 1)
     prefix_attn_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kv_map) {
   using S = Shape<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   Bars& bars = *reinterpret_cast<Bars*>(smem + S::kOffBars);
   const SharedAttnParams& a = p.a;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  pdl_trigger();                                        // own_attn_kernel may start beside this one
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -639,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 4) {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = (warp - 4) >> 2, quarter = warp & 3;
     const int r_local = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -870,13 +886,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         part[128 * D + 128 + r_local] = l;
       }
     }
-  } else if (warp == 0) {
+  } else {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+  if (warp == 0) {
     // ------------------------------------------------------------ items and TMA producer
     // Item k + 1 is claimed and read while item k loads.  Lane r brings the r-th copy of a
     // block.  The page of load x + 4 is fetched while load x is issued (unrolled by four,
     // so that no register that a fetch is still filling is moved).
     pdl_wait();
-    pdl_trigger();
     const int total = __ldcg(&p.head->total);
     const int copies = kBlock / p.copy_tokens;
     bool ok = true;
@@ -1081,27 +1098,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars.full[slot], (pos / S::kSlots) & 1, p.wait_limit));
         if (!ok) break;
         const uint32_t vb = smem_u32(smem + S::kOffRing + slot * S::kSlotBytes);
-        const int first = max(half * 64, it.prefix - c0);         // tokens before it are the prefix
-        for (int x = first * (D / 8) + lane; x < (half + 1) * 64 * (D / 8); x += 32) {
+        auto at = [&](int x) -> uint32_t {                // 16-byte piece x of the block's values, token by token
           const int tok = x / (D / 8), ch = x % (D / 8);
-          const uint32_t at =
-              vb + (tok >> 3) * S::kGroupBytes + (ch >> 3) * 1024 + (tok & 7) * 128 + (((ch & 7) ^ (tok & 7)) << 4);
-          if (c0 + tok >= it.tokens) {
-            st_shared_v4(at, 0u, 0u, 0u, 0u);
-          } else {
-            const uint4 v = ld_shared_v4(at);
-            const int tree = c0 + tok - it.prefix;      // causal rows past the notes keep the value as it is
-            if ((odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w)) && tree < 32 * kMaxTreeWords) {
+          return vb + (tok >> 3) * S::kGroupBytes + (ch >> 3) * 1024 + (tok & 7) * 128 + (((ch & 7) ^ (tok & 7)) << 4);
+        };
+        const int lo = max(half * 64, it.prefix - c0);  // tokens before it are the prefix
+        const int end = min((half + 1) * 64, max(lo, it.tokens - c0)), stop = end * (D / 8);
+        for (int x = lo * (D / 8) + lane; x < stop; x += 32 * 8) {
+          uint4 v[8];                                   // eight pieces in flight
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = x + 32 * u < stop ? ld_shared_v4(at(x + 32 * u)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int y = x + 32 * u, tree = c0 + y / (D / 8) - it.prefix;
+            // causal rows past the notes keep the value as it is
+            if ((odd2(v[u].x) || odd2(v[u].y) || odd2(v[u].z) || odd2(v[u].w)) && tree < 32 * kMaxTreeWords) {
               auto fix = [](uint32_t w) {
                 if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
                 if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
                 return w;
               };
-              st_shared_v4(at, fix(v.x), fix(v.y), fix(v.z), fix(v.w));
+              st_shared_v4(at(y), fix(v[u].x), fix(v[u].y), fix(v[u].z), fix(v[u].w));
               atomicOr(&odd[tree >> 5], 1u << (tree & 31));
             }
           }
         }
+        for (int x = max(end, half * 64) * (D / 8) + lane; x < (half + 1) * 64 * (D / 8); x += 32)
+          if (c0 + x / (D / 8) >= it.tokens) st_shared_v4(at(x), 0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
         __threadfence_block();
         __syncwarp();
@@ -1111,6 +1134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       base += 2 * n;
     }
     if (!ok && lane == 0) give_up(p, 91);
+  }
   }
   tc_fence_before();
   __syncthreads();
@@ -1257,7 +1281,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const PrefixPa
 }
 
 struct PrefixPlan {
-  int few, own_rows, own_tiles, own_splits, own_warps, max_items, ctas;
+  int few, own_rows, own_splits, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
@@ -1278,25 +1302,13 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   const int64_t rows = (int64_t)max_qo_len * g;
   f.few = rows <= kFewRows;
   f.own_rows = rows <= 8 ? 8 : 16;
-  f.own_tiles = f.few ? 1 : 0;
   f.ctas = sm_count();
-  // Own columns in the first kernel: slices for about three CTAs of four warps per SM, each
-  // warp with two runs at least; where there are more (request, head) pairs than that,
-  // CTAs of three or two warps if they then all run at once.
+  // own columns: slices for about six CTAs of two warps per SM, each warp with two runs at least
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
   f.own_splits = 1;
-  f.own_warps = kMaxOwnWarps;
-  if (f.few) {
-    const int64_t pairs = std::max<int64_t>((int64_t)batch * Hkv, 1);
-    f.own_splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({3ll * f.ctas / pairs, (own + 8 * kRun - 1) / (8 * kRun), kMaxOwnSplits}));
-    const int per_warp = D == 128 ? (int)own_smem<128, 2>() : (int)own_smem<64, 2>();
-    for (int w = kMaxOwnWarps; w >= 2; --w)
-      if (pairs * f.own_splits <= (int64_t)f.ctas * ((227 * 1024) / (w * per_warp + 3 * 1024))) {
-        f.own_warps = w;
-        break;
-      }
-  }
+  if (f.few)
+    f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({6ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
+                                                                (own + 4 * kRun - 1) / (4 * kRun), kMaxOwnSplits}));
   int64_t units = ((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups;
   if (!f.few) units += ((int64_t)total_q * g + kTileRows - 1) / kTileRows + batch;
   f.max_items = (int)std::min<int64_t>(units * Hkv + 2 * f.ctas, 1 << 28);
@@ -1329,12 +1341,12 @@ int encode_kv(CUtensorMap* map, const SharedAttnParams& a, int copy_tokens) {
 }
 
 template <int D, int NR>
-int launch_own(const PrefixParams& p, const PrefixPlan& f, const CUtensorMap& map, cudaStream_t stream) {
-  const size_t smem = f.own_warps * own_smem<D, NR>() + 1024;
-  if (int rc = ensure_smem_attr((const void*)plan_own_kernel<D, NR>, kMaxOwnWarps * own_smem<D, NR>() + 1024)) return rc;
-  const dim3 grid = f.few ? dim3(1 + p.a.batch * p.own_tiles, p.a.Hkv, p.own_splits) : dim3(1);
-  PTS_CUDA_TRY(launch_pdl(plan_own_kernel<D, NR>, grid, dim3(32 * f.own_warps), smem, stream, p, map));
-  return launch_status("plan_own_kernel");
+int launch_own(const PrefixParams& p, const CUtensorMap& map, cudaStream_t stream) {
+  constexpr size_t smem = own_smem<D, NR>();
+  if (int rc = ensure_smem_attr((const void*)own_attn_kernel<D, NR>, smem, true)) return rc;
+  PTS_CUDA_TRY(launch_pdl(own_attn_kernel<D, NR>, dim3(p.a.batch, p.a.Hkv, p.own_splits), dim3(32 * kOwnWarps), smem,
+                          stream, p, map));
+  return launch_status("own_attn_kernel");
 }
 
 template <int D>
@@ -1342,11 +1354,22 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
   CUtensorMap run_map, block_map;
   if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
   if (int rc = encode_kv<D>(&block_map, p.a, p.copy_tokens)) return rc;
-  if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, f, run_map, stream) : launch_own<D, 2>(p, f, run_map, stream))
-    return rc;
+  PTS_CUDA_TRY(launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p));
+  if (int rc = launch_status("plan_kernel")) return rc;
   if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem)) return rc;
+  // setmaxnreg.inc would wait for good for registers that the launch does not have
+  static std::atomic<int> regs{0};
+  if (!regs.load()) {
+    cudaFuncAttributes attr;
+    PTS_CUDA_TRY(cudaFuncGetAttributes(&attr, (const void*)prefix_attn_kernel<D>));
+    regs.store(attr.numRegs);
+  }
+  if (regs.load() < kLaunchRegs)
+    return set_error(PTS_ERR_CUDA, "prefix_attn_kernel was built with %d registers (%d needed)", regs.load(), kLaunchRegs);
   PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
   if (int rc = launch_status("prefix_attn_kernel")) return rc;
+  if (f.few)
+    if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, run_map, stream) : launch_own<D, 2>(p, run_map, stream)) return rc;
   const int row_tiles = (int)(((int64_t)max_qo_len * p.a.g + kJoinRows - 1) / kJoinRows);
   PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(kJoinThreads), 0,
                           stream, p, row_tiles));
@@ -1390,7 +1413,6 @@ int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, i
   p.entries = (Entry*)(ws + f.entries);
   p.items = (Item*)(ws + f.items);
   p.parts = (float*)(ws + f.parts);
-  p.own_tiles = f.own_tiles;
   p.own_splits = f.own_splits;
   p.own_o = (float*)(ws + f.own_o);
   p.own_ml = (float2*)(ws + f.own_ml);
