@@ -147,4 +147,6 @@ def check(code: int, fn: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    code = getattr(_lib or lib(), name)(*args)
+    if code != PTS_OK:
+        check(code, name)

@@ -47,8 +47,8 @@ constexpr int kBoundThreads = 512;        // the launch bound that gives 128 reg
 static_assert(128 * kHelperRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, "the split draws on the launch's registers");
 constexpr int kMaxSplits = 32;            // block ranges of a column set
 constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in own_attn_kernel
+constexpr int kDirectCost = 3600;          // in tokens' time: the rounds' 3 us count 600 each
 constexpr int kFewRows = 16;              // rows per KV head up to which own_attn_kernel takes them
-constexpr int kMaxTreeWords = PTS_MAX_TREE_NODES / 32;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
 
@@ -66,7 +66,7 @@ struct Shape {
   static constexpr uint32_t kOffQ = 0;
   static constexpr uint32_t kOffRing = 2 * kSlotBytes;
   static constexpr uint32_t kOffBars = kOffRing + kSlots * kSlotBytes;
-  static constexpr uint32_t kSmem = kOffBars + 1408;            // barriers
+  static constexpr uint32_t kSmem = kOffBars + 512;             // barriers
   static constexpr int kPartFloats = 2 * 128 * (D + 2);         // one item's part: two streams' rows
 };
 static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared memory above 227 KB");
@@ -106,9 +106,9 @@ struct __align__(16) Bars {
   uint32_t tmem;
   // masked value blocks so far: in shared memory; gone over by warps 2 and 3
   volatile int arrived, cleaned[2];
-  uint32_t odd[4][2][kMaxTreeWords];      // by item count mod 4 and warp: tree slots with infinities or NaN in V
+  volatile int odd[4][2];   // by item count mod 4 and warp: V held infinities or NaN in masked blocks
 };
-static_assert(sizeof(Bars) <= 1408, "barrier block");
+static_assert(sizeof(Bars) <= 512, "barrier block");
 
 struct PrefixParams {
   SharedAttnParams a;
@@ -127,7 +127,7 @@ struct PrefixParams {
   Item* items;
   float* parts;
   // own columns in own_attn_kernel
-  int own_splits;
+  int own_splits;           // slices of a request's columns
   float* own_o;             // [T * Hq][own_splits][D]
   float2* own_ml;           // [T * Hq][own_splits]
 
@@ -182,23 +182,24 @@ __device__ __forceinline__ bool odd2(uint32_t w) {
 
 // ------------------------------------------------------------------------- plan
 constexpr int kPlanThreads = 256;
-constexpr int kOwnWarps = 2;
+constexpr int kOwnWarps = 2, kDirectWarps = 8;
 constexpr int kOwnStages = 2;
-constexpr int kPlanCache = 512;           // entries whose shapes the plan keeps in shared memory
+constexpr int kPlanCache = 512;           // entries that the plan keeps in shared memory
 
 // The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
 // and end cost about one and a half), and the launch about the larger of the total over
 // the CTAs and the large items' rounds; the cheapest of up to 32 ranges of
 // ceil(longest / k) blocks is taken.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p) {
-  __shared__ __align__(8) int sums[64 + 4 + 2 * kPlanCache];         // [2][32] items, large items; red; shapes
+  __shared__ int sums[64 + 4];                          // [2][32] items, large items; red
+  __shared__ Entry cache[kPlanCache];                   // the first entries, as in p.entries
   const SharedAttnParams& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int warps = kPlanThreads / 32, threads = kPlanThreads;
   pdl_wait();
   pdl_trigger();
   int* red = sums + 64;                                 // longest, blocks, chunk, total
-  int2* shape = (int2*)(red + 4);                       // (units, blocks) of the first kPlanCache entries
+  Entry* entry = a.groups + (p.own_items ? a.batch : 0) <= kPlanCache ? cache : p.entries;
   if (tid < 68) sums[tid] = 0;
   for (int g = warp; g < a.groups; g += warps) {
     int lead;
@@ -207,24 +208,21 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
     const int tok0 = a.qo_indptr[b0], rows = (a.qo_indptr[b1] - tok0) * a.g;
     if (lane == 0) {
       const int tokens = rows > 0 ? pages * a.page_len : 0;
-      p.entries[g] = Entry{tokens, tokens, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0, rows > 0 ? pages : 0};
-      if (g < kPlanCache) shape[g] = make_int2(tiles_of(rows) * a.Hkv, blocks_of(tokens));
+      entry[g] = Entry{tokens, tokens, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0, rows > 0 ? pages : 0};
     }
   }
   __syncthreads();
   const int entries = a.groups + (p.own_items ? a.batch : 0);
   if (p.own_items) {
     for (int b = tid; b < a.batch; b += threads) {
-      const int tok0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - tok0, pages = p.entries[group_of(a, b)].pages;
-      const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0, e = a.groups + b;
-      p.entries[e] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
-      if (e < kPlanCache) shape[e] = make_int2(tiles_of(n * a.g) * a.Hkv, blocks_of(len));
+      const int tok0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - tok0, pages = entry[group_of(a, b)].pages;
+      const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0;
+      entry[a.groups + b] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
     }
     __syncthreads();
   }
   auto shape_of = [&](int e) -> int2 {
-    if (e < kPlanCache) return shape[e];
-    return make_int2(tiles_of(p.entries[e].rows) * a.Hkv, blocks_of(p.entries[e].tokens));
+    return make_int2(tiles_of(entry[e].rows) * a.Hkv, blocks_of(entry[e].tokens));
   };
   int longest = 1, blocks = 0;
   for (int e = tid; e < entries; e += threads) {
@@ -286,8 +284,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
         if (lane >= o) incl += y;
       }
       if (e < entries) {
-        p.entries[e].splits = splits;
-        p.entries[e].first = run + incl - n;
+        entry[e].splits = splits;
+        entry[e].first = run + incl - n;
       }
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
@@ -298,14 +296,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
   }
   __syncthreads();
   const int total = red[3];
+  if (entry != p.entries)
+    for (int e = tid; e < entries; e += threads) p.entries[e] = entry[e];
   for (int i = tid; i < total; i += threads) {
     int lo = 0, hi = entries;                           // the last entry whose first item is <= i
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (p.entries[mid].first <= i) lo = mid;
+      if (entry[mid].first <= i) lo = mid;
       else hi = mid;
     }
-    const Entry x = p.entries[lo];
+    const Entry x = entry[lo];
     const int u = small_div(i - x.first, x.splits), split = i - x.first - u * x.splits, tiles = tiles_of(x.rows);
     const int h = small_div(u, tiles), row0 = (u - h * tiles) * kTileRows;
     p.items[i] = Item{x.tokens, x.prefix, min(kTileRows, x.rows - row0), x.tok0, x.table, row0, h, lo >= a.groups,
@@ -314,40 +314,47 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
 }
 
 // ------------------------------------------------------------------ own columns
-// The own columns of a request with at most 8 NR rows.  The CTA's two warps take its
+// The own columns of a request with at most 8 NR rows.  The CTA's NW warps take its
 // 16-token runs in turn, each through a ring of its own, and compute
 //   S^T = K Q^T (16 tokens x 8 rows per product), O^T += V^T P^T,
 // P^T handed to the second product by movmatrix; the warps' O, m and l are added up at
 // the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
 // in use, and the 8 columns are query rows: half the products of the plain form at 8
 // rows or fewer.
-template <int D, int NR>
-__global__ void __launch_bounds__(32 * kOwnWarps, 7)
+// kDirect: all columns, the shared ones too, and the output itself: for small calls, where
+// reading a short prefix once per request costs less than the plan and the join.
+template <int D, int NR, int NW, bool kDirect>
+__global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
     own_attn_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap run_map) {
   using S = Shape<D>;
   constexpr int kRows = 8 * NR;
   constexpr uint32_t kStage = 2 * S::kRunBytes, kWarp = kOwnStages * kStage;
-  extern __shared__ __align__(1024) uint8_t smem[];      // the warps' rings; barriers and (m, l) behind
-  constexpr int warps = kOwnWarps;
+  extern __shared__ __align__(1024) uint8_t smem[];      // the warps' rings; barriers behind
+  constexpr int warps = NW;
   uint64_t(*full)[kOwnStages] = (uint64_t(*)[kOwnStages])(smem + warps * kWarp);
-  float2(*ml)[kRows] = (float2(*)[kRows])(smem + warps * kWarp + sizeof(uint64_t) * warps * kOwnStages);
+  // after the loop the rings hold the warps' O, [warps][kRows][D + 4], and (m, l)
+  constexpr int kStride = D + 4;
+  float2(*ml)[kRows] = (float2(*)[kRows])(smem + warps * kRows * kStride * 4);
   const SharedAttnParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
   if (lane < kOwnStages) mbar_init(&full[warp][lane], 1);
   fence_mbar_init();
   __syncwarp();
+  if (kDirect) pdl_wait();
   pdl_trigger();
-  // Nothing here depends on the two kernels before: what this one reads is not theirs, and
-  // everything before them had completed when they were launched.  It waits for them at the
-  // end, so that what follows may wait for this kernel alone.
+  // Beside the others nothing here depends on the two kernels before: what this one reads is not theirs, and
+  // everything before them had completed when they were launched.  Only the grid's last CTA
+  // waits for them, so that what follows may wait for this kernel alone while the other
+  // CTAs make room.
+  const bool last = !kDirect && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
   const int b = blockIdx.x, h = blockIdx.y;
   const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
   if (total_rows <= 0) {
-    pdl_wait();
+    if (last) pdl_wait();
     return;
   }
   const int rows = min(kRows, total_rows);
-  const int shared = group_shared_pages(a, group_of(a, b));
+  const int shared = kDirect ? 0 : group_shared_pages(a, group_of(a, b));
   const int32_t* table = a.page_indices + a.page_indptr[b] + shared;
   const int len = max(0, kv_tokens(a, b) - shared * a.page_len), prefix = len - n_tok;
   const int n_runs = (len + kRun - 1) / kRun;
@@ -538,8 +545,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 7)
     for (int x = i; x < loaded; ++x) mbar_wait(&full[warp][x % kOwnStages], (x / kOwnStages) & 1);
   }
   __syncthreads();
-  float* os = (float*)smem;                             // [warps][kRows][D + 4]
-  constexpr int kStride = D + 4;
+  float* os = (float*)smem;
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -572,22 +578,30 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 7)
       acc.z = fmaf(f, v.z, acc.z);
       acc.w = fmaf(f, v.w, acc.w);
     }
-    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + r - tk * a.g, part = row * p.own_splits + blockIdx.z;
+    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + r - tk * a.g;
+    if (kDirect) {
+      const float f = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;    // nothing seen: 0
+      *(uint2*)((uint16_t*)a.out + row * D + quad * 4) =
+          make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+      continue;
+    }
+    const int64_t part = row * p.own_splits + blockIdx.z;
     *(float4*)(p.own_o + part * D + quad * 4) = acc;
     if (quad == 0) p.own_ml[part] = make_float2(M, L);
   }
-  pdl_wait();
+  if (last) pdl_wait();
 }
 
-// Shared memory of own_attn_kernel: the rings (later the warps' O), barriers, (m, l).
-template <int D, int NR>
+// Shared memory of own_attn_kernel: the rings (later the warps' O, m and l), barriers.
+template <int D, int NR, int NW>
 constexpr size_t own_smem() {
-  constexpr size_t ring = (size_t)kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)8 * NR * (D + 4) * 4;
-  static_assert(ring >= o, "the rings hold the warps' O");
-  return kOwnWarps * (ring + 8 * kOwnStages + 8 * 8 * NR);
+  constexpr size_t ring = (size_t)kOwnStages * 2 * Shape<D>::kRunBytes, o = (size_t)8 * NR * ((D + 4) * 4 + 8);
+  static_assert(ring >= o, "the rings hold the warps' O, m and l");
+  return NW * (ring + 8 * kOwnStages);
 }
-// with prefix_attn_kernel's CTA beside it (and 1 KB that the system takes for each)
-static_assert(own_smem<128, 2>() + Shape<128>::kSmem + 2048 <= 228 * 1024, "both fit an SM");
+// with prefix_attn_kernel's CTA beside it (in whole KB, and one more that the system takes
+// for each)
+static_assert((own_smem<128, 2, kOwnWarps>() + 1023) / 1024 + (Shape<128>::kSmem + 1023) / 1024 + 2 <= 228, "both fit an SM");
 
 // ------------------------------------------------------------------- work items
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
@@ -830,8 +844,9 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
         l = mine * l + theirs * l2;
         m = M;
       }
-      // tree slots whose infinite or NaN values were taken out of V
-      const bool odd = it.own && __any_sync(0xffffffffu, (bars.odd[k & 3][0][lane] | bars.odd[k & 3][1][lane]) != 0u);
+      // infinite or NaN values of tree slots were taken out of V: the rows that see them get
+      // them from the cache
+      const bool odd = it.own && (bars.odd[k & 3][0] | bars.odd[k & 3][1]) != 0;
       // the part: O as [column quad][row] so that a warp stores 512 contiguous bytes
       float* part = p.parts + (int64_t)index * S::kPartFloats + (two ? t * (S::kPartFloats / 2) : 0);
       const int cb0 = two ? 0 : t * (D / 64), cb1 = two ? D / 32 : cb0 + D / 64;
@@ -851,24 +866,18 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
           }
         }
         tmem_ld_wait();
-        if (odd) {
-          // the rows that see them get them
-          for (int w = 0; w < kMaxTreeWords; ++w) {
-            uint32_t bits = bars.odd[k & 3][0][w] | bars.odd[k & 3][1][w];
-            for (; bits; bits &= bits - 1) {
-              const int slot = 32 * w + __ffs(bits) - 1, col = it.prefix + slot, blk = col / kBlock;
-              if (!valid || blk < it.ja || blk >= it.jb) continue;
-              if (!(seen_columns(a, it.tok0 + node, node, col & ~63, it.prefix, it.tokens) >> (col & 63) & 1ull)) continue;
-              const int pg = p.page_of(col), page = a.page_indices[it.table + pg];
-              if (page < 0 || page >= a.max_pages) continue;
-              const uint16_t* v = (const uint16_t*)a.kv +
-                                  (((int64_t)page * 2 + 1) * a.page_len + (col - pg * a.page_len)) * a.Hkv * D +
-                                  (int64_t)it.h * D + 32 * cb;
+        if (odd && valid) {
+          for (int col = max(it.ja * kBlock, it.prefix); col < min(it.jb * kBlock, it.tokens); ++col) {
+            if (!(seen_columns(a, it.tok0 + node, node, col & ~63, it.prefix, it.tokens) >> (col & 63) & 1ull)) continue;
+            const int pg = p.page_of(col), page = a.page_indices[it.table + pg];
+            if (page < 0 || page >= a.max_pages) continue;
+            const uint16_t* v = (const uint16_t*)a.kv +
+                                (((int64_t)page * 2 + 1) * a.page_len + (col - pg * a.page_len)) * a.Hkv * D +
+                                (int64_t)it.h * D + 32 * cb;
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const float y = bf16_bits_to_float(v[c]);
-                if (!(fabsf(y) < INFINITY)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
-              }
+            for (int c = 0; c < 32; ++c) {
+              const float y = bf16_bits_to_float(v[c]);
+              if (!(fabsf(y) < INFINITY)) o[c] = __float_as_uint(__uint_as_float(o[c]) + y);
             }
           }
         }
@@ -1076,17 +1085,17 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
     // A masked probability is 0, and 0 * v is 0 only for finite v.  Warps 2 and 3 each go
     // over half the tokens of an own item's masked value blocks while the scores' softmax
     // runs: slots from the length on (the rest of a page) are zeroed, and so are infinite
-    // or NaN values of tree slots, which are noted for the rows that do see them.
+    // or NaN values of tree slots, which is noted for the rows that do see them.
     const int half = warp - 2;
     bool ok = true;
     int base = 0, done = 0;                             // ring positions before this item; masked blocks so far
     Item it;
     for (int k = 0; ok; ++k) {
       if (!__all_sync(0xffffffffu, next_item(k, it))) break;
-      uint32_t* odd = bars.odd[k & 3][half];
-      odd[lane] = 0u;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.item_free[k & 1]);
+      if (lane == 0) {
+        bars.odd[k & 3][half] = 0;
+        mbar_arrive(&bars.item_free[k & 1]);
+      }
       const bool two = it.rows > 128;
       const int n = it.jb - it.ja;
       for (int j = it.own ? max(0, max(it.prefix, 0) / kBlock - it.ja) : n; ok && j < n; ++j) {
@@ -1110,16 +1119,14 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
           for (int u = 0; u < 8; ++u) v[u] = x + 32 * u < stop ? ld_shared_v4(at(x + 32 * u)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int y = x + 32 * u, tree = c0 + y / (D / 8) - it.prefix;
-            // causal rows past the notes keep the value as it is
-            if ((odd2(v[u].x) || odd2(v[u].y) || odd2(v[u].z) || odd2(v[u].w)) && tree < 32 * kMaxTreeWords) {
+            if (odd2(v[u].x) || odd2(v[u].y) || odd2(v[u].z) || odd2(v[u].w)) {
               auto fix = [](uint32_t w) {
                 if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
                 if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
                 return w;
               };
-              st_shared_v4(at(y), fix(v[u].x), fix(v[u].y), fix(v[u].z), fix(v[u].w));
-              atomicOr(&odd[tree >> 5], 1u << (tree & 31));
+              st_shared_v4(at(x + 32 * u), fix(v[u].x), fix(v[u].y), fix(v[u].z), fix(v[u].w));
+              bars.odd[k & 3][half] = 1;
             }
           }
         }
@@ -1146,24 +1153,22 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
 
 // ---------------------------------------------------------------- third kernel
 // A CTA joins 16 rows of a request and KV head: the parts of its group's shared columns,
-// and those of its own.  Every part's m and l come in at once and become weights
-// e^(m - M); then the O values are summed, a thread per row and column quad: four rows and
-// eight quads per warp, so that both the parts ([quad][row]) and the output are touched in
-// 64-byte pieces.  With few rows the parts are split over the spare threads too.  Bound by
-// the latency of reading what other SMs have just written, so every load is issued
-// before the first is used.
+// and those of its own.  A thread has a row and a column quad -- four rows and eight
+// quads per warp, so that both the parts ([quad][row]) and the output are touched in
+// 64-byte pieces -- and, with few rows, every slices-th of the parts.  Bound by the
+// latency of reading what other SMs have just written: the first O values are asked for
+// together with the parts' m and l, which become weights e^(m - M) meanwhile.
 constexpr int kJoinRows = 16;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 6;             // O values in flight per thread
 constexpr int kMaxParts = 2 * kMaxSplits;
 static_assert(kMaxOwnSplits <= kMaxSplits, "");
 
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const PrefixParams p, int row_tiles) {
+__global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const PrefixParams p, int row_tiles) {
   const SharedAttnParams& a = p.a;
   constexpr int kPart = Shape<D>::kPartFloats, kHalf = kPart / 2;
   __shared__ float w[kMaxParts][kJoinRows], lw[kMaxParts][kJoinRows];
-  __shared__ const float* src[2][kJoinRows];            // first part's O of the shared and the own columns
-  __shared__ int cnt[2][kJoinRows];
   __shared__ float inv[kJoinRows];
   __shared__ float4 sum[kJoinThreads];
   pdl_trigger();
@@ -1172,116 +1177,137 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const PrefixPa
   pdl_wait();                                           // (the lengths are no kernel's of this call)
   if (row0 >= total_rows) return;
   const int n = min(kJoinRows, total_rows - row0);
-  // Where row R's parts are: thread (set, row).  A stored part is [quad][128 rows] with m and
-  // l behind; the first kernel's are [quad] with (m, l) apart.
-  if (threadIdx.x < 2 * kJoinRows) {
-    const int set = threadIdx.x / kJoinRows, r = threadIdx.x % kJoinRows, R = row0 + r;
-    if (set == 1 && !p.own_items) {
-      const int tk = p.div_g.div(R);
-      const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g;
-      src[1][r] = p.own_o + row * p.own_splits * D;
-      cnt[1][r] = p.own_splits;
-    } else {
-      const Entry e = p.entries[set == 0 ? gi : a.groups + b];
-      const int in_entry = (tok0 - e.tok0) * a.g + R, tile = in_entry / kTileRows, in = in_entry % kTileRows;
-      src[set][r] = p.parts + ((int64_t)e.first + ((int64_t)h * tiles_of(e.rows) + tile) * e.splits) * kPart +
-                    (in >> 7) * kHalf + (in & 127) * 4;
-      cnt[set][r] = e.splits;
-    }
-  }
-  __syncthreads();
-  const int shared = cnt[0][0], own = cnt[1][0], parts = shared + own;
+  // A stored part is [quad][128 rows] with m and l behind; own_attn_kernel's are [quad] with
+  // (m, l) apart.
+  const Entry group = p.entries[gi];
+  Entry mine = group;
+  if (p.own_items) mine = p.entries[a.groups + b];
+  const int shared = group.splits, own = p.own_items ? mine.splits : p.own_splits, parts = shared + own;
+  auto part_of = [&](const Entry& e, int R, int& in) -> const float* {   // the first part's half with row R, its place
+    const int at = (tok0 - e.tok0) * a.g + R, tile = at / kTileRows;
+    in = at & 127;
+    return p.parts + ((int64_t)e.first + ((int64_t)h * tiles_of(e.rows) + tile) * e.splits) * kPart +
+           ((at >> 7) & 1) * kHalf;
+  };
+  auto row_of = [&](int R) -> int64_t {
+    const int tk = p.div_g.div(R);
+    return (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g;
+  };
+  const int units = (n + 3) / 4 * D, slices = max(1, kJoinThreads / units);
   const int64_t own_step = p.own_items ? kPart : D;
-#pragma unroll 4
+  // this thread's place in round `idx`: row, quad, first parts
+  int r = 0, quad = 0;
+  const float *s0 = nullptr, *s1 = nullptr;
+  auto place = [&](int unit) {
+    const int lo = unit & 31, hi = unit >> 5;
+    r = (hi / (D / 32)) * 4 + (lo & 3);
+    quad = (hi % (D / 32)) * 8 + (lo >> 2);
+    const int R = row0 + min(r, n - 1);
+    int in;
+    s0 = part_of(group, R, in);
+    s0 += quad * 512 + in * 4;
+    if (p.own_items) {
+      s1 = part_of(mine, R, in);
+      s1 += quad * 512 + in * 4;
+    } else {
+      s1 = p.own_o + row_of(R) * p.own_splits * D + quad * 4;
+    }
+  };
+  float4 v[kJoinAhead];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int k = k0 + u * slices;
+      if (k < parts) v[u] = __ldcg((const float4*)(k < shared ? s0 + (int64_t)k * kPart : s1 + (k - shared) * own_step));
+    }
+  };
+  int idx = threadIdx.x;
+  const bool busy = idx < units * slices;
+  if (busy) {
+    place(idx % units);
+    fetch(idx / units);
+  }
+#pragma unroll 2
   for (int e = threadIdx.x; e < parts * kJoinRows; e += kJoinThreads) {
-    const int r = e % kJoinRows, k = e / kJoinRows;
+    const int rr = e % kJoinRows, k = e / kJoinRows, R = row0 + rr;
     float m = -INFINITY, l = 0.0f;
-    if (r < n) {
+    if (rr < n) {
       if (k >= shared && !p.own_items) {
-        const float2 x = __ldcg(p.own_ml + (src[1][r] - p.own_o) / D + (k - shared));
+        const float2 x = __ldcg(p.own_ml + row_of(R) * p.own_splits + (k - shared));
         m = x.x;
         l = x.y;
       } else {
-        // src is (row & 127) * 4 floats into the part: m is 128 D + row & 127 floats in
-        const int set = k >= shared, at = (int)((src[set][r] - p.parts) % kHalf);
-        const float* part = src[set][r] - at + at / 4 + 128 * D + (int64_t)(set ? k - shared : k) * kPart;
-        m = __ldcg(part);
-        l = __ldcg(part + 128);
+        int in;
+        const float* s = k < shared ? part_of(group, R, in) + (int64_t)k * kPart
+                                    : part_of(mine, R, in) + (int64_t)(k - shared) * kPart;
+        m = __ldcg(s + 128 * D + in);
+        l = __ldcg(s + 128 * D + 128 + in);
       }
     }
-    w[k][r] = m;
-    lw[k][r] = l;
+    w[k][rr] = m;
+    lw[k][rr] = l;
   }
   __syncthreads();
   {
     // sixteen threads per row
-    const int r = threadIdx.x / 16, j = threadIdx.x % 16;
+    const int rr = threadIdx.x / 16, j = threadIdx.x % 16;
     float M = -INFINITY, L = 0.0f;
-    for (int k = j; k < parts; k += 16) M = fmaxf(M, w[k][r]);
+    for (int k = j; k < parts; k += 16) M = fmaxf(M, w[k][rr]);
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
     const float base = M == -INFINITY ? 0.0f : M;
     for (int k = j; k < parts; k += 16) {
-      const float x = fast_exp2(w[k][r] - base);
-      L = fmaf(x, lw[k][r], L);
-      w[k][r] = x;
+      const float x = fast_exp2(w[k][rr] - base);
+      L = fmaf(x, lw[k][rr], L);
+      w[k][rr] = x;
     }
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-    if (j == 0) inv[r] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;   // nothing seen: 0
+    if (j == 0) inv[rr] = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;   // nothing seen: 0
   }
   __syncthreads();
-  // units of four rows x eight quads per warp; `slices` threads share a unit's parts
-  const int units = (n + 3) / 4 * D, slices = max(1, kJoinThreads / units);
-  for (int idx = threadIdx.x; idx < units * slices; idx += kJoinThreads) {
-    const int unit = idx % units, slice = idx / units, lo = unit & 31, hi = unit >> 5;
-    const int r = (hi / (D / 32)) * 4 + (lo & 3), quad = (hi % (D / 32)) * 8 + (lo >> 2);
+  for (; idx < units * slices; idx += kJoinThreads) {
+    const int unit = idx % units, slice = idx / units;
+    if (idx != (int)threadIdx.x) {
+      place(unit);
+      fetch(slice);
+    }
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (r < n) {
-      const float* s0 = src[0][r] + quad * 512;
-      const float* s1 = src[1][r] + (p.own_items ? quad * 512 : quad * 4);
-      for (int k0 = slice; k0 < parts; k0 += 12 * slices) {
-        float4 v[12];
+    for (int k0 = slice; k0 < parts; k0 += kJoinAhead * slices) {
+      if (k0 != slice) fetch(k0);
 #pragma unroll
-        for (int u = 0; u < 12; ++u) {
-          const int k = k0 + u * slices;
-          if (k < parts) v[u] = __ldcg((const float4*)(k < shared ? s0 + (int64_t)k * kPart : s1 + (k - shared) * own_step));
-        }
-#pragma unroll
-        for (int u = 0; u < 12; ++u) {
-          const int k = k0 + u * slices;
-          const float x = k < parts ? w[k][r] : 0.0f;
-          if (x != 0.0f) {                              // a part of no columns has no O
-            o.x = fmaf(x, v[u].x, o.x);
-            o.y = fmaf(x, v[u].y, o.y);
-            o.z = fmaf(x, v[u].z, o.z);
-            o.w = fmaf(x, v[u].w, o.w);
-          }
+      for (int u = 0; u < kJoinAhead; ++u) {
+        const int k = k0 + u * slices;
+        const float x = k < parts ? w[k][r] : 0.0f;
+        if (x != 0.0f) {                                // a part of no columns has no O
+          o.x = fmaf(x, v[u].x, o.x);
+          o.y = fmaf(x, v[u].y, o.y);
+          o.z = fmaf(x, v[u].z, o.z);
+          o.w = fmaf(x, v[u].w, o.w);
         }
       }
     }
-    if (slices > 1) {                                   // (then units * slices <= the CTA: one round)
+    if (slices > 1) {                                   // (then units * slices is the CTA's threads: one round)
       sum[idx] = o;
       __syncthreads();
       if (slice > 0) return;
       for (int i = 1; i < slices; ++i) {
-        const float4 v = sum[unit + i * units];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
+        const float4 y = sum[unit + i * units];
+        o.x += y.x;
+        o.y += y.y;
+        o.z += y.z;
+        o.w += y.w;
       }
     }
     if (r >= n) continue;
     const float f = inv[r];
-    const int R = row0 + r, tk = p.div_g.div(R);
-    *(uint2*)((uint16_t*)a.out + ((int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g) * D + quad * 4) =
+    *(uint2*)((uint16_t*)a.out + row_of(row0 + r) * D + quad * 4) =
         make_uint2(pack_bf16x2(o.x * f, o.y * f), pack_bf16x2(o.z * f, o.w * f));
   }
 }
 
 struct PrefixPlan {
-  int few, own_rows, own_splits, max_items, ctas;
+  int few, direct, own_rows, own_splits, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
@@ -1303,6 +1329,18 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   f.few = rows <= kFewRows;
   f.own_rows = rows <= 8 ? 8 : 16;
   f.ctas = sm_count();
+  // One launch that reads each request's columns takes about 3 us + 5 ns a token for each
+  // round of (request, KV head) pairs over the SMs (512 tokens: 6.4 us at 48 pairs of
+  // head_dim 64, 7.7 at 128 pairs of 128; 1900: 12.4 and 14.4); the plan, the work items
+  // and the join take 16 to 25 us for the same calls.
+  f.direct = f.few && ((batch * (int64_t)Hkv + f.ctas - 1) / f.ctas) * (600 + (int64_t)max_kv_len) <= kDirectCost;
+  if (f.direct) {
+    f.own_splits = 1;
+    f.max_items = 0;
+    f.head = f.entries = f.items = f.parts = f.own_ml = f.own_o = 0;
+    f.bytes = 256;
+    return f;
+  }
   // own columns: slices for about six CTAs of two warps per SM, each warp with two runs at least
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
   f.own_splits = 1;
@@ -1340,23 +1378,30 @@ int encode_kv(CUtensorMap* map, const SharedAttnParams& a, int copy_tokens) {
   return encode_tiled_bf16_sw128(map, 5, a.kv, dims, strides, box);
 }
 
-template <int D, int NR>
+template <int D, int NR, int NW, bool kDirect>
 int launch_own(const PrefixParams& p, const CUtensorMap& map, cudaStream_t stream) {
-  constexpr size_t smem = own_smem<D, NR>();
-  if (int rc = ensure_smem_attr((const void*)own_attn_kernel<D, NR>, smem, true)) return rc;
-  PTS_CUDA_TRY(launch_pdl(own_attn_kernel<D, NR>, dim3(p.a.batch, p.a.Hkv, p.own_splits), dim3(32 * kOwnWarps), smem,
-                          stream, p, map));
+  constexpr size_t smem = own_smem<D, NR, NW>();
+  auto kernel = own_attn_kernel<D, NR, NW, kDirect>;
+  if (int rc = ensure_smem_attr((const void*)kernel, smem, true)) return rc;
+  PTS_CUDA_TRY(launch_pdl(kernel, dim3(p.a.batch, p.a.Hkv, p.own_splits), dim3(32 * NW), smem, stream, p, map));
   return launch_status("own_attn_kernel");
 }
 
 template <int D>
 int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cudaStream_t stream) {
   CUtensorMap run_map, block_map;
-  if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
+  if (f.few)
+    if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
+  if (f.direct)
+    return f.own_rows == 8 ? launch_own<D, 1, kDirectWarps, true>(p, run_map, stream)
+                           : launch_own<D, 2, kDirectWarps, true>(p, run_map, stream);
   if (int rc = encode_kv<D>(&block_map, p.a, p.copy_tokens)) return rc;
+  // (the small kernels ask for the same shared-memory split, which an SM changes only when idle)
+  if (int rc = ensure_smem_attr((const void*)plan_kernel, 1, true)) return rc;
+  if (int rc = ensure_smem_attr((const void*)join_parts_kernel<D>, 1, true)) return rc;
   PTS_CUDA_TRY(launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p));
   if (int rc = launch_status("plan_kernel")) return rc;
-  if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem)) return rc;
+  if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem, true)) return rc;
   // setmaxnreg.inc would wait for good for registers that the launch does not have
   static std::atomic<int> regs{0};
   if (!regs.load()) {
@@ -1369,7 +1414,9 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
   PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
   if (int rc = launch_status("prefix_attn_kernel")) return rc;
   if (f.few)
-    if (int rc = f.own_rows == 8 ? launch_own<D, 1>(p, run_map, stream) : launch_own<D, 2>(p, run_map, stream)) return rc;
+    if (int rc = f.own_rows == 8 ? launch_own<D, 1, kOwnWarps, false>(p, run_map, stream)
+                                 : launch_own<D, 2, kOwnWarps, false>(p, run_map, stream))
+      return rc;
   const int row_tiles = (int)(((int64_t)max_qo_len * p.a.g + kJoinRows - 1) / kJoinRows);
   PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(kJoinThreads), 0,
                           stream, p, row_tiles));

@@ -613,51 +613,51 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
     ``cache_extend`` gives these tensors for forked sequences.  ``max_own_len`` bounds
     the tokens after the shared pages, where the caller knows it; it and
     ``max_kv_len`` only choose the schedule."""
-    dev = q.device
-    if dev.type != "cuda":
+    index = q.get_device()
+    if index < 0:
         raise ValueError("tensors must be on a CUDA device (this path has no CPU implementation)")
-    if q.dtype not in (torch.bfloat16, torch.float32) or kv_layer.dtype != q.dtype:
+    if (q.dtype is not torch.bfloat16 and q.dtype is not torch.float32) or kv_layer.dtype is not q.dtype:
         raise ValueError("tree attention takes bf16 or fp32 queries and a cache of the same type")
-    if q.dim() != 3 or kv_layer.dim() != 5 or kv_layer.shape[1] != 2 or kv_layer.shape[4] != q.shape[2]:
-        raise ValueError("q must be [T, Hq, D] and kv_layer [max_pages, 2, page_len, Hkv, D] with the same D")
-    if not q.is_contiguous() or not kv_layer.is_contiguous():
-        raise ValueError("q and kv_layer must be contiguous")
-    if kv_layer.device != dev:
-        raise ValueError("all tensors must be on the same device")
+    if q.dim() != 3 or kv_layer.dim() != 5 or not q.is_contiguous() or not kv_layer.is_contiguous():
+        raise ValueError("q [T, Hq, D] and kv_layer [max_pages, 2, page_len, Hkv, D] must be contiguous")
     T, Hq, D = q.shape
-    P, _, pl, Hkv, _ = kv_layer.shape
-    B = _cache_ints("qo_indptr", qo_indptr, dev).numel() - 1
-    G = _cache_ints("shared_pages", shared_pages, dev).numel()
-    _cache_ints("page_indptr", page_indptr, dev, B + 1)
-    _cache_ints("page_indices", page_indices, dev)
-    _cache_ints("last_page_len", last_page_len, dev, B)
-    _cache_ints("group_indptr", group_indptr, dev, G + 1)
-    words = 1
+    P, two, pl, Hkv, D2 = kv_layer.shape
+    if two != 2 or D2 != D:
+        raise ValueError("q must be [T, Hq, D] and kv_layer [max_pages, 2, page_len, Hkv, D] with the same D")
+    if kv_layer.get_device() != index:
+        raise ValueError("all tensors must be on the same device")
+    B = _cache_ints("qo_indptr", qo_indptr, index).shape[0] - 1
+    G = _cache_ints("shared_pages", shared_pages, index).shape[0]
+    _cache_ints("page_indptr", page_indptr, index, B + 1)
+    _cache_ints("page_indices", page_indices, index)
+    _cache_ints("last_page_len", last_page_len, index, B)
+    _cache_ints("group_indptr", group_indptr, index, G + 1)
+    bits, words = None, 1
     if mask_bits is not None:
-        if mask_bits.dtype != torch.int64 or mask_bits.dim() != 2 or not mask_bits.is_contiguous() or \
-                mask_bits.shape[0] < T or mask_bits.device != dev:
+        if mask_bits.dtype is not torch.int64 or mask_bits.dim() != 2 or not mask_bits.is_contiguous() or \
+                mask_bits.shape[0] < T or mask_bits.get_device() != index:
             raise ValueError("mask_bits must be a contiguous int64 [T, mask_words] tensor on the same device")
-        words = mask_bits.shape[1]
+        bits, words = mask_bits.data_ptr(), mask_bits.shape[1]
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like q")
     own = int(max_own_len) if max_own_len is not None else 0
-    es = q.element_size()
-    lib = _lib.lib()
-    with _on(dev):
-        nbytes = lib.pts_tree_attn_shared_workspace_size(B, G, T, int(max_qo_len), int(max_kv_len), own, Hq, Hkv, D, pl,
-                                                         es)
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-        err = workspace(dev, "attn_shared", 256)
+    es = 2 if q.dtype is torch.bfloat16 else 4
+    with _on(index):
+        nbytes = _lib.lib().pts_tree_attn_shared_workspace_size(B, G, T, max_qo_len, max_kv_len, own, Hq, Hkv, D, pl, es)
+        ws = qo_indptr.new_empty(max(nbytes, 256) // 4)
+        stream = _raw_stream(index)
+        err = _WS.get((index, stream, "attn_shared"))
+        if err is None:
+            err = workspace(q.device, "attn_shared", 256)
         _lib.call("pts_tree_attn_run_shared", q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(),
-                  page_indptr.data_ptr(), page_indices.data_ptr(), last_page_len.data_ptr(),
-                  mask_bits.data_ptr() if mask_bits is not None else None, words, group_indptr.data_ptr(),
-                  shared_pages.data_ptr(), G, out.data_ptr(), B, T, int(max_qo_len), int(max_kv_len), own, Hq, Hkv, D,
-                  pl, P, float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D), es, ws.data_ptr(), ws.numel(),
-                  err.data_ptr(), _stream(dev))
+                  page_indptr.data_ptr(), page_indices.data_ptr(), last_page_len.data_ptr(), bits, words,
+                  group_indptr.data_ptr(), shared_pages.data_ptr(), G, out.data_ptr(), B, T, max_qo_len, max_kv_len, own,
+                  Hq, Hkv, D, pl, P, sm_scale if sm_scale is not None else D ** -0.5, es, ws.data_ptr(), nbytes,
+                  err.data_ptr(), stream)
     if _CHECK_ATTENTION:
-        check_attention(dev)
+        check_attention(q.device)
     return out
 
 
@@ -846,53 +846,59 @@ def check_cache_status(status: torch.Tensor) -> None:
     raise (IndexError if code & 1 else ValueError if code & 2 else RuntimeError)(msg)
 
 
-def _on(dev: torch.device):
-    """The launches' device as the current one (a no-op context where it is already)."""
-    if dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _raw_stream(index: int) -> int:
+    """The current stream's handle on device ``index``."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _cache_ints(name: str, t: torch.Tensor, dev: torch.device, size: Optional[int] = None) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+def _on(index: int):
+    """Device ``index`` as the current one (a no-op context where it is already)."""
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _cache_ints(name: str, t: torch.Tensor, index: int, size: Optional[int] = None) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
-    if t.device != dev:
+    if t.get_device() != index:
         raise ValueError("all tensors must be on the same device")
-    if size is not None and t.numel() != size:
-        raise ValueError(f"{name} has {t.numel()} entries, expected {size}")
+    if size is not None and t.shape[0] != size:
+        raise ValueError(f"{name} has {t.shape[0]} entries, expected {size}")
     return t
 
 
-def _page_state(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: Optional[torch.Tensor]):
-    dev = page_refs.device
-    if dev.type != "cuda":
+def _page_state(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: Optional[torch.Tensor]) -> int:
+    index = page_refs.get_device()
+    if index < 0:
         raise ValueError("tensors must be on a CUDA device (this path has no CPU implementation)")
-    _cache_ints("page_refs", page_refs, dev)
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or \
+    _cache_ints("page_refs", page_refs, index)
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or \
             page_table.stride(0) < page_table.shape[1]:
         raise ValueError("page_table must be a 2-D int32 tensor with contiguous rows")
-    if page_table.device != dev:
+    if page_table.get_device() != index:
         raise ValueError("all tensors must be on the same device")
     if kv_lens is not None:
-        _cache_ints("kv_lens", kv_lens, dev, page_table.shape[0])
-    return dev
+        _cache_ints("kv_lens", kv_lens, index, page_table.shape[0])
+    return index
 
 
 def _page_pool(pool: torch.Tensor, page_refs: torch.Tensor):
     if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous [L, max_pages, 2, page_len, Hkv, D] tensor")
-    if pool.device != page_refs.device:
+    if pool.get_device() != page_refs.get_device():
         raise ValueError("all tensors must be on the same device")
-    if pool.shape[1] != page_refs.numel():
-        raise ValueError("page_refs needs one count per page of the pool")
     L, P, _, pl, H, D = pool.shape
+    if P != page_refs.shape[0]:
+        raise ValueError("page_refs needs one count per page of the pool")
     return L, P, pl, H * D * pool.element_size()
 
 
-def _status_word(status: Optional[torch.Tensor], dev: torch.device) -> torch.Tensor:
+def _status_word(status: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if status is None:
-        return torch.empty(1, dtype=torch.int32, device=dev)
-    return _cache_ints("status", status, dev, 1)
+        return like.new_empty(1)
+    return _cache_ints("status", status, like.get_device(), 1)
 
 
 def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, src_rows: torch.Tensor,
@@ -904,16 +910,17 @@ def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch
     partial page when one of its holders grows.  ``page_refs`` [P], ``page_table``
     [R, W] (-1 past a sequence's end) and ``kv_lens`` [R] are int32 and updated in
     place.  Returns the status word (``check_cache_status``)."""
-    dev = _page_state(page_refs, page_table, kv_lens)
-    n = _cache_ints("src_rows", src_rows, dev).numel()
-    _cache_ints("dst_rows", dst_rows, dev, n)
-    status = _status_word(status, dev)
+    index = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("src_rows", src_rows, index).shape[0]
+    _cache_ints("dst_rows", dst_rows, index, n)
+    status = _status_word(status, page_refs)
     if n == 0:
         return status.zero_()
-    with _on(dev):
+    R, W = page_table.shape
+    with _on(index):
         _lib.call("pts_cache_fork", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                  kv_lens.data_ptr(), page_table.shape[0], page_table.shape[1], page_refs.numel(), src_rows.data_ptr(),
-                  dst_rows.data_ptr(), n, status.data_ptr(), _stream(dev))
+                  kv_lens.data_ptr(), R, W, page_refs.shape[0], src_rows.data_ptr(), dst_rows.data_ptr(), n,
+                  status.data_ptr(), _raw_stream(index))
     return status
 
 
@@ -928,40 +935,42 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     last_page_len [B], seq_lens [B], shared_pages [G] or None) to write into; entries of
     page_indices past page_indptr[B] are left as they are.  A call that cannot be done
     (see the status) changes nothing."""
-    dev = _page_state(page_refs, page_table, kv_lens)
+    index = _page_state(page_refs, page_table, kv_lens)
     L, P, pl, row_bytes = _page_pool(pool, page_refs)
-    B, (R, W) = _cache_ints("rows", rows, dev).numel(), page_table.shape
+    B, (R, W) = _cache_ints("rows", rows, index).shape[0], page_table.shape
     if B == 0:
         raise ValueError("rows is empty")
     each, add_all = None, 0
     if isinstance(add, torch.Tensor):
-        each = _cache_ints("add", add, dev, B).data_ptr()
+        each = _cache_ints("add", add, index, B).data_ptr()
     else:
         add_all = int(add)
     G = 0
     if group_indptr is not None:
-        G = _cache_ints("group_indptr", group_indptr, dev).numel() - 1
+        G = _cache_ints("group_indptr", group_indptr, index).shape[0] - 1
         if G < 1:
             raise ValueError("group_indptr needs at least two entries")
     if out is None:
-        e = lambda n: torch.empty(n, dtype=torch.int32, device=dev)
-        out = (e(B + 1), e(B * W), e(B), e(B), e(G) if G else None)
+        e = page_refs.new_empty
+        indptr, indices, last, lens, shared = e(B + 1), e(B * W), e(B), e(B), e(G) if G else None
     else:
-        out = tuple(out[:5])
-        for name, t, n in zip(("page_indptr", "page_indices", "last_page_len", "seq_lens"), out, (B + 1, None, B, B)):
-            _cache_ints(name, t, dev, n)
+        indptr, indices, last, lens, shared = out[:5]
+        _cache_ints("page_indptr", indptr, index, B + 1)
+        _cache_ints("page_indices", indices, index)
+        _cache_ints("last_page_len", last, index, B)
+        _cache_ints("seq_lens", lens, index, B)
         if G:
-            _cache_ints("shared_pages", out[4], dev, G)
-    status = _status_word(status, dev)
-    nbytes = _lib.lib().pts_cache_workspace_size(P, B)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
+            _cache_ints("shared_pages", shared, index, G)
+    status = _status_word(status, page_refs)
+    words = 2 * P + 3 * B + 4                                # pts_cache_workspace_size
+    ws = page_refs.new_empty(words)
+    with _on(index):
         _lib.call("pts_cache_extend", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
                   page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), R, W, rows.data_ptr(), each, add_all,
-                  B, group_indptr.data_ptr() if G else None, G, out[0].data_ptr(), out[1].data_ptr(), out[1].numel(),
-                  out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr() if G else None, status.data_ptr(),
-                  ws.data_ptr(), nbytes, _stream(dev))
-    return CacheBatch(*out, status)
+                  B, group_indptr.data_ptr() if G else None, G, indptr.data_ptr(), indices.data_ptr(),
+                  indices.shape[0], last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else None,
+                  status.data_ptr(), ws.data_ptr(), 4 * words, _raw_stream(index))
+    return CacheBatch(indptr, indices, last, lens, shared, status)
 
 
 def cache_truncate(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, page_len: int,
@@ -970,18 +979,18 @@ def cache_truncate(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: t
     """Cut the listed sequences to ``new_lens`` tokens (int32 [n]; None frees them):
     pages past the new length lose this holder.  A sequence already shorter keeps its
     length.  Returns the status word; rows outside the table are skipped."""
-    dev = _page_state(page_refs, page_table, kv_lens)
-    n = _cache_ints("rows", rows, dev).numel()
+    index = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("rows", rows, index).shape[0]
     if new_lens is not None:
-        _cache_ints("new_lens", new_lens, dev, n)
-    status = _status_word(status, dev)
+        _cache_ints("new_lens", new_lens, index, n)
+    status = _status_word(status, page_refs)
     if n == 0:
         return status.zero_()
-    with _on(dev):
+    R, W = page_table.shape
+    with _on(index):
         _lib.call("pts_cache_truncate", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                  kv_lens.data_ptr(), page_table.shape[0], page_table.shape[1], page_refs.numel(), int(page_len),
-                  rows.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, n, status.data_ptr(),
-                  _stream(dev))
+                  kv_lens.data_ptr(), R, W, page_refs.shape[0], int(page_len), rows.data_ptr(),
+                  new_lens.data_ptr() if new_lens is not None else None, n, status.data_ptr(), _raw_stream(index))
     return status
 
 
@@ -989,16 +998,15 @@ def cache_compact(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch
     """Close the gaps of ``pool``: its n live pages end up in pages 0 .. n-1, moving
     only those at or past n.  Returns the new counts and table (the inputs keep their
     values), the page map and the counts."""
-    dev = _page_state(page_refs, page_table, None)
+    index = _page_state(page_refs, page_table, None)
     L, P, pl, row_bytes = _page_pool(pool, page_refs)
     R, W = page_table.shape
-    e = lambda *n: torch.empty(*n, dtype=torch.int32, device=dev)
-    out = CompactedCache(e(P), e(R, W), e(P), e(2))
-    nbytes = _lib.lib().pts_cache_workspace_size(P, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
+    refs, table, page_map, counts = (page_refs.new_empty(P), page_table.new_empty(R, W), page_refs.new_empty(P),
+                                     page_refs.new_empty(2))
+    words = 2 * P + 4                                        # pts_cache_workspace_size
+    ws = page_refs.new_empty(words)
+    with _on(index):
         _lib.call("pts_cache_compact", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
-                  page_table.data_ptr(), page_table.stride(0), R, W, out.page_refs.data_ptr(),
-                  out.page_table.data_ptr(), out.page_map.data_ptr(), out.counts.data_ptr(), ws.data_ptr(), nbytes,
-                  _stream(dev))
-    return out
+                  page_table.data_ptr(), page_table.stride(0), R, W, refs.data_ptr(), table.data_ptr(),
+                  page_map.data_ptr(), counts.data_ptr(), ws.data_ptr(), 4 * words, _raw_stream(index))
+    return CompactedCache(refs, table, page_map, counts)
