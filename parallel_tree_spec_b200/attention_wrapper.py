@@ -10,7 +10,10 @@ the paged cache + attention over it.  Behind it:
   bitmasks (``pts_tree_mask_from_bool``); a mask whose prefix columns are not
   all true is rejected with ``ValueError``;
 * mode "tree"/"prefill" without a mask and mode "decode": causal rows;
-* append: ``pts_kv_append``; attention: ``pts_tree_attn_run_any``.
+* append: ``pts_kv_append``; attention: ``pts_tree_attn_run_any``, or
+  ``pts_tree_attn_run_shared`` where the batch position names pages that its
+  requests share (``SharedKvCache.extend``, a beam search with
+  ``shared_prefix``): same result, the shared pages read once per group.
 
 No FlashInfer, no CPU path.  bf16 caches with head_dim 128, 16-token pages
 and GQA groups up to 16 run on the tcgen05 kernel; fp32 caches and other
@@ -154,7 +157,14 @@ class BeFlashinferWrapper:
         else:
             self.append_kv_cache(q, k, v, append_pos, cacheData, self.page_len)
         bp = plan["bp"]
-        out = K.tree_attention(q.contiguous(), cacheData, bp.seq_indptr, bp.kv_page_indptr, bp.kv_page_indices,
-                               bp.kv_last_page_len, plan["bits"], plan["max_qo"], plan["max_kv"],
-                               sm_scale=1.0 / math.sqrt(self._head_padded_dim))
+        scale = 1.0 / math.sqrt(self._head_padded_dim)
+        if bp.shared_pages is not None:
+            out = K.tree_attention_shared(q.contiguous(), cacheData, bp.seq_indptr, bp.kv_page_indptr,
+                                          bp.kv_page_indices, bp.kv_last_page_len, plan["bits"], plan["max_qo"],
+                                          plan["max_kv"], bp.group_indptr, bp.shared_pages,
+                                          max_own_len=bp.max_own_len, sm_scale=scale)
+        else:
+            out = K.tree_attention(q.contiguous(), cacheData, bp.seq_indptr, bp.kv_page_indptr, bp.kv_page_indices,
+                                   bp.kv_last_page_len, plan["bits"], plan["max_qo"], plan["max_kv"],
+                                   sm_scale=scale)
         return out.view(-1, self.hidden_size)

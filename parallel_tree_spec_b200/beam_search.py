@@ -59,6 +59,9 @@ class BeamSearchConfig:
     max_depth: int = 10        # number of decode steps
     temperature: float = 1.0   # softmax temperature
     use_cuda_graph: bool = False  # capture decode steps in a CUDA graph
+    # read the prompt's full pages once for all beams (tree_attention_shared) instead of once
+    # per beam; no counterpart in the reference, ignored with a sparse strategy
+    shared_prefix: bool = False
 
 
 def _copy_block(kvCachePool: KvCachePool, src_page: int, off: int) -> int:
@@ -163,6 +166,10 @@ class CudaGraphRunner:
             positions=torch.zeros(K, dtype=torch.int32, device=device),
         )
         _with_host_lens(self.batch_position, K, 0)
+        # the pages that the beams share: read by the captured attention when it was captured
+        # with them (``capture(..., shared_prefix=True)``)
+        self.group_indptr = torch.tensor([0, K], dtype=torch.int32, device=device)
+        self.shared_pages = torch.zeros(1, dtype=torch.int32, device=device)
 
     def _forward(self, model, flashinfer_wrapper, kvCachePool):
         return model(self.input_ids_buf, position_ids=self.position_ids_buf, past_key_values=None, use_cache=False,
@@ -170,9 +177,14 @@ class CudaGraphRunner:
                      flashinferWrapper=flashinfer_wrapper)
 
     def capture(self, model: torch.nn.Module, flashinfer_wrapper: BeFlashinferWrapper, kvCachePool: KvCachePool,
-                page_size: int, dtype: torch.dtype):
-        """Warm up on K scratch pages, then capture one decode forward."""
+                page_size: int, dtype: torch.dtype, shared_prefix: bool = False, max_kv_len: int = 1):
+        """Warm up on K scratch pages, then capture one decode forward.  With
+        ``shared_prefix`` the attention is captured for beams that share pages (any
+        number, also none, at a replay) and scheduled for ``max_kv_len`` tokens."""
         K_ = self.K
+        self.shared_pages.zero_()
+        self.batch_position.group_indptr = self.group_indptr if shared_prefix else None
+        self.batch_position.shared_pages = self.shared_pages if shared_prefix else None
         temp_pages = kvCachePool.allocate(K_)
         self.input_ids_buf.fill_(0)
         self.position_ids_buf.fill_(0)
@@ -180,7 +192,7 @@ class CudaGraphRunner:
         self.batch_position.kv_page_indices[:K_].copy_(torch.tensor(temp_pages, dtype=torch.int32, device=self.device))
         self.batch_position.kv_last_page_len.fill_(1)
         self.batch_position.positions.fill_(0)
-        _with_host_lens(self.batch_position, K_, 0)
+        _with_host_lens(self.batch_position, K_, max_kv_len - 1 if shared_prefix else 0)
         for _ in range(2):
             flashinfer_wrapper.prepareAttention("decode", self.batch_position, page_size, "NONE", dtype)
             self._forward(model, flashinfer_wrapper, kvCachePool)
@@ -202,6 +214,11 @@ class CudaGraphRunner:
         self.batch_position.kv_page_indices[:n_idx].copy_(batch_position.kv_page_indices)
         self.batch_position.kv_last_page_len.copy_(batch_position.kv_last_page_len)
         self.batch_position.positions.copy_(batch_position.positions)
+        if self.batch_position.shared_pages is not None:
+            if batch_position.shared_pages is not None:
+                self.shared_pages.copy_(batch_position.shared_pages)
+            else:
+                self.shared_pages.zero_()
         self.batch_position.host_qo_lens = batch_position.host_qo_lens
         self.batch_position.host_kv_lens = batch_position.host_kv_lens
         plan_pos = sparse_batch_position if sparse_batch_position is not None else self.batch_position
@@ -246,6 +263,7 @@ def beam_search(model: torch.nn.Module, request_kv_cache: RequestKvCache, input_
         kv_len += input_len
 
     use_sparse = sparse_strategy is not None and sparse_strategy.config.enabled
+    share = config.shared_prefix and not use_sparse
     cuda_runner = None
     if config.use_cuda_graph:                                          # :395-408
         if cuda_graph_runner is not None and cuda_graph_runner.graph is not None:
@@ -258,6 +276,9 @@ def beam_search(model: torch.nn.Module, request_kv_cache: RequestKvCache, input_
 
     tree = Tree(input_ids[0, -1], dtype)
     prompt_pages = list(request_kv_cache.kv_page_indices)
+    if share:                                  # full pages of the prompt, which no beam writes
+        beam_groups = torch.tensor([0, K_], dtype=torch.int32, device=device)
+        beam_shared = torch.tensor([kv_len // PAGE_SIZE], dtype=torch.int32, device=device)
     if use_sparse:                                                     # :415-430
         sparse_strategy.reset()
         q_vectors = None
@@ -324,6 +345,9 @@ def beam_search(model: torch.nn.Module, request_kv_cache: RequestKvCache, input_
 
         beam_pages_list = [node_pages[beam_node[k]] for k in range(K_)]
         full_batch_position = static_bp.fill(beam_pages_list, current_pos, PAGE_SIZE)
+        if share:
+            full_batch_position.group_indptr, full_batch_position.shared_pages = beam_groups, beam_shared
+            full_batch_position.max_own_len = current_pos + 1 - kv_len // PAGE_SIZE * PAGE_SIZE
         append_batch_position = None
         if use_sparse:
             sparse_pages_list = [sparse_strategy.filter_pages(pages, seq_len=current_pos, page_len=PAGE_SIZE)
@@ -349,7 +373,8 @@ def beam_search(model: torch.nn.Module, request_kv_cache: RequestKvCache, input_
                 fwd_kwargs["append_batch_position"] = append_batch_position
             outputs = model(beam_input_ids, **fwd_kwargs)
             if cuda_runner is not None and cuda_runner.graph is None:
-                cuda_runner.capture(model, flashinfer_wrapper, kvCachePool, PAGE_SIZE, dtype)
+                cuda_runner.capture(model, flashinfer_wrapper, kvCachePool, PAGE_SIZE, dtype, shared_prefix=share,
+                                    max_kv_len=kv_len + max_depth)
 
         # score and select: one fused selection, one copy to the host  :546-561
         scores, flat, step_p = K.beam_select(outputs.logits[:, -1, :], K_, T, cum)

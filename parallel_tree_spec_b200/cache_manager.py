@@ -17,11 +17,15 @@ device work goes through libpts_b200:
   request's page table, which is identical whenever the request owns
   physical pages 0..n-1 in order (the only case in which the reference's
   flat-slot arithmetic addresses the request's own pages).
+
+``SharedKvCache`` (no counterpart in the reference, whose requests share no pages)
+keeps the page state of many sequences on the device, where they may share pages:
+several samples of one prompt, beams, requests under one system prompt.
 """
 from __future__ import annotations
 
 import math
-from typing import List
+from typing import List, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -42,6 +46,11 @@ class KvCacheBatchPosition:
         self.positions = positions
         self.host_qo_lens = None
         self.host_kv_lens = None
+        # requests that share leading pages (SharedKvCache.extend, beam_search): groups of
+        # consecutive requests and each group's common pages, for tree_attention_shared
+        self.group_indptr = None
+        self.shared_pages = None
+        self.max_own_len = None
 
     def print_info(self):
         for k in ("seq_indptr", "kv_page_indptr", "kv_page_indices", "kv_last_page_len", "batch_indices", "positions"):
@@ -189,3 +198,126 @@ def getKvCacheBatchPosition(request_kv_caches: List[RequestKvCache], mode: str, 
     bp.host_qo_lens = app
     bp.host_kv_lens = kv_lens
     return bp
+
+
+class SharedKvCache:
+    """Sequences over a ``KvCachePool`` that share pages, their page state (counts of
+    holders, page tables, lengths) on the device.
+
+    ``fork`` makes a sequence hold another's pages without moving K/V; ``extend`` makes
+    room for new tokens, copying a partial last page that others hold too, and returns the
+    batch position for the append and the attention, with each group's common pages;
+    ``truncate`` and ``release`` give pages back; ``compact`` closes the pool's gaps.  Rows
+    (sequence numbers) and lengths may be lists or int32 tensors on the pool's device;
+    tensors keep every call free of host copies and synchronisations, so a step can be
+    captured in a CUDA graph (not ``compact``, which replaces the state's tensors).  A
+    call that cannot be done changes nothing; ``check`` raises for it.  The cache takes
+    all pages of the pool, which must be free, until ``close``."""
+
+    def __init__(self, pool: KvCachePool, max_sequences: int, max_pages_per_sequence: int):
+        if pool.num_free_pages() != pool.max_pages:
+            raise ValueError("the pool's pages must all be free")
+        self.pool = pool
+        self._held = pool.allocate(pool.max_pages)
+        dev = pool.cache_data.device
+        self.page_refs = torch.zeros(pool.max_pages, dtype=torch.int32, device=dev)
+        self.page_table = torch.full((max_sequences, max_pages_per_sequence), -1, dtype=torch.int32, device=dev)
+        self.kv_lens = torch.zeros(max_sequences, dtype=torch.int32, device=dev)
+        self._bound = [0] * max_sequences                 # upper bounds of the lengths, for schedules only
+        self._statuses: List[torch.Tensor] = []
+
+    def _ints(self, x) -> torch.Tensor:
+        if isinstance(x, torch.Tensor):
+            return x
+        return torch.tensor(list(x), dtype=torch.int32, device=self.page_refs.device)
+
+    def _note(self, status: torch.Tensor) -> None:
+        self._statuses.append(status)
+        del self._statuses[:-256]
+
+    def _limit(self) -> int:
+        return self.page_table.shape[1] * self.pool.page_len
+
+    def fork(self, src_rows, dst_rows) -> None:
+        """``dst_rows[i]`` becomes a fork of ``src_rows[i]`` (all read before any is
+        written; the destinations' former pages are given back)."""
+        self._note(K.cache_fork(self.page_refs, self.page_table, self.kv_lens, self._ints(src_rows),
+                                self._ints(dst_rows)))
+        if isinstance(src_rows, torch.Tensor) or isinstance(dst_rows, torch.Tensor):
+            self._bound = [max(self._bound)] * len(self._bound)
+        else:
+            old = list(self._bound)
+            for a, b in zip(src_rows, dst_rows):
+                if 0 <= a < len(old) and 0 <= b < len(old):
+                    self._bound[b] = old[a]
+
+    def extend(self, rows, add: Union[int, Sequence[int]], groups: Optional[Sequence[int]] = None) -> KvCacheBatchPosition:
+        """Room for ``add`` more tokens (an int, or one per row) in every listed sequence.
+        Returns the batch position of these rows: append positions of the new tokens, page
+        lists, and for ``groups`` (starts of consecutive groups of the listed rows and
+        their number at the end, by default one group of all) the pages that each group's
+        rows hold in common."""
+        r = self._ints(rows)
+        B = r.numel()
+        adds = [int(add)] * B if isinstance(add, int) else [int(n) for n in add]
+        if len(adds) != B:
+            raise ValueError(f"add has {len(adds)} entries, expected {B}")
+        dev = self.page_refs.device
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+        gi = i32([0, B]) if groups is None else self._ints(groups)
+        out = K.cache_extend(self.pool.cache_data, self.page_refs, self.page_table, self.kv_lens, r,
+                             adds[0] if len(set(adds)) == 1 else i32(adds), group_indptr=gi)
+        self._note(out.status)
+        seq = [0]
+        for n in adds:
+            seq.append(seq[-1] + n)
+        bp = KvCacheBatchPosition(i32(seq), out.page_indptr, out.page_indices, out.last_page_len, None, None)
+        bp.batch_indices, bp.positions = K.batch_positions(bp.seq_indptr, out.seq_lens, seq[-1])
+        if isinstance(rows, torch.Tensor):
+            top = max(self._bound) + max(adds)
+            self._bound = [min(top, self._limit())] * len(self._bound)
+            lens = [self._bound[0]] * B
+        else:
+            for row, n in zip(rows, adds):
+                if 0 <= row < len(self._bound):
+                    self._bound[row] = min(self._bound[row] + n, self._limit())
+            lens = [self._bound[row] if 0 <= row < len(self._bound) else 0 for row in rows]
+        bp.host_qo_lens, bp.host_kv_lens = adds, [max(1, n) for n in lens]
+        bp.group_indptr, bp.shared_pages = gi, out.shared_pages
+        return bp
+
+    def truncate(self, rows, new_lens=None) -> None:
+        """Cut the listed sequences to ``new_lens`` tokens (None: free them)."""
+        self._note(K.cache_truncate(self.page_refs, self.page_table, self.kv_lens, self.pool.page_len,
+                                    self._ints(rows), None if new_lens is None else self._ints(new_lens)))
+        if not isinstance(rows, torch.Tensor) and not isinstance(new_lens, torch.Tensor):
+            for i, row in enumerate(rows):
+                if 0 <= row < len(self._bound):
+                    self._bound[row] = min(self._bound[row], max(0, new_lens[i]) if new_lens is not None else 0)
+
+    def release(self, rows) -> None:
+        self.truncate(rows)
+
+    def compact(self) -> torch.Tensor:
+        """Close the pool's gaps; returns the map from old to new page (-1: free)."""
+        r = K.cache_compact(self.pool.cache_data, self.page_refs, self.page_table)
+        self.page_refs, self.page_table = r.page_refs, r.page_table
+        return r.page_map
+
+    def lengths(self) -> List[int]:
+        """The lengths, read from the device (they then also bound the schedules)."""
+        self._bound = self.kv_lens.tolist()
+        return list(self._bound)
+
+    def check(self) -> None:
+        """Raise for a call since the last check that could not be done."""
+        pending, self._statuses = self._statuses, []
+        if pending:
+            for code in torch.cat(pending).tolist():
+                K.raise_cache_status(code)
+
+    def close(self) -> None:
+        """Give the pool's pages back; the sequences are gone."""
+        if self._held:
+            self.pool.deallocate(self._held)
+            self._held = []

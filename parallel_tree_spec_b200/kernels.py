@@ -648,17 +648,29 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
         nbytes = _lib.lib().pts_tree_attn_shared_workspace_size(B, G, T, max_qo_len, max_kv_len, own, Hq, Hkv, D, pl, es)
         ws = qo_indptr.new_empty(max(nbytes, 256) // 4)
         stream = _raw_stream(index)
-        err = _WS.get((index, stream, "attn_shared"))
+        err = _ERROR_WORDS.get(index)
         if err is None:
-            err = workspace(q.device, "attn_shared", 256)
+            err = _error_word(index)
         _lib.call("pts_tree_attn_run_shared", q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(),
                   page_indptr.data_ptr(), page_indices.data_ptr(), last_page_len.data_ptr(), bits, words,
                   group_indptr.data_ptr(), shared_pages.data_ptr(), G, out.data_ptr(), B, T, max_qo_len, max_kv_len, own,
                   Hq, Hkv, D, pl, P, sm_scale if sm_scale is not None else D ** -0.5, es, ws.data_ptr(), nbytes,
-                  err.data_ptr(), stream)
+                  err.data_ptr() if err is not None else None, stream)
     if _CHECK_ATTENTION:
         check_attention(q.device)
     return out
+
+
+_ERROR_WORDS: Dict[int, torch.Tensor] = {}
+
+
+def _error_word(index: int) -> Optional[torch.Tensor]:
+    """The word in which tree_attention_shared's launches on a device report that they gave
+    up waiting: one for all streams and graphs, made outside of captures."""
+    if index not in _ERROR_WORDS and not torch.cuda.is_current_stream_capturing():
+        _ERROR_WORDS[index] = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()     # zero before another stream's launch writes it
+    return _ERROR_WORDS.get(index)
 
 
 # PTS_B200_CHECK=1: read the attention kernels' error word after every call
@@ -671,8 +683,8 @@ def check_attention(device: Optional[torch.device] = None) -> None:
     (pts_tree_attn_check: synchronises the stream, then clears the error)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     status = C.c_int(0)
-    for kind in ("attn", "attn_shared"):
-        ws = workspace(dev, kind, 256)
+    word = _error_word(dev.index if dev.index is not None else torch.cuda.current_device())
+    for ws in [workspace(dev, "attn", 256)] + ([word] if word is not None else []):
         _lib.call("pts_tree_attn_check", ws.data_ptr(), C.addressof(status), _stream(dev))
         if status.value != 0:
             break
@@ -839,7 +851,11 @@ def check_cache_status(status: torch.Tensor) -> None:
     """Raise for a status of the cache calls (reads it from the device): IndexError
     for a row outside the table, ValueError for a row listed twice, RuntimeError when
     the table is too narrow or the pool too small."""
-    code = int(status.item())
+    raise_cache_status(int(status.item()))
+
+
+def raise_cache_status(code: int) -> None:
+    """``check_cache_status`` for a status already on the host."""
     if code == 0:
         return
     msg = "; ".join(text for bit, text in CACHE_STATUS.items() if code & bit) or f"status {code}"

@@ -1,0 +1,240 @@
+"""Sequences that share pages, as they are used: ``SharedKvCache`` with the wrapper's
+append and attention over several steps (forks, copies on write, truncations, a
+compaction, graph replays) against dense attention over each sequence's own history;
+beam search with ``shared_prefix``; and a wait of the attention that runs out."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from parallel_tree_spec_b200 import beam_search as pbs
+from parallel_tree_spec_b200 import kernels as K
+from parallel_tree_spec_b200.attention_wrapper import AttentionRotaryParams, BeFlashinferWrapper
+from parallel_tree_spec_b200.cache_manager import KvCachePool, RequestKvCache, SharedKvCache
+from tests.test_gpu_attention_shared import Case, chain, tree
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+class History:
+    """Every sequence's keys and values as they should be, [tokens, 2, Hkv, D] a layer."""
+
+    def __init__(self, layers):
+        self.kv = {}
+        self.layers = layers
+
+    def append(self, row, k, v):
+        new = torch.stack([k, v], dim=2)                      # [layers, n, 2, Hkv, D]
+        old = self.kv.get(row)
+        self.kv[row] = new if old is None else torch.cat([old, new], dim=1)
+
+
+def dense(q, kv, mask):
+    """fp64 attention of q [n, Hq, D] over kv [L, 2, Hkv, D]; (o, sum p |v|)."""
+    g = q.shape[1] // kv.shape[2]
+    k, v = kv[:, 0].double().repeat_interleave(g, 1), kv[:, 1].double().repeat_interleave(g, 1)
+    s = torch.einsum("nhd,lhd->nhl", q.double(), k) / math.sqrt(q.shape[2])
+    p = torch.softmax(s.masked_fill(~mask[:, None], float("-inf")), -1)
+    return torch.einsum("nhl,lhd->nhd", p, v), torch.einsum("nhl,lhd->nhd", p, v.abs())
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,page", [(torch.bfloat16, 8, 2, 128, 16), (torch.bfloat16, 4, 4, 64, 32),
+                                                 (torch.float32, 4, 2, 64, 16), (torch.bfloat16, 2, 1, 64, 8)])
+def test_steps_of_shared_sequences(dtype, Hq, Hkv, D, page):
+    """A prompt, samples forked from it, single tokens and draft trees of which some
+    tokens are kept, a second generation of forks, a released sequence, a compaction.
+    Attention tolerance: probabilities and output rounded to the type (2 h with h its
+    half step, times sum p |v|), scores in fp32 (2^-12 covers (D + 3) 2^-24 |q||k| / sqrt D
+    at |q||k| below 300, twice)."""
+    layers, gen = 2, torch.Generator().manual_seed(D + page)
+    pool = KvCachePool(120, layers, Hkv, D, page, dtype, torch.device(DEV))
+    cache = SharedKvCache(pool, 8, 20)
+    assert pool.num_free_pages() == 0
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    h = History(layers)
+    half = torch.finfo(dtype).eps / 2
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(DEV)
+
+    def step(rows, parents, groups=None):
+        """Extend the rows by their trees (parents per row), append, attend in every layer."""
+        bp = cache.extend(rows, [len(p) for p in parents], groups)
+        flat = torch.tensor(sum(parents, []), dtype=torch.int32, device=DEV)
+        w.set_tree_masks(flat, bp, max(len(p) for p in parents))
+        T = flat.numel()
+        q, k, v = rnd(layers, T, Hq, D), rnd(layers, T, Hkv, D), rnd(layers, T, Hkv, D)
+        outs = [w.computeAttention(q[i], k[i], v[i], pool.cache_data[i], "tree", bp, AttentionRotaryParams(),
+                                   i).view(T, Hq, D) for i in range(layers)]
+        t0 = 0
+        for row, par in zip(rows, parents):
+            n = len(par)
+            h.append(row, k[:, t0:t0 + n], v[:, t0:t0 + n])
+            L = h.kv[row].shape[1]
+            mask = torch.ones(n, L, dtype=torch.bool)
+            mask[:, L - n:] = False
+            for i in range(n):
+                j = i
+                while j >= 0:
+                    mask[i, L - n + j] = True
+                    j = par[j]
+            for i in range(layers):
+                o, A = dense(q[i, t0:t0 + n], h.kv[row][i], mask.to(DEV))
+                bad = (outs[i][t0:t0 + n].double() - o).abs() / ((2 * half + 2.0 ** -12) * A + half * o.abs())
+                assert bad.max().item() <= 1.0, (row, bad.max().item())
+            t0 += n
+        return bp
+
+    def keep(rows, lens):
+        cache.truncate(rows, lens)
+        for r, n in zip(rows, lens):
+            h.kv[r] = h.kv[r][:, :n]
+
+    def fork(src, dst):
+        cache.fork(src, dst)
+        old = {a: h.kv[a] for a in src}
+        for a, b in zip(src, dst):
+            h.kv[b] = old[a]
+
+    step([0], [chain(3 * page + 5)])                          # the prompt
+    fork([0] * 4, [1, 2, 3, 4])
+    bp = step([1, 2, 3, 4], [chain(1)] * 4)
+    assert bp.shared_pages.tolist() == [3]
+    step([0, 1, 2, 3, 4], [tree(1, 3, 3), tree(2, 2, 2), chain(1), tree(3, 4, 2), chain(2)], groups=[0, 1, 5])
+    lens = cache.lengths()
+    keep([0, 1, 3], [lens[0] - 6, lens[1] - 2, lens[3] - 8])
+    step([4, 3, 2, 1, 0], [chain(1)] * 5)
+    fork([1, 1, 3], [5, 6, 1])                                # row 1 is a source and a destination
+    step([1, 3, 5, 6], [tree(4, 2, 3), tree(5, 2, 3), chain(1), chain(1)], groups=[0, 2, 4])
+    cache.release([2])
+    h.kv.pop(2)
+    before = int((cache.page_refs > 0).sum())
+    cache.compact()
+    assert (cache.page_refs[:before] > 0).all() and (cache.page_refs[before:] == 0).all()
+    step([0, 1, 3, 4, 5, 6], [chain(2)] * 6, groups=[0, 1, 3, 6])
+    cache.check()
+    held = np.bincount([p for r in cache.page_table.tolist() for p in r if p >= 0], minlength=120)
+    assert held.tolist() == cache.page_refs.tolist()
+    cache.close()
+    assert pool.num_free_pages() == 120
+
+
+def test_failed_calls_are_reported_and_change_nothing():
+    pool = KvCachePool(6, 1, 1, 32, 4, torch.float32, torch.device(DEV))
+    cache = SharedKvCache(pool, 3, 4)
+    with pytest.raises(ValueError):
+        SharedKvCache(pool, 1, 1)                             # no free pages
+    cache.extend([0, 1], 10)
+    cache.check()
+    state = cache.page_refs.tolist(), cache.page_table.tolist(), cache.kv_lens.tolist()
+    for call, error in ((lambda: cache.extend([0, 1], 4), RuntimeError), (lambda: cache.extend([0, 0], 1), ValueError),
+                        (lambda: cache.extend([7], 1), IndexError), (lambda: cache.extend([0], 30), RuntimeError),
+                        (lambda: cache.fork([0, 1], [2, 2]), ValueError)):
+        call()
+        with pytest.raises(error):
+            cache.check()
+        assert state == (cache.page_refs.tolist(), cache.page_table.tolist(), cache.kv_lens.tolist())
+    cache.check()
+
+
+def test_captured_step():
+    """fork, extend, append and attention captured once: each replay forks the prompt
+    anew, as it then is."""
+    Hq, Hkv, D, page = 8, 2, 128, 16
+    pool = KvCachePool(64, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, 5, 8)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    gen = torch.Generator().manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    hist = torch.empty(0, 2, Hkv, D, dtype=torch.bfloat16, device=DEV)
+
+    def prompt(n):
+        nonlocal hist
+        bp = cache.extend([0], n)
+        k, v = rnd(n, Hkv, D), rnd(n, Hkv, D)
+        w.append_kv_cache(None, k, v, bp, pool.cache_data[0], page)
+        hist = torch.cat([hist, torch.stack([k, v], 1)])
+
+    src, dst, groups = i32([0] * 4), i32([1, 2, 3, 4]), i32([0, 4])
+    seq, bits = i32([0, 1, 2, 3, 4]), torch.ones(4, 1, dtype=torch.int64, device=DEV)
+    q, k, v = rnd(4, Hq, D), rnd(4, Hkv, D), rnd(4, Hkv, D)
+    out = torch.empty_like(q)
+
+    def body():
+        K.cache_fork(cache.page_refs, cache.page_table, cache.kv_lens, src, dst)
+        b = K.cache_extend(pool.cache_data, cache.page_refs, cache.page_table, cache.kv_lens, dst, 1, group_indptr=groups)
+        bi, pos = K.batch_positions(seq, b.seq_lens, 4)
+        K.kv_append(k, v, pool.cache_data[0], bi, pos, b.page_indptr, b.page_indices)
+        K.tree_attention_shared(q, pool.cache_data[0], seq, b.page_indptr, b.page_indices, b.last_page_len, bits, 1,
+                                8 * page, groups, b.shared_pages, out=out)
+
+    prompt(20)
+    body()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        body()
+    for n in (0, 9, 33, 16):
+        if n:
+            prompt(n)
+        q.copy_(rnd(4, Hq, D))
+        k.copy_(rnd(4, Hkv, D))
+        v.copy_(rnd(4, Hkv, D))
+        g.replay()
+        for i in range(4):
+            kv = torch.cat([hist, torch.stack([k[i:i + 1], v[i:i + 1]], 1)])
+            o, A = dense(q[i:i + 1], kv, torch.ones(1, kv.shape[0], dtype=torch.bool, device=DEV))
+            bad = (out[i:i + 1].double() - o).abs() / ((2 ** -7 + 2.0 ** -12) * A + 2 ** -8 * o.abs())
+            assert bad.max().item() <= 1.0
+    cache.check()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_beam_search_with_a_shared_prefix(graph):
+    """The same search with and without ``shared_prefix`` on the fp32 model finds the same
+    tree (its scores differ in the last bits only), leaves the same free pages, and
+    goes through the shared attention."""
+    from tests.test_gpu_reference_flow import D, HKV, PAGE, V, _patched_model
+    model = _patched_model()
+    ids = torch.randint(0, V, (1, 75), generator=torch.Generator().manual_seed(3)).to(DEV)
+    trees, free = [], []
+    real, calls = K.tree_attention_shared, []
+    for shared in (False, True):
+        pool = KvCachePool(64, 2, HKV, D, PAGE, torch.float32, torch.device(DEV))
+        req = RequestKvCache(pool, PAGE, 0)
+        w = BeFlashinferWrapper(4, HKV, 256, PAGE, torch.device(DEV))
+        cfg = pbs.BeamSearchConfig(topk_len=5, max_depth=6, use_cuda_graph=graph, shared_prefix=shared)
+        K.tree_attention_shared = lambda *a, **kw: (calls.append(shared), real(*a, **kw))[1]
+        try:
+            tree_, _, runner = pbs.beam_search(model, req, ids, cfg, w)
+            if graph:                                        # replays of the captured step, another prompt's length
+                req2 = RequestKvCache(pool, PAGE, 0)
+                tree_, _, _ = pbs.beam_search(model, req2, ids[:, :50], cfg, w, cuda_graph_runner=runner)
+        finally:
+            K.tree_attention_shared = real
+        trees.append([(n.parent, n.token_id, n.depth) for n in tree_.nodes])
+        free.append(pool.free_page_mask.tolist())
+    assert trees[0] == trees[1] and len(trees[0]) > 20
+    assert free[0] == free[1]
+    assert calls and all(calls)
+
+
+@pytest.mark.parametrize("groups", [[(40, [(30, chain(1))] * 40)], [(100, [(30, tree(1, 8, 8))] * 4)]])
+def test_a_wait_that_runs_out_is_reported(groups):
+    """With a wait limit of a few clocks the launches give up, report it and return; the
+    next call is right again.  (The one launch of small decoding calls waits only for its
+    own copies, which may land within any limit.)"""
+    c = Case(groups, Hq=32, Hkv=8, seed=2)
+    a = c.device()
+    want = K.tree_attention_shared(**a)
+    K.check_attention(torch.device(DEV))
+    before = K.set_wait_limit(1)
+    try:
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            K.tree_attention_shared(**a)
+            K.check_attention(torch.device(DEV))
+    finally:
+        K.set_wait_limit(before)
+    assert torch.equal(K.tree_attention_shared(**a), want)
+    K.check_attention(torch.device(DEV))
