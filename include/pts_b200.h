@@ -376,12 +376,26 @@ int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t table_stride
  * rows of the group hold alike, for pts_tree_attn_run_shared.  workspace:
  * pts_cache_workspace_size(max_pages, batch) bytes, any contents. */
 size_t pts_cache_workspace_size(int max_pages, int batch);
-int pts_cache_extend(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
-                     int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
-                     int table_width, const int32_t* rows, const int32_t* add_each, int add, int batch,
-                     const int32_t* group_indptr, int num_groups, int32_t* page_indptr, int32_t* page_indices,
-                     int64_t page_indices_size, int32_t* last_page_len, int32_t* seq_lens, int32_t* shared_pages,
-                     int32_t* status, void* workspace, size_t workspace_bytes, pts_stream_t stream);
+typedef struct pts_cache_extend_args {
+  void* kv_pool;
+  int64_t row_bytes;
+  int32_t* page_refs;
+  int32_t* page_table;
+  int64_t table_stride;
+  int32_t* kv_lens;
+  const int32_t* rows;
+  const int32_t* add_each;      /* nullable */
+  const int32_t* group_indptr;  /* nullable */
+  int32_t* page_indptr;
+  int32_t* page_indices;
+  int64_t page_indices_size;
+  int32_t* last_page_len;
+  int32_t* seq_lens;
+  int32_t* shared_pages;        /* nullable */
+  int32_t* status;
+  int num_layers, max_pages, page_len, num_rows, table_width, add, batch, num_groups;
+} pts_cache_extend_args;
+int pts_cache_extend(const pts_cache_extend_args* args, void* workspace, size_t workspace_bytes, pts_stream_t stream);
 
 /* kv_lens[rows[i]] = min(kv_lens[rows[i]], new_lens[i]) (NULL or negative: 0); the
  * pages past the new length lose this holder and their entries become -1.  A row
@@ -397,10 +411,20 @@ int pts_cache_truncate(int32_t* page_refs, int32_t* page_table, int64_t table_st
  * [max_pages] from old to new page (-1: free) and out_counts = {live, moved}.  The
  * outputs must not overlap the inputs.  workspace: pts_cache_workspace_size(max_pages,
  * 0) bytes, any contents. */
-int pts_cache_compact(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
-                      const int32_t* page_refs, const int32_t* page_table, int64_t table_stride, int num_rows,
-                      int table_width, int32_t* out_refs, int32_t* out_table, int32_t* out_map, int32_t* out_counts,
-                      void* workspace, size_t workspace_bytes, pts_stream_t stream);
+typedef struct pts_cache_compact_args {
+  void* kv_pool;
+  int64_t row_bytes;
+  const int32_t* page_refs;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t* out_refs;
+  int32_t* out_table;
+  int32_t* out_map;
+  int32_t* out_counts;
+  int num_layers, max_pages, page_len, num_rows, table_width;
+} pts_cache_compact_args;
+int pts_cache_compact(const pts_cache_compact_args* args, void* workspace, size_t workspace_bytes,
+                      pts_stream_t stream);
 
 /* ------------------------------------------------------------------ attention
  * Ancestor bitmask of every tree row: bit j of row i's mask_words-word mask is
@@ -545,13 +569,24 @@ int pts_tree_attn_run_any(const void* q, const void* kv_layer, const int32_t* qo
 size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups, int total_q, int max_qo_len, int max_kv_len,
                                            int max_own_len, int num_qo_heads, int num_kv_heads, int head_dim,
                                            int page_len, int elem_bytes);
-int pts_tree_attn_run_shared(const void* q, const void* kv_layer, const int32_t* qo_indptr,
-                             const int32_t* page_indptr, const int32_t* page_indices, const int32_t* last_page_len,
-                             const uint64_t* mask_bits, int mask_words, const int32_t* group_indptr,
-                             const int32_t* shared_pages, int num_groups, void* out, int batch, int total_q,
-                             int max_qo_len, int max_kv_len, int max_own_len, int num_qo_heads, int num_kv_heads,
-                             int head_dim, int page_len, int max_pages, float sm_scale, int elem_bytes,
-                             void* workspace, size_t workspace_bytes, int32_t* error, pts_stream_t stream);
+typedef struct pts_shared_attn_args {
+  const void* q;
+  const void* kv_layer;
+  const int32_t* qo_indptr;
+  const int32_t* page_indptr;
+  const int32_t* page_indices;
+  const int32_t* last_page_len;
+  const uint64_t* mask_bits;    /* nullable */
+  const int32_t* group_indptr;
+  const int32_t* shared_pages;
+  void* out;
+  int32_t* error;               /* nullable */
+  int mask_words, num_groups, batch, total_q, max_qo_len, max_kv_len, max_own_len;
+  int num_qo_heads, num_kv_heads, head_dim, page_len, max_pages, elem_bytes;
+  float sm_scale;
+} pts_shared_attn_args;
+int pts_tree_attn_run_shared(const pts_shared_attn_args* args, void* workspace, size_t workspace_bytes,
+                             pts_stream_t stream);
 
 /* pts_tree_attn_run with page tables per (request, KV head): head_page_indptr
  * [B*Hkv+1] and head_last_page_len [B*Hkv] indexed b * Hkv + h, every list

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -32,6 +33,32 @@ class KvCompactArgs(C.Structure):
                 ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("elem_bytes", C.c_int),
                 ("page_indptr", C.c_void_p), ("page_indices", C.c_void_p), ("offsets", C.c_void_p),
                 ("new_kv_len", C.c_void_p), ("new_last_page_len", C.c_void_p)]
+
+
+def _packer(fields) -> struct.Struct:
+    """Packs the fields of an argument structure, in order, as C lays them out: pointers
+    (P), int64 (q), int (i) and float (f).  One call that packs replaces one conversion per
+    argument, which for some thirty arguments costs as much as a launch."""
+    return struct.Struct("@" + "".join(code for _, code in fields) + "0P")
+
+
+# pts_cache_extend_args, pts_cache_compact_args, pts_shared_attn_args
+CACHE_EXTEND_FIELDS = [(n, "P") for n in ("kv_pool",)] + [("row_bytes", "q"), ("page_refs", "P"), ("page_table", "P"),
+                       ("table_stride", "q")] + [(n, "P") for n in ("kv_lens", "rows", "add_each", "group_indptr",
+                       "page_indptr", "page_indices")] + [("page_indices_size", "q")] + [(n, "P") for n in (
+                       "last_page_len", "seq_lens", "shared_pages", "status")] + [(n, "i") for n in (
+                       "num_layers", "max_pages", "page_len", "num_rows", "table_width", "add", "batch", "num_groups")]
+CACHE_COMPACT_FIELDS = [("kv_pool", "P"), ("row_bytes", "q"), ("page_refs", "P"), ("page_table", "P"),
+                        ("table_stride", "q")] + [(n, "P") for n in ("out_refs", "out_table", "out_map", "out_counts")] + [
+                        (n, "i") for n in ("num_layers", "max_pages", "page_len", "num_rows", "table_width")]
+SHARED_ATTN_FIELDS = [(n, "P") for n in ("q", "kv_layer", "qo_indptr", "page_indptr", "page_indices", "last_page_len",
+                      "mask_bits", "group_indptr", "shared_pages", "out", "error")] + [(n, "i") for n in (
+                      "mask_words", "num_groups", "batch", "total_q", "max_qo_len", "max_kv_len", "max_own_len",
+                      "num_qo_heads", "num_kv_heads", "head_dim", "page_len", "max_pages", "elem_bytes")] + [
+                      ("sm_scale", "f")]
+pack_cache_extend = _packer(CACHE_EXTEND_FIELDS).pack
+pack_cache_compact = _packer(CACHE_COMPACT_FIELDS).pack
+pack_shared_attn = _packer(SHARED_ATTN_FIELDS).pack
 
 
 SIGNATURES = {
@@ -76,16 +103,12 @@ SIGNATURES = {
     "pts_kv_compact": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_int,
                                  vp, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp]),
     "pts_tree_attn_shared_workspace_size": (sz, [C.c_int] * 11),
-    "pts_tree_attn_run_shared": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, C.c_int, vp, vp, C.c_int, vp, C.c_int, C.c_int,
-                                           C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, f32,
-                                           C.c_int, vp, sz, vp, vp]),
+    "pts_tree_attn_run_shared": (C.c_int, [vp, vp, sz, vp]),
     "pts_cache_workspace_size": (sz, [C.c_int, C.c_int]),
     "pts_cache_fork": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
-    "pts_cache_extend": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, i64, vp, C.c_int, C.c_int, vp, vp, C.c_int,
-                                   C.c_int, vp, C.c_int, vp, vp, i64, vp, vp, vp, vp, vp, sz, vp]),
+    "pts_cache_extend": (C.c_int, [vp, vp, sz, vp]),
     "pts_cache_truncate": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
-    "pts_cache_compact": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, i64, vp, vp, i64, C.c_int, C.c_int, vp, vp, vp, vp, vp,
-                                    sz, vp]),
+    "pts_cache_compact": (C.c_int, [vp, vp, sz, vp]),
     "pts_tree_mask_from_parents": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, vp]),
     "pts_tree_prepare": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp]),
     "pts_kv_append_rope": (C.c_int, [vp, i64, vp, C.c_int, vp, vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp,

@@ -326,66 +326,62 @@ extern "C" size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups,
   return make_plan(batch, num_groups, total_q, max_qo_len, max_kv_len, num_qo_heads, num_kv_heads, head_dim).bytes;
 }
 
-extern "C" int pts_tree_attn_run_shared(const void* q, const void* kv_layer, const int32_t* qo_indptr,
-                                        const int32_t* page_indptr, const int32_t* page_indices,
-                                        const int32_t* last_page_len, const uint64_t* mask_bits, int mask_words,
-                                        const int32_t* group_indptr, const int32_t* shared_pages, int num_groups,
-                                        void* out, int batch, int total_q, int max_qo_len, int max_kv_len,
-                                        int max_own_len, int num_qo_heads, int num_kv_heads, int head_dim,
-                                        int page_len, int max_pages, float sm_scale, int elem_bytes, void* workspace,
-                                        size_t workspace_bytes, int32_t* error, pts_stream_t stream) {
-  PTS_CHECK_ARG(q && kv_layer && qo_indptr && page_indptr && page_indices && last_page_len && out, "null pointer");
-  PTS_CHECK_ARG(group_indptr && shared_pages && num_groups > 0, "groups need group_indptr and shared_pages");
-  PTS_CHECK_ARG(batch > 0 && total_q > 0 && max_qo_len > 0 && max_kv_len > 0 && max_own_len >= 0, "bad sizes");
-  PTS_CHECK_ARG(num_qo_heads > 0 && num_kv_heads > 0 && num_qo_heads % num_kv_heads == 0, "bad head counts");
-  PTS_CHECK_ARG(page_len > 0 && max_pages > 0, "bad page sizes");
-  if (head_dim <= 0 || head_dim % 32 || head_dim > 256)
-    return set_error(PTS_ERR_UNSUPPORTED, "head_dim %d (a multiple of 32 up to 256)", head_dim);
-  if (elem_bytes != 2 && elem_bytes != 4) return set_error(PTS_ERR_UNSUPPORTED, "element size %d", elem_bytes);
-  if (mask_bits) {
-    if (max_qo_len > PTS_MAX_TREE_NODES)
-      return set_error(PTS_ERR_CAPACITY, "tree of %d rows above %d", max_qo_len, PTS_MAX_TREE_NODES);
-    PTS_CHECK_ARG(mask_words >= (max_qo_len + 63) / 64, "mask_words %d too small for %d rows", mask_words,
-                  max_qo_len);
+extern "C" int pts_tree_attn_run_shared(const pts_shared_attn_args* args, void* workspace, size_t workspace_bytes,
+                                        pts_stream_t stream) {
+  PTS_CHECK_ARG(args, "null arguments");
+  const pts_shared_attn_args& x = *args;
+  PTS_CHECK_ARG(x.q && x.kv_layer && x.qo_indptr && x.page_indptr && x.page_indices && x.last_page_len && x.out, "null pointer");
+  PTS_CHECK_ARG(x.group_indptr && x.shared_pages && x.num_groups > 0, "groups need group_indptr and shared_pages");
+  PTS_CHECK_ARG(x.batch > 0 && x.total_q > 0 && x.max_qo_len > 0 && x.max_kv_len > 0 && x.max_own_len >= 0, "bad sizes");
+  PTS_CHECK_ARG(x.num_qo_heads > 0 && x.num_kv_heads > 0 && x.num_qo_heads % x.num_kv_heads == 0, "bad head counts");
+  PTS_CHECK_ARG(x.page_len > 0 && x.max_pages > 0, "bad page sizes");
+  if (x.head_dim <= 0 || x.head_dim % 32 || x.head_dim > 256)
+    return set_error(PTS_ERR_UNSUPPORTED, "head_dim %d (a multiple of 32 up to 256)", x.head_dim);
+  if (x.elem_bytes != 2 && x.elem_bytes != 4) return set_error(PTS_ERR_UNSUPPORTED, "element size %d", x.elem_bytes);
+  if (x.mask_bits) {
+    if (x.max_qo_len > PTS_MAX_TREE_NODES)
+      return set_error(PTS_ERR_CAPACITY, "tree of %d rows above %d", x.max_qo_len, PTS_MAX_TREE_NODES);
+    PTS_CHECK_ARG(x.mask_words >= (x.max_qo_len + 63) / 64, "mask_words %d too small for %d rows", x.mask_words,
+                  x.max_qo_len);
   }
-  PTS_CHECK_ARG((((uintptr_t)q | (uintptr_t)kv_layer | (uintptr_t)out) & 15) == 0,
+  PTS_CHECK_ARG((((uintptr_t)x.q | (uintptr_t)x.kv_layer | (uintptr_t)x.out) & 15) == 0,
                 "q, kv_layer and out must be 16-byte aligned");
   PTS_CHECK_ARG(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
-  if (num_kv_heads > 65535) return set_error(PTS_ERR_CAPACITY, "grid too large");
-  const size_t need = pts_tree_attn_shared_workspace_size(batch, num_groups, total_q, max_qo_len, max_kv_len,
-                                                          max_own_len, num_qo_heads, num_kv_heads, head_dim, page_len,
-                                                          elem_bytes);
+  if (x.num_kv_heads > 65535) return set_error(PTS_ERR_CAPACITY, "grid too large");
+  const size_t need = pts_tree_attn_shared_workspace_size(x.batch, x.num_groups, x.total_q, x.max_qo_len, x.max_kv_len,
+                                                          x.max_own_len, x.num_qo_heads, x.num_kv_heads, x.head_dim, x.page_len,
+                                                          x.elem_bytes);
   if (!workspace || workspace_bytes < need)
     return set_error(PTS_ERR_CAPACITY, "workspace of %zu bytes (%zu needed)", workspace_bytes, need);
   SharedAttnParams a{};
-  a.q = q;
-  a.kv = kv_layer;
-  a.qo_indptr = qo_indptr;
-  a.page_indptr = page_indptr;
-  a.page_indices = page_indices;
-  a.last_page_len = last_page_len;
-  a.mask_bits = mask_bits;
-  a.mask_words = mask_words;
-  a.out = out;
-  a.group_indptr = group_indptr;
-  a.shared_pages = shared_pages;
-  a.batch = batch;
-  a.groups = num_groups;
-  a.Hq = num_qo_heads;
-  a.Hkv = num_kv_heads;
-  a.g = num_qo_heads / num_kv_heads;
-  a.D = head_dim;
-  a.page_len = page_len;
-  a.max_pages = max_pages;
-  a.scale = sm_scale;
-  if (prefix_attn_supports(head_dim, page_len, elem_bytes))
-    return prefix_attn_launch(a, total_q, max_qo_len, max_kv_len, max_own_len, workspace, error, (cudaStream_t)stream);
-  const Plan pl = make_plan(batch, num_groups, total_q, max_qo_len, max_kv_len, num_qo_heads, num_kv_heads, head_dim);
-  const int64_t gx = (int64_t)pl.group_tiles + (int64_t)batch * pl.request_tiles;
+  a.q = x.q;
+  a.kv = x.kv_layer;
+  a.qo_indptr = x.qo_indptr;
+  a.page_indptr = x.page_indptr;
+  a.page_indices = x.page_indices;
+  a.last_page_len = x.last_page_len;
+  a.mask_bits = x.mask_bits;
+  a.mask_words = x.mask_words;
+  a.out = x.out;
+  a.group_indptr = x.group_indptr;
+  a.shared_pages = x.shared_pages;
+  a.batch = x.batch;
+  a.groups = x.num_groups;
+  a.Hq = x.num_qo_heads;
+  a.Hkv = x.num_kv_heads;
+  a.g = x.num_qo_heads / x.num_kv_heads;
+  a.D = x.head_dim;
+  a.page_len = x.page_len;
+  a.max_pages = x.max_pages;
+  a.scale = x.sm_scale;
+  if (prefix_attn_supports(x.head_dim, x.page_len, x.elem_bytes))
+    return prefix_attn_launch(a, x.total_q, x.max_qo_len, x.max_kv_len, x.max_own_len, workspace, x.error, (cudaStream_t)stream);
+  const Plan pl = make_plan(x.batch, x.num_groups, x.total_q, x.max_qo_len, x.max_kv_len, x.num_qo_heads, x.num_kv_heads, x.head_dim);
+  const int64_t gx = (int64_t)pl.group_tiles + (int64_t)x.batch * pl.request_tiles;
   if (gx > 2147483647ll) return set_error(PTS_ERR_CAPACITY, "grid too large");
   PartsParams p{a, pl.splits, pl.group_tiles, pl.request_tiles, (float*)((char*)workspace + pl.part_o),
                 (float2*)workspace};
-  const dim3 grid((unsigned)gx, num_kv_heads, pl.splits);
-  return elem_bytes == 4 ? launch_any<float>(p, grid, total_q, (cudaStream_t)stream)
-                         : launch_any<uint16_t>(p, grid, total_q, (cudaStream_t)stream);
+  const dim3 grid((unsigned)gx, x.num_kv_heads, pl.splits);
+  return x.elem_bytes == 4 ? launch_any<float>(p, grid, x.total_q, (cudaStream_t)stream)
+                         : launch_any<uint16_t>(p, grid, x.total_q, (cudaStream_t)stream);
 }

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = bad;
   if (bad) return;
   const int c0 = blockIdx.x * cols;
+#pragma unroll 4
   for (int e = threadIdx.x; e < n * cols; e += kForkThreads) {
     const int c = c0 + e % cols;
     stage[e] = c < s.width ? s.table[from[e / cols] * s.stride + c] : -1;
@@ -91,15 +92,22 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n * cols; e += kForkThreads) {
-    const int c = c0 + e % cols;
-    if (c >= s.width) continue;
-    int32_t* at = s.table + to[e / cols] * s.stride + c;
-    const int old = *at, page = stage[e];
-    if (old == page) continue;
-    *at = page;
-    if (page >= 0 && page < s.pages) atomicAdd(&s.refs[page], 1);
-    if (old >= 0 && old < s.pages) atomicSub(&s.refs[old], 1);
+  for (int e0 = threadIdx.x; e0 < n * cols; e0 += 4 * kForkThreads) {
+    int old[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {                       // four entries in flight
+      const int e = e0 + u * kForkThreads;
+      old[u] = e < n * cols && c0 + e % cols < s.width ? s.table[to[e / cols] * s.stride + c0 + e % cols] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kForkThreads;
+      if (e >= n * cols || c0 + e % cols >= s.width || old[u] == stage[e]) continue;
+      const int page = stage[e];
+      s.table[to[e / cols] * s.stride + c0 + e % cols] = page;
+      if (page >= 0 && page < s.pages) atomicAdd(&s.refs[page], 1);
+      if (old[u] >= 0 && old[u] < s.pages) atomicSub(&s.refs[old[u]], 1);
+    }
   }
   if (blockIdx.x == 0) {
 #pragma unroll
@@ -650,8 +658,10 @@ extern "C" int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t t
   PTS_CHECK_ARG(src_rows && dst_rows && status && num_forks > 0, "bad fork list");
   if (num_forks > kMaxForks) return set_error(PTS_ERR_CAPACITY, "%d forks above %d", num_forks, kMaxForks);
   const PageState s{page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages};
-  int cols = 32;                                        // whole 128-byte lines of the table where the forks' entries fit
-  while (cols * num_forks > kStageEntries) cols /= 2;
+  // a CTA's columns: a line of the table for few forks, a sector of it for many (128 forks of
+  // 95 columns: 18 us in three CTAs of a line, 4 us in twelve of a sector)
+  const int cols = num_forks <= 16 ? 32 : num_forks <= 64 ? 16 : 8;
+  static_assert(8 * kMaxForks <= kStageEntries, "a CTA's entries");
   const size_t smem = (size_t)(num_rows + 31) / 32 * 4;
   if (smem > 4 * 1024)
     if (int rc = ensure_smem_attr((const void*)cache_fork_kernel, smem)) return rc;
@@ -677,92 +687,88 @@ extern "C" size_t pts_cache_workspace_size(int max_pages, int batch) {
   return ((size_t)2 * max_pages + (size_t)3 * batch + 4) * sizeof(int32_t);
 }
 
-extern "C" int pts_cache_extend(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
-                                int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
-                                int num_rows, int table_width, const int32_t* rows, const int32_t* add_each, int add,
-                                int batch, const int32_t* group_indptr, int num_groups, int32_t* page_indptr,
-                                int32_t* page_indices, int64_t page_indices_size, int32_t* last_page_len,
-                                int32_t* seq_lens, int32_t* shared_pages, int32_t* status, void* workspace,
-                                size_t workspace_bytes, pts_stream_t stream) {
-  if (int rc = check_state(page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages, true))
+extern "C" int pts_cache_extend(const pts_cache_extend_args* args, void* workspace, size_t workspace_bytes,
+                                pts_stream_t stream) {
+  PTS_CHECK_ARG(args, "null arguments");
+  const pts_cache_extend_args& x = *args;
+  if (int rc = check_state(x.page_refs, x.page_table, x.table_stride, x.kv_lens, x.num_rows, x.table_width, x.max_pages, true))
     return rc;
-  if (int rc = check_pool(kv_pool, num_layers, page_len, row_bytes)) return rc;
-  PTS_CHECK_ARG(rows && page_indptr && page_indices && last_page_len && seq_lens && status, "null pointer");
-  PTS_CHECK_ARG(batch > 0 && add >= 0 && num_groups >= 0, "bad sizes");
-  PTS_CHECK_ARG(!shared_pages || (group_indptr && num_groups > 0), "shared_pages needs group_indptr");
-  PTS_CHECK_ARG(page_indices_size >= (int64_t)batch * table_width, "page_indices holds fewer than batch * width");
-  if (batch > kMaxBatch) return set_error(PTS_ERR_CAPACITY, "%d sequences above %d", batch, kMaxBatch);
-  if ((int64_t)batch * table_width > INT_MAX) return set_error(PTS_ERR_CAPACITY, "page lists above 2^31 entries");
-  if (!workspace || workspace_bytes < pts_cache_workspace_size(max_pages, batch))
+  if (int rc = check_pool(x.kv_pool, x.num_layers, x.page_len, x.row_bytes)) return rc;
+  PTS_CHECK_ARG(x.rows && x.page_indptr && x.page_indices && x.last_page_len && x.seq_lens && x.status, "null pointer");
+  PTS_CHECK_ARG(x.batch > 0 && x.add >= 0 && x.num_groups >= 0, "bad sizes");
+  PTS_CHECK_ARG(!x.shared_pages || (x.group_indptr && x.num_groups > 0), "shared_pages needs group_indptr");
+  PTS_CHECK_ARG(x.page_indices_size >= (int64_t)x.batch * x.table_width, "page_indices holds fewer than batch * width");
+  if (x.batch > kMaxBatch) return set_error(PTS_ERR_CAPACITY, "%d sequences above %d", x.batch, kMaxBatch);
+  if ((int64_t)x.batch * x.table_width > INT_MAX) return set_error(PTS_ERR_CAPACITY, "page lists above 2^31 entries");
+  if (!workspace || workspace_bytes < pts_cache_workspace_size(x.max_pages, x.batch))
     return set_error(PTS_ERR_CAPACITY, "workspace too small");
   PTS_CHECK_ARG(((uintptr_t)workspace & 3) == 0, "workspace must be 4-byte aligned");
   ExtendParams p{};
-  p.s = PageState{page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages};
-  p.rows = rows;
-  p.add_each = add_each;
-  p.add = add;
-  p.batch = batch;
-  p.group_indptr = group_indptr;
-  p.groups = num_groups;
-  p.page_len = page_len;
-  p.page_indptr = page_indptr;
-  p.page_indices = page_indices;
-  p.capacity = page_indices_size;
-  p.last_page_len = last_page_len;
-  p.seq_lens = seq_lens;
-  p.shared_pages = shared_pages;
-  p.status = status;
+  p.s = PageState{x.page_refs, x.page_table, x.table_stride, x.kv_lens, x.num_rows, x.table_width, x.max_pages};
+  p.rows = x.rows;
+  p.add_each = x.add_each;
+  p.add = x.add;
+  p.batch = x.batch;
+  p.group_indptr = x.group_indptr;
+  p.groups = x.num_groups;
+  p.page_len = x.page_len;
+  p.page_indptr = x.page_indptr;
+  p.page_indices = x.page_indices;
+  p.capacity = x.page_indices_size;
+  p.last_page_len = x.last_page_len;
+  p.seq_lens = x.seq_lens;
+  p.shared_pages = x.shared_pages;
+  p.status = x.status;
   p.holders = (int32_t*)workspace;
-  p.final_row = p.holders + max_pages;
-  p.pairs = p.final_row + max_pages;
-  p.counts = p.pairs + 3 * (int64_t)batch;
-  p.pool = (char*)kv_pool;
-  p.layers = num_layers;
-  p.row_bytes = row_bytes;
-  const size_t smem = ((size_t)(max_pages + 31) / 32 + (num_rows + 31) / 32 + batch + 1) * 4;
+  p.final_row = p.holders + x.max_pages;
+  p.pairs = p.final_row + x.max_pages;
+  p.counts = p.pairs + 3 * (int64_t)x.batch;
+  p.pool = (char*)x.kv_pool;
+  p.layers = x.num_layers;
+  p.row_bytes = x.row_bytes;
+  const size_t smem = ((size_t)(x.max_pages + 31) / 32 + (x.num_rows + 31) / 32 + x.batch + 1) * 4;
   if (smem > 32 * 1024)
     if (int rc = ensure_smem_attr((const void*)cache_extend_plan_kernel, smem)) return rc;
   PTS_CUDA_TRY(launch_pdl(cache_extend_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, p));
   if (int rc = launch_status("cache_extend_plan_kernel")) return rc;
-  const int64_t units = std::max<int64_t>((int64_t)batch * 2 * num_layers, (batch + 7) / 8);
+  const int64_t units = std::max<int64_t>((int64_t)x.batch * 2 * x.num_layers, (x.batch + 7) / 8);
   PTS_CUDA_TRY(launch_pdl(cache_extend_apply_kernel, dim3((unsigned)std::min<int64_t>(copy_grid(), units)),
                           dim3(kCopyThreads), 0, (cudaStream_t)stream, p));
   return launch_status("cache_extend_apply_kernel");
 }
 
-extern "C" int pts_cache_compact(void* kv_pool, int num_layers, int max_pages, int page_len, int64_t row_bytes,
-                                 const int32_t* page_refs, const int32_t* page_table, int64_t table_stride,
-                                 int num_rows, int table_width, int32_t* out_refs, int32_t* out_table,
-                                 int32_t* out_map, int32_t* out_counts, void* workspace, size_t workspace_bytes,
+extern "C" int pts_cache_compact(const pts_cache_compact_args* args, void* workspace, size_t workspace_bytes,
                                  pts_stream_t stream) {
-  if (int rc = check_state(page_refs, page_table, table_stride, nullptr, num_rows, table_width, max_pages, false))
+  PTS_CHECK_ARG(args, "null arguments");
+  const pts_cache_compact_args& x = *args;
+  if (int rc = check_state(x.page_refs, x.page_table, x.table_stride, nullptr, x.num_rows, x.table_width, x.max_pages, false))
     return rc;
-  if (int rc = check_pool(kv_pool, num_layers, page_len, row_bytes)) return rc;
-  PTS_CHECK_ARG(out_refs && out_table && out_map && out_counts, "null output pointer");
-  PTS_CHECK_ARG(out_refs != page_refs && out_table != page_table, "the outputs must not be the inputs");
-  if (!workspace || workspace_bytes < pts_cache_workspace_size(max_pages, 0))
+  if (int rc = check_pool(x.kv_pool, x.num_layers, x.page_len, x.row_bytes)) return rc;
+  PTS_CHECK_ARG(x.out_refs && x.out_table && x.out_map && x.out_counts, "null output pointer");
+  PTS_CHECK_ARG(x.out_refs != x.page_refs && x.out_table != x.page_table, "the outputs must not be the inputs");
+  if (!workspace || workspace_bytes < pts_cache_workspace_size(x.max_pages, 0))
     return set_error(PTS_ERR_CAPACITY, "workspace too small");
   PTS_CHECK_ARG(((uintptr_t)workspace & 3) == 0, "workspace must be 4-byte aligned");
   CompactParams p{};
-  p.s = PageState{const_cast<int32_t*>(page_refs), const_cast<int32_t*>(page_table), table_stride, nullptr, num_rows,
-                  table_width, max_pages};
-  p.page_len = page_len;
-  p.pool = (char*)kv_pool;
-  p.layers = num_layers;
-  p.row_bytes = row_bytes;
-  p.out_refs = out_refs;
-  p.out_table = out_table;
-  p.out_map = out_map;
-  p.out_counts = out_counts;
+  p.s = PageState{const_cast<int32_t*>(x.page_refs), const_cast<int32_t*>(x.page_table), x.table_stride, nullptr, x.num_rows,
+                  x.table_width, x.max_pages};
+  p.page_len = x.page_len;
+  p.pool = (char*)x.kv_pool;
+  p.layers = x.num_layers;
+  p.row_bytes = x.row_bytes;
+  p.out_refs = x.out_refs;
+  p.out_table = x.out_table;
+  p.out_map = x.out_map;
+  p.out_counts = x.out_counts;
   p.pairs = (int32_t*)workspace;
-  const size_t smem = (size_t)(max_pages + 31) / 32 * 4;
+  const size_t smem = (size_t)(x.max_pages + 31) / 32 * 4;
   if (smem > 32 * 1024)
     if (int rc = ensure_smem_attr((const void*)cache_compact_plan_kernel, smem)) return rc;
   PTS_CUDA_TRY(launch_pdl(cache_compact_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, p));
   if (int rc = launch_status("cache_compact_plan_kernel")) return rc;
-  const int64_t pieces = (2 * page_len * row_bytes + kPieceBytes - 1) / kPieceBytes;
-  const int64_t units = std::max<int64_t>((int64_t)max_pages * num_layers * pieces / 2,
-                                          ((int64_t)num_rows * table_width + kCopyThreads - 1) / kCopyThreads);
+  const int64_t pieces = (2 * x.page_len * x.row_bytes + kPieceBytes - 1) / kPieceBytes;
+  const int64_t units = std::max<int64_t>((int64_t)x.max_pages * x.num_layers * pieces / 2,
+                                          ((int64_t)x.num_rows * x.table_width + kCopyThreads - 1) / kCopyThreads);
   PTS_CUDA_TRY(launch_pdl(cache_compact_apply_kernel,
                           dim3((unsigned)std::min<int64_t>(2 * copy_grid(), std::max<int64_t>(units, 1))),
                           dim3(kCopyThreads), 0, (cudaStream_t)stream, p));

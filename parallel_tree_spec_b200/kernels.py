@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import math
 import os
 from typing import Dict, NamedTuple, Optional, Tuple, Union
@@ -632,7 +633,7 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
     _cache_ints("page_indices", page_indices, index)
     _cache_ints("last_page_len", last_page_len, index, B)
     _cache_ints("group_indptr", group_indptr, index, G + 1)
-    bits, words = None, 1
+    bits, words = 0, 1
     if mask_bits is not None:
         if mask_bits.dtype is not torch.int64 or mask_bits.dim() != 2 or not mask_bits.is_contiguous() or \
                 mask_bits.shape[0] < T or mask_bits.get_device() != index:
@@ -642,23 +643,30 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like q")
+    max_qo, max_kv = int(max_qo_len), min(int(max_kv_len), 2 ** 31 - 1)
     own = int(max_own_len) if max_own_len is not None else 0
     es = 2 if q.dtype is torch.bfloat16 else 4
     with _on(index):
-        nbytes = _lib.lib().pts_tree_attn_shared_workspace_size(B, G, T, max_qo_len, max_kv_len, own, Hq, Hkv, D, pl, es)
-        ws = qo_indptr.new_empty(max(nbytes, 256) // 4)
-        stream = _raw_stream(index)
+        nbytes = _shared_attn_workspace(index, B, G, T, max_qo, max_kv, own, Hq, Hkv, D, pl, es)
+        ws = qo_indptr.new_empty((nbytes + 3) // 4)
         err = _ERROR_WORDS.get(index)
         if err is None:
             err = _error_word(index)
-        _lib.call("pts_tree_attn_run_shared", q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(),
-                  page_indptr.data_ptr(), page_indices.data_ptr(), last_page_len.data_ptr(), bits, words,
-                  group_indptr.data_ptr(), shared_pages.data_ptr(), G, out.data_ptr(), B, T, max_qo_len, max_kv_len, own,
-                  Hq, Hkv, D, pl, P, sm_scale if sm_scale is not None else D ** -0.5, es, ws.data_ptr(), nbytes,
-                  err.data_ptr() if err is not None else None, stream)
+        _lib.call("pts_tree_attn_run_shared", _lib.pack_shared_attn(
+            q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
+            last_page_len.data_ptr(), bits, group_indptr.data_ptr(), shared_pages.data_ptr(), out.data_ptr(),
+            err.data_ptr() if err is not None else 0, words, G, B, T, max_qo, max_kv, own, Hq, Hkv, D, pl, P, es,
+            sm_scale if sm_scale is not None else D ** -0.5), ws.data_ptr(), nbytes, _raw_stream(index))
     if _CHECK_ATTENTION:
         check_attention(q.device)
     return out
+
+
+@functools.lru_cache(maxsize=512)
+def _shared_attn_workspace(index: int, *sizes: int) -> int:
+    """pts_tree_attn_shared_workspace_size on device ``index`` (at least 256 bytes, so that
+    sizes it refuses reach the launch's own checks)."""
+    return max(_lib.lib().pts_tree_attn_shared_workspace_size(*sizes), 256)
 
 
 _ERROR_WORDS: Dict[int, torch.Tensor] = {}
@@ -880,8 +888,8 @@ def _cache_ints(name: str, t: torch.Tensor, index: int, size: Optional[int] = No
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
     if t.get_device() != index:
         raise ValueError("all tensors must be on the same device")
-    if size is not None and t.shape[0] != size:
-        raise ValueError(f"{name} has {t.shape[0]} entries, expected {size}")
+    if size is not None and t.numel() != size:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {size}")
     return t
 
 
@@ -956,11 +964,13 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     B, (R, W) = _cache_ints("rows", rows, index).shape[0], page_table.shape
     if B == 0:
         raise ValueError("rows is empty")
-    each, add_all = None, 0
+    each, add_all = 0, 0
     if isinstance(add, torch.Tensor):
         each = _cache_ints("add", add, index, B).data_ptr()
     else:
         add_all = int(add)
+        if not 0 <= add_all < 2 ** 31:
+            raise ValueError(f"add {add_all} is negative or too large")
     G = 0
     if group_indptr is not None:
         G = _cache_ints("group_indptr", group_indptr, index).shape[0] - 1
@@ -981,11 +991,11 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     words = 2 * P + 3 * B + 4                                # pts_cache_workspace_size
     ws = page_refs.new_empty(words)
     with _on(index):
-        _lib.call("pts_cache_extend", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
-                  page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), R, W, rows.data_ptr(), each, add_all,
-                  B, group_indptr.data_ptr() if G else None, G, indptr.data_ptr(), indices.data_ptr(),
-                  indices.shape[0], last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else None,
-                  status.data_ptr(), ws.data_ptr(), 4 * words, _raw_stream(index))
+        _lib.call("pts_cache_extend", _lib.pack_cache_extend(
+            pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+            kv_lens.data_ptr(), rows.data_ptr(), each, group_indptr.data_ptr() if G else 0, indptr.data_ptr(),
+            indices.data_ptr(), indices.numel(), last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else 0,
+            status.data_ptr(), L, P, pl, R, W, add_all, B, G), ws.data_ptr(), 4 * words, _raw_stream(index))
     return CacheBatch(indptr, indices, last, lens, shared, status)
 
 
@@ -1022,7 +1032,8 @@ def cache_compact(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch
     words = 2 * P + 4                                        # pts_cache_workspace_size
     ws = page_refs.new_empty(words)
     with _on(index):
-        _lib.call("pts_cache_compact", pool.data_ptr(), L, P, pl, row_bytes, page_refs.data_ptr(),
-                  page_table.data_ptr(), page_table.stride(0), R, W, refs.data_ptr(), table.data_ptr(),
-                  page_map.data_ptr(), counts.data_ptr(), ws.data_ptr(), 4 * words, _raw_stream(index))
+        _lib.call("pts_cache_compact", _lib.pack_cache_compact(
+            pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+            refs.data_ptr(), table.data_ptr(), page_map.data_ptr(), counts.data_ptr(), L, P, pl, R, W), ws.data_ptr(),
+            4 * words, _raw_stream(index))
     return CompactedCache(refs, table, page_map, counts)

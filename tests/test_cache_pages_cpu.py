@@ -1,5 +1,7 @@
 """Refusals of the page-state calls (no GPU: every check is on the host)."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
@@ -8,6 +10,8 @@ import torch
 from oracle import cache as oc
 from parallel_tree_spec_b200 import _lib
 from parallel_tree_spec_b200 import kernels as K
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "pts_b200.h")
 
 
 def test_cpu_tensors_are_refused():
@@ -24,20 +28,21 @@ def test_cpu_tensors_are_refused():
 P = C.c_void_p(256)                                          # never read: the checks come first
 
 
-def _extend(**kw):
-    a = dict(pool=P, layers=1, pages=8, pl=4, row_bytes=32, refs=P, table=P, stride=4, lens=P, rows_n=2, width=4, rows=P,
-             add_each=None, add=1, batch=2, groups=None, G=0, indptr=P, indices=P, size=8, last=P, seq=P, shared=None,
-             status=P, ws=P, ws_bytes=1 << 20, stream=None)
+def _extend(ws_bytes=1 << 20, **kw):
+    a = dict.fromkeys((n for n, _ in _lib.CACHE_EXTEND_FIELDS), 256)
+    a.update(row_bytes=32, table_stride=4, add_each=0, group_indptr=0, shared_pages=0, page_indices_size=8, num_layers=1,
+             max_pages=8, page_len=4, num_rows=2, table_width=4, add=1, batch=2, num_groups=0)
     a.update(kw)
-    return _lib.lib().pts_cache_extend(*a.values())
+    return _lib.lib().pts_cache_extend(_lib.pack_cache_extend(*a.values()), P, ws_bytes, None)
 
 
 @pytest.mark.parametrize("kw,code", [
-    (dict(row_bytes=24), _lib.PTS_ERR_INVALID), (dict(pool=C.c_void_p(8)), _lib.PTS_ERR_INVALID),
-    (dict(stride=3), _lib.PTS_ERR_INVALID), (dict(add=-1), _lib.PTS_ERR_INVALID), (dict(batch=0), _lib.PTS_ERR_INVALID),
-    (dict(size=7), _lib.PTS_ERR_INVALID), (dict(shared=P), _lib.PTS_ERR_INVALID),
-    (dict(ws_bytes=63), _lib.PTS_ERR_CAPACITY), (dict(batch=4097, size=4097 * 4), _lib.PTS_ERR_CAPACITY),
-    (dict(pages=(1 << 20) + 1), _lib.PTS_ERR_CAPACITY), (dict(rows_n=(1 << 17) + 1), _lib.PTS_ERR_CAPACITY)])
+    (dict(row_bytes=24), _lib.PTS_ERR_INVALID), (dict(kv_pool=8), _lib.PTS_ERR_INVALID),
+    (dict(table_stride=3), _lib.PTS_ERR_INVALID), (dict(add=-1), _lib.PTS_ERR_INVALID),
+    (dict(batch=0), _lib.PTS_ERR_INVALID), (dict(page_indices_size=7), _lib.PTS_ERR_INVALID),
+    (dict(shared_pages=256), _lib.PTS_ERR_INVALID), (dict(page_refs=0), _lib.PTS_ERR_INVALID),
+    (dict(ws_bytes=63), _lib.PTS_ERR_CAPACITY), (dict(batch=4097, page_indices_size=4097 * 4), _lib.PTS_ERR_CAPACITY),
+    (dict(max_pages=(1 << 20) + 1), _lib.PTS_ERR_CAPACITY), (dict(num_rows=(1 << 17) + 1), _lib.PTS_ERR_CAPACITY)])
 def test_extend_refusals(kw, code):
     assert _extend(**kw) == code
 
@@ -47,10 +52,55 @@ def test_fork_truncate_and_compact_refusals():
     assert lib.pts_cache_fork(P, P, 4, P, 2, 4, 8, P, P, 1025, P, None) == _lib.PTS_ERR_CAPACITY
     assert lib.pts_cache_fork(P, P, 4, P, 2, 4, 8, P, P, 0, P, None) == _lib.PTS_ERR_INVALID
     assert lib.pts_cache_truncate(P, P, 4, P, 2, 4, 8, 0, P, None, 1, P, None) == _lib.PTS_ERR_INVALID
-    other = C.c_void_p(512)
-    ok = (P, 1, 8, 4, 32, P, P, 4, 2, 4)
-    assert lib.pts_cache_compact(*ok, P, other, other, other, other, 1 << 20, None) == _lib.PTS_ERR_INVALID
-    assert lib.pts_cache_compact(*ok, other, other, other, other, other, 8, None) == _lib.PTS_ERR_CAPACITY
+    def compact(out_refs, ws_bytes=1 << 20, out_table=512):
+        return lib.pts_cache_compact(_lib.pack_cache_compact(256, 32, 256, 256, 4, out_refs, out_table, 512, 512, 1, 8, 4, 2,
+                                                             4), P, ws_bytes, None)
+
+    assert compact(256) == _lib.PTS_ERR_INVALID              # the output is the input
+    assert compact(512, out_table=256) == _lib.PTS_ERR_INVALID
+    assert compact(512, ws_bytes=8) == _lib.PTS_ERR_CAPACITY
+
+
+def _attend(ws_bytes=256, **kw):
+    a = dict.fromkeys((n for n, _ in _lib.SHARED_ATTN_FIELDS), 256)
+    a.update(error=0, mask_words=1, num_groups=1, batch=2, total_q=2, max_qo_len=1, max_kv_len=40, max_own_len=0,
+             num_qo_heads=4, num_kv_heads=2, head_dim=96, page_len=16, max_pages=8, elem_bytes=4, sm_scale=0.1)
+    a.update(kw)
+    return _lib.lib().pts_tree_attn_run_shared(_lib.pack_shared_attn(*a.values()), P, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(q=0), _lib.PTS_ERR_INVALID), (dict(q=264), _lib.PTS_ERR_INVALID), (dict(shared_pages=0), _lib.PTS_ERR_INVALID),
+    (dict(num_groups=0), _lib.PTS_ERR_INVALID), (dict(num_qo_heads=5), _lib.PTS_ERR_INVALID),
+    (dict(max_qo_len=65), _lib.PTS_ERR_INVALID), (dict(max_qo_len=1025, mask_words=17), _lib.PTS_ERR_CAPACITY),
+    (dict(head_dim=48), _lib.PTS_ERR_UNSUPPORTED), (dict(head_dim=288), _lib.PTS_ERR_UNSUPPORTED),
+    (dict(elem_bytes=1), _lib.PTS_ERR_UNSUPPORTED), (dict(), _lib.PTS_ERR_CAPACITY)])
+def test_attention_refusals(kw, code):
+    assert _attend(**kw) == code
+
+
+@pytest.mark.parametrize("name,fields", [("pts_cache_extend_args", _lib.CACHE_EXTEND_FIELDS),
+                                         ("pts_cache_compact_args", _lib.CACHE_COMPACT_FIELDS),
+                                         ("pts_shared_attn_args", _lib.SHARED_ATTN_FIELDS)])
+def test_argument_structures_match_the_header(name, fields):
+    """Names, order and types of the packed fields are the header's, and their offsets C's."""
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, flags=re.S).group(1)
+    want = []
+    for decl in body.split(";"):
+        if not decl.strip():
+            continue
+        kind, names = re.match(r"\s*((?:const )?\w+\s*\*?)\s*(.*)", decl.strip(), flags=re.S).groups()
+        code = "P" if "*" in kind else {"int64_t": "q", "int": "i", "float": "f"}[kind.strip()]
+        want += [(n.strip(), code) for n in names.split(",")]
+    assert want == list(fields)
+    types = {"P": C.c_void_p, "q": C.c_int64, "i": C.c_int, "f": C.c_float}
+    S = type(name, (C.Structure,), {"_fields_": [(n, types[c]) for n, c in fields]})
+    values = [3 * i + 1 for i in range(len(fields))]
+    packed = _lib._packer(fields).pack(*values)
+    assert len(packed) == C.sizeof(S)
+    s = S.from_buffer_copy(packed)
+    assert [getattr(s, n) for n, _ in fields] == values
 
 
 def test_oracle_counts_holders():
