@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kWarps * 32) parts_kernel(const PartsParams p)
   for (int c = c0; c < c1; c += kTile) {
     bool odd = false;                                   // a value that 0 * v does not cancel
     __syncthreads();
+#pragma unroll 4
     for (int e = threadIdx.x; e < kTile * (D / 4); e += kWarps * 32) {
       const int t = e / (D / 4), d = e % (D / 4) * 4;
       float4 kx = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vx = kx;
@@ -267,14 +268,15 @@ struct Plan {
   size_t part_o, bytes;
 };
 
-// Slices so that about four CTAs per SM run, each of at least four tiles.
+// Slices so that about four CTAs per SM run, each of a tile at least: at the small sizes
+// this kernel is for, a tile's latency (some 5 us) is what counts.
 Plan make_plan(int batch, int groups, int total_q, int max_qo_len, int max_kv_len, int Hq, int Hkv, int D) {
   Plan pl;
   const int g = Hq / Hkv;
   pl.group_tiles = (int)(((int64_t)total_q * g + kRows - 1) / kRows) + groups;
   pl.request_tiles = (max_qo_len * g + kRows - 1) / kRows;
   const int64_t ctas = ((int64_t)pl.group_tiles + (int64_t)batch * pl.request_tiles) * Hkv;
-  const int64_t most = std::max<int64_t>(1, max_kv_len / (4 * kTile));
+  const int64_t most = std::max<int64_t>(1, (max_kv_len + kTile - 1) / kTile);
   pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * 148 / std::max<int64_t>(ctas, 1), most, 32}));
   const size_t slots = (size_t)total_q * Hq * 2 * pl.splits;
   pl.part_o = align_up(slots * sizeof(float2), 256);

@@ -78,11 +78,6 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = bad;
   if (bad) return;
   const int c0 = blockIdx.x * cols;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < n * cols; e += kForkThreads) {
-    const int c = c0 + e % cols;
-    stage[e] = c < s.width ? s.table[from[e / cols] * s.stride + c] : -1;
-  }
   int32_t len[kMaxForks / kForkThreads];
   if (blockIdx.x == 0) {
 #pragma unroll
@@ -91,24 +86,35 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
       if (i < n) len[k] = s.lens[from[i]];
     }
   }
-  __syncthreads();
-  for (int e0 = threadIdx.x; e0 < n * cols; e0 += 4 * kForkThreads) {
-    int old[4];
+  // entry e: column e % cols of fork e / cols; its new page waits in shared memory, the page
+  // it replaces in a register (the first kHeld of a thread's entries, else read again)
+  constexpr int kHeld = 4;
+  int old[kHeld];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {                       // four entries in flight
-      const int e = e0 + u * kForkThreads;
-      old[u] = e < n * cols && c0 + e % cols < s.width ? s.table[to[e / cols] * s.stride + c0 + e % cols] : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = e0 + u * kForkThreads;
-      if (e >= n * cols || c0 + e % cols >= s.width || old[u] == stage[e]) continue;
-      const int page = stage[e];
-      s.table[to[e / cols] * s.stride + c0 + e % cols] = page;
-      if (page >= 0 && page < s.pages) atomicAdd(&s.refs[page], 1);
-      if (old[u] >= 0 && old[u] < s.pages) atomicSub(&s.refs[old[u]], 1);
+  for (int u = 0; u < kHeld; ++u) {
+    const int e = threadIdx.x + u * kForkThreads, c = c0 + e % cols;
+    if (e < n * cols && c < s.width) {
+      stage[e] = s.table[from[e / cols] * s.stride + c];
+      old[u] = s.table[to[e / cols] * s.stride + c];
     }
   }
+  for (int e = threadIdx.x + kHeld * kForkThreads; e < n * cols; e += kForkThreads)
+    if (c0 + e % cols < s.width) stage[e] = s.table[from[e / cols] * s.stride + c0 + e % cols];
+  __syncthreads();
+  auto exchange = [&](int e, int before) {
+    const int page = stage[e];
+    if (page == before) return;
+    s.table[to[e / cols] * s.stride + c0 + e % cols] = page;
+    if (page >= 0 && page < s.pages) atomicAdd(&s.refs[page], 1);
+    if (before >= 0 && before < s.pages) atomicSub(&s.refs[before], 1);
+  };
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int e = threadIdx.x + u * kForkThreads;
+    if (e < n * cols && c0 + e % cols < s.width) exchange(e, old[u]);
+  }
+  for (int e = threadIdx.x + kHeld * kForkThreads; e < n * cols; e += kForkThreads)
+    if (c0 + e % cols < s.width) exchange(e, s.table[to[e / cols] * s.stride + c0 + e % cols]);
   if (blockIdx.x == 0) {
 #pragma unroll
     for (int k = 0; k < kMaxForks / kForkThreads; ++k) {
@@ -153,13 +159,16 @@ __global__ void __launch_bounds__(128) cache_truncate_kernel(PageState s, int pa
 // once into a bitmap; what follows is ranks in that bitmap.
 constexpr int kPlanThreads = 1024;
 
-// bitmap bit p = (refs[p] > 0) == live.  Four counts per load; eight lanes make a word.
-__device__ void build_bitmap(const int32_t* refs, int pages, bool live, uint32_t* bitmap) {
+// bitmap bit p = (refs[p] > 0) == live, for pages from `begin` (a multiple of kRound) to
+// `end`.  Four counts per load, eight loads in flight per thread; eight lanes make a word.
+constexpr int kRound = 8 * 4 * kPlanThreads;            // pages that one round of loads covers
+
+__device__ void build_bitmap(const int32_t* refs, int pages, bool live, uint32_t* bitmap, int begin, int end) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int quads = (pages + 3) / 4;
-  constexpr int kUnroll = 4;
+  const int quads = (min(pages, end) + 3) / 4;
+  constexpr int kUnroll = 8;
   const bool aligned = ((uintptr_t)refs & 15) == 0;
-  for (int q0 = warp * 32 * kUnroll; q0 < quads; q0 += kPlanThreads * kUnroll) {
+  for (int q0 = begin / 4 + warp * 32 * kUnroll; q0 < quads; q0 += kPlanThreads * kUnroll) {
     uint32_t nib[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -292,6 +301,7 @@ struct RowPlan {
   int r, old_len, need, copy, n_old, n_new;
 };
 
+template <int kPerThread>
 __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const ExtendParams p) {
   extern __shared__ uint32_t smem[];
   const int words = (p.s.pages + 31) / 32, row_words = (p.s.rows + 31) / 32;
@@ -301,7 +311,6 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
   __shared__ int below[kPlanThreads];
   __shared__ unsigned long long part[33];
   __shared__ int bad, pairs;
-  constexpr int kPerThread = kMaxBatch / kPlanThreads;
   const int tid = threadIdx.x;
   pdl_trigger();
   for (int i = tid; i < row_words; i += kPlanThreads) seen[i] = 0u;
@@ -347,7 +356,9 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
       }
     }
   }
-  build_bitmap(p.s.refs, p.s.pages, false, free_bits);
+  // the first round of counts comes in while the rows' pages are looked up
+  int scanned = min(p.s.pages, kRound);
+  build_bitmap(p.s.refs, p.s.pages, false, free_bits, 0, scanned);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
@@ -381,8 +392,18 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
     }
   }
   if (tid == 0) start[p.batch] = want;
-  const int per = (words + kPlanThreads - 1) / kPlanThreads;
-  const int have = rank_bitmap(free_bits, words, per, below, part);     // synchronises: start and bad are complete
+  // Fresh pages are the lowest free ones, so the counts are read only until there are enough
+  int per, have;
+  for (;;) {
+    const int w = (scanned + 31) / 32;
+    per = (w + kPlanThreads - 1) / kPlanThreads;
+    have = rank_bitmap(free_bits, w, per, below, part);   // synchronises: start and bad are complete
+    if (have >= want || scanned >= p.s.pages) break;
+    const int more = min(p.s.pages, scanned + 4 * kRound);
+    build_bitmap(p.s.refs, p.s.pages, false, free_bits, scanned, more);
+    scanned = more;
+    __syncthreads();
+  }
   int failed = bad;
   if (!failed && want > have) failed = kNoPages;
   if (failed) {
@@ -551,7 +572,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_compact_plan_kernel(const 
   pdl_trigger();
   pdl_wait();
   if (tid == 0) kept = 0;
-  build_bitmap(p.s.refs, p.s.pages, true, live);
+  build_bitmap(p.s.refs, p.s.pages, true, live, 0, p.s.pages);
   __syncthreads();
   const int n = rank_bitmap(live, words, per, below, part);
   int c = 0;                                            // live pages below n
@@ -727,9 +748,10 @@ extern "C" int pts_cache_extend(const pts_cache_extend_args* args, void* workspa
   p.layers = x.num_layers;
   p.row_bytes = x.row_bytes;
   const size_t smem = ((size_t)(x.max_pages + 31) / 32 + (x.num_rows + 31) / 32 + x.batch + 1) * 4;
+  auto plan = x.batch <= kPlanThreads ? cache_extend_plan_kernel<1> : cache_extend_plan_kernel<kMaxBatch / kPlanThreads>;
   if (smem > 32 * 1024)
-    if (int rc = ensure_smem_attr((const void*)cache_extend_plan_kernel, smem)) return rc;
-  PTS_CUDA_TRY(launch_pdl(cache_extend_plan_kernel, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, p));
+    if (int rc = ensure_smem_attr((const void*)plan, smem)) return rc;
+  PTS_CUDA_TRY(launch_pdl(plan, dim3(1), dim3(kPlanThreads), smem, (cudaStream_t)stream, p));
   if (int rc = launch_status("cache_extend_plan_kernel")) return rc;
   const int64_t units = std::max<int64_t>((int64_t)x.batch * 2 * x.num_layers, (x.batch + 7) / 8);
   PTS_CUDA_TRY(launch_pdl(cache_extend_apply_kernel, dim3((unsigned)std::min<int64_t>(copy_grid(), units)),
