@@ -21,7 +21,8 @@
 //   launched to run beside the second kernel, which is bound by its arithmetic: a CTA of
 //   two warps fits an SM next to that kernel's CTA (its ring and its registers are kept
 //   that small).
-// join_parts_kernel: joins every row's parts and writes the output.
+// join_parts_kernel: joins every row's parts and writes the output (join_tiles_kernel where
+//   the own columns are work items).
 //
 // Scores are kept in units of log2: x = s * scale * log2(e), e^(s - m) = 2^(x - m').
 #include <algorithm>
@@ -73,7 +74,7 @@ static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared
 
 // A column set: entries 0 .. groups - 1 are the groups' shared columns, groups + b the
 // own columns of request b (where they are work items).
-struct Entry {
+struct __align__(16) Entry {
   int tokens;     // columns
   int prefix;     // of those, the ones that every row sees; from there on the tree mask
   int rows;       // query rows per KV head
@@ -899,8 +900,9 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
   if (warp == 0) {
     // ------------------------------------------------------------ items and TMA producer
-    // Item k + 1 is claimed and read while item k loads.  Lane r brings the r-th copy of a
-    // block.  The page of load x + 4 is fetched while load x is issued (unrolled by four,
+    // Item k + 1 is claimed when item k's last copies have been issued, a ring's length
+    // before it ends (any earlier, a CTA holds a second item while others have none).
+    // Lane r brings the r-th copy of a block.  The page of load x + 4 is fetched while load x is issued (unrolled by four,
     // so that no register that a fetch is still filling is moved).
     pdl_wait();
     const int total = __ldcg(&p.head->total);
@@ -910,8 +912,6 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
     for (int k = 0; ok; ++k) {
       const bool more = mine < total;
       const Item it = p.items[min(mine, p.max_items - 1)];   // (read beside the total, not after it)
-      int claim = 0;
-      if (lane == 0 && more) claim = atomicAdd(&p.head->next, 1);
       // the slot's last item, k - 2, has been copied by everyone
       ok = k < 2 || __all_sync(0xffffffffu, mbar_wait(&bars.item_free[k & 1], ((k >> 1) + 1) & 1, p.wait_limit));
       if (!ok) break;
@@ -977,7 +977,8 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
         push(x + 3, p3);
         p3 = fetch(x + 7);
       }
-      mine = __shfl_sync(0xffffffffu, claim, 0);
+      if (lane == 0) mine = atomicAdd(&p.head->next, 1);
+      mine = __shfl_sync(0xffffffffu, mine, 0);
     }
     if (!ok && lane == 0) give_up(p, 51);
     // the copies in flight must land before the CTA can exit
@@ -1151,7 +1152,12 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
   }
 }
 
-// ---------------------------------------------------------------- third kernel
+// ----------------------------------------------------------------------- joining
+__device__ __forceinline__ Entry load_entry(const Entry* e) {
+  const int4 x = __ldcg((const int4*)e), y = __ldcg((const int4*)e + 1);
+  return Entry{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+
 // A CTA joins 16 rows of a request and KV head: the parts of its group's shared columns,
 // and those of its own.  A thread has a row and a column quad -- four rows and eight
 // quads per warp, so that both the parts ([quad][row]) and the output are touched in
@@ -1180,9 +1186,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
   // A stored part is [quad][128 rows] with m and l behind; own_attn_kernel's are [quad] with
   // (m, l) apart.
   const Entry group = p.entries[gi];
-  Entry mine = group;
-  if (p.own_items) mine = p.entries[a.groups + b];
-  const int shared = group.splits, own = p.own_items ? mine.splits : p.own_splits, parts = shared + own;
+  const int shared = group.splits, parts = shared + p.own_splits;
   auto part_of = [&](const Entry& e, int R, int& in) -> const float* {   // the first part's half with row R, its place
     const int at = (tok0 - e.tok0) * a.g + R, tile = at / kTileRows;
     in = at & 127;
@@ -1194,7 +1198,6 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
     return (int64_t)(tok0 + tk) * a.Hq + h * a.g + R - tk * a.g;
   };
   const int units = (n + 3) / 4 * D, slices = max(1, kJoinThreads / units);
-  const int64_t own_step = p.own_items ? kPart : D;
   // this thread's place in round `idx`: row, quad, first parts
   int r = 0, quad = 0;
   const float *s0 = nullptr, *s1 = nullptr;
@@ -1206,19 +1209,14 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
     int in;
     s0 = part_of(group, R, in);
     s0 += quad * 512 + in * 4;
-    if (p.own_items) {
-      s1 = part_of(mine, R, in);
-      s1 += quad * 512 + in * 4;
-    } else {
-      s1 = p.own_o + row_of(R) * p.own_splits * D + quad * 4;
-    }
+    s1 = p.own_o + row_of(R) * p.own_splits * D + quad * 4;
   };
   float4 v[kJoinAhead];
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < kJoinAhead; ++u) {
       const int k = k0 + u * slices;
-      if (k < parts) v[u] = __ldcg((const float4*)(k < shared ? s0 + (int64_t)k * kPart : s1 + (k - shared) * own_step));
+      if (k < parts) v[u] = __ldcg((const float4*)(k < shared ? s0 + (int64_t)k * kPart : s1 + (int64_t)(k - shared) * D));
     }
   };
   int idx = threadIdx.x;
@@ -1232,14 +1230,13 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
     const int rr = e % kJoinRows, k = e / kJoinRows, R = row0 + rr;
     float m = -INFINITY, l = 0.0f;
     if (rr < n) {
-      if (k >= shared && !p.own_items) {
+      if (k >= shared) {
         const float2 x = __ldcg(p.own_ml + row_of(R) * p.own_splits + (k - shared));
         m = x.x;
         l = x.y;
       } else {
         int in;
-        const float* s = k < shared ? part_of(group, R, in) + (int64_t)k * kPart
-                                    : part_of(mine, R, in) + (int64_t)(k - shared) * kPart;
+        const float* s = part_of(group, R, in) + (int64_t)k * kPart;
         m = __ldcg(s + 128 * D + in);
         l = __ldcg(s + 128 * D + 128 + in);
       }
@@ -1306,19 +1303,77 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
   }
 }
 
+// The same where own columns are work items: many rows and few parts, so a warp takes four
+// rows, and a lane the quads q, q + 8, .. of one; a part's m, l and O are all asked for at
+// once, and the sums are rescaled as the maximum grows.
+constexpr int kTilesThreads = 128;
+
+template <int D>
+__global__ void __launch_bounds__(kTilesThreads, 8) join_tiles_kernel(const PrefixParams p, int row_tiles) {
+  constexpr int kPart = Shape<D>::kPartFloats, kHalf = kPart / 2, kQuads = D / 32;
+  const SharedAttnParams& a = p.a;
+  const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  const int b = blockIdx.x / row_tiles, h = blockIdx.y;
+  const int row0 = (blockIdx.x - b * row_tiles) * kJoinRows + threadIdx.x / 32 * 4;
+  const int tok0 = a.qo_indptr[b], rows = (a.qo_indptr[b + 1] - tok0) * a.g, group = group_of(a, b);
+  pdl_wait();                                           // (the lengths are no kernel's of this call)
+  if (row0 >= rows) return;
+  const Entry shared = load_entry(p.entries + group), own = load_entry(p.entries + a.groups + b);
+  const int r = min(row0 + (lane & 3), rows - 1), R = r + (tok0 - shared.tok0) * a.g, parts = shared.splits + own.splits;
+  auto part_of = [&](const Entry& e, int at) -> const float* {
+    return p.parts + ((int64_t)e.first + (int64_t)(h * tiles_of(e.rows) + at / kTileRows) * e.splits) * kPart +
+           ((at >> 7) & 1) * kHalf + (at & 127);
+  };
+  const float *s0 = part_of(shared, R), *s1 = part_of(own, r);
+  float M = -INFINITY, L = 0.0f;
+  float4 acc[kQuads];
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int k = 0; k < parts; ++k) {
+    const float* s = k < shared.splits ? s0 + (int64_t)k * kPart : s1 + (int64_t)(k - shared.splits) * kPart;
+    const int in = (k < shared.splits ? R : r) & 127;
+    const float m = __ldcg(s + 128 * D), l = __ldcg(s + 128 * D + 128);
+    float4 v[kQuads];
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) v[j] = __ldcg((const float4*)(s - in + (8 * j + (lane >> 2)) * 512 + in * 4));
+    const float top = fmaxf(M, m), base = top == -INFINITY ? 0.0f : top;
+    const float f = fast_exp2(M - base), w = fast_exp2(m - base);
+    L = f * L + w * l;
+    M = top;
+    // a part of no columns has no O
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) {
+      acc[j].x = (f != 0.0f ? f * acc[j].x : 0.0f) + (w != 0.0f ? w * v[j].x : 0.0f);
+      acc[j].y = (f != 0.0f ? f * acc[j].y : 0.0f) + (w != 0.0f ? w * v[j].y : 0.0f);
+      acc[j].z = (f != 0.0f ? f * acc[j].z : 0.0f) + (w != 0.0f ? w * v[j].z : 0.0f);
+      acc[j].w = (f != 0.0f ? f * acc[j].w : 0.0f) + (w != 0.0f ? w * v[j].w : 0.0f);
+    }
+  }
+  if (row0 + (lane & 3) >= rows) return;
+  const float c = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;        // nothing seen: 0
+  const int tk = p.div_g.div(r);
+  uint16_t* out = (uint16_t*)a.out + ((int64_t)(tok0 + tk) * a.Hq + h * a.g + r - tk * a.g) * D + (lane >> 2) * 4;
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j)
+    *(uint2*)(out + 32 * j) = make_uint2(pack_bf16x2(acc[j].x * c, acc[j].y * c), pack_bf16x2(acc[j].z * c, acc[j].w * c));
+}
+
 struct PrefixPlan {
   int few, direct, own_rows, own_splits, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
 int sm_count() {
-  static int count = 0;
-  if (!count) {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
-      count = n;
-  }
-  return count ? count : 148;
+  static std::atomic<int> counts[64];                   // per device
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  n = counts[dev].load();
+  if (n) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  counts[dev].store(n);
+  return n;
 }
 
 PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int max_kv_len, int max_own_len, int Hq,
@@ -1398,7 +1453,8 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
   if (int rc = encode_kv<D>(&block_map, p.a, p.copy_tokens)) return rc;
   // (the small kernels ask for the same shared-memory split, which an SM changes only when idle)
   if (int rc = ensure_smem_attr((const void*)plan_kernel, 1, true)) return rc;
-  if (int rc = ensure_smem_attr((const void*)join_parts_kernel<D>, 1, true)) return rc;
+  if (int rc = ensure_smem_attr(f.few ? (const void*)join_parts_kernel<D> : (const void*)join_tiles_kernel<D>, 1, true))
+    return rc;
   PTS_CUDA_TRY(launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p));
   if (int rc = launch_status("plan_kernel")) return rc;
   if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem, true)) return rc;
@@ -1418,8 +1474,9 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
                                  : launch_own<D, 2, kOwnWarps, false>(p, run_map, stream))
       return rc;
   const int row_tiles = (int)(((int64_t)max_qo_len * p.a.g + kJoinRows - 1) / kJoinRows);
-  PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, dim3(p.a.batch * row_tiles, p.a.Hkv), dim3(kJoinThreads), 0,
-                          stream, p, row_tiles));
+  const dim3 grid(p.a.batch * row_tiles, p.a.Hkv);
+  if (f.few) PTS_CUDA_TRY(launch_pdl(join_parts_kernel<D>, grid, dim3(kJoinThreads), 0, stream, p, row_tiles));
+  else PTS_CUDA_TRY(launch_pdl(join_tiles_kernel<D>, grid, dim3(kTilesThreads), 0, stream, p, row_tiles));
   return launch_status("join_parts_kernel");
 }
 
