@@ -158,7 +158,9 @@ class BeFlashinferWrapper:
             self.append_kv_cache(q, k, v, append_pos, cacheData, self.page_len)
         bp = plan["bp"]
         scale = 1.0 / math.sqrt(self._head_padded_dim)
-        if bp.shared_pages is not None:
+        if bp.shared_pages is not None and K.sharing_pays(plan["max_qo"], bp.seq_indptr.numel() - 1,
+                                                          self.num_attention_heads, self.num_key_value_heads,
+                                                          cacheData.shape[-1], self.page_len, cacheData.dtype):
             out = K.tree_attention_shared(q.contiguous(), cacheData, bp.seq_indptr, bp.kv_page_indptr,
                                           bp.kv_page_indices, bp.kv_last_page_len, plan["bits"], plan["max_qo"],
                                           plan["max_kv"], bp.group_indptr, bp.shared_pages,

@@ -14,6 +14,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -661,8 +662,14 @@ int check_pool(const void* pool, int layers, int page_len, int64_t row_bytes) {
 }
 
 int copy_grid() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<int> counts[64];                    // SMs per device
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148 * 4;
+  sms = counts[dev].load();
+  if (!sms) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+    counts[dev].store(sms);
+  }
   return sms * 4;
 }
 

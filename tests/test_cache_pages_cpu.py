@@ -119,3 +119,14 @@ def test_oracle_counts_holders():
         held = np.bincount([p for row in s.table for p in row if p >= 0], minlength=70)
         assert held.tolist() == s.refs
         assert all(len([p for p in row if p >= 0]) == oc.pages_of(n, 4) for row, n in zip(s.table, s.lens))
+
+
+@pytest.mark.parametrize("rows,batch,Hq,Hkv,D,page,dtype,pays", [
+    (1, 64, 32, 8, 128, 16, torch.bfloat16, True), (65, 16, 32, 8, 128, 16, torch.bfloat16, False),
+    (49, 16, 32, 8, 128, 16, torch.bfloat16, True), (50, 16, 32, 8, 128, 16, torch.bfloat16, False),
+    (33, 16, 32, 8, 128, 16, torch.bfloat16, True), (65, 13, 32, 8, 128, 16, torch.bfloat16, True),
+    (65, 14, 32, 8, 128, 16, torch.bfloat16, False), (67, 14, 32, 8, 128, 16, torch.bfloat16, True),
+    (65, 16, 32, 8, 64, 16, torch.bfloat16, True), (65, 16, 32, 8, 128, 32, torch.bfloat16, True),
+    (65, 16, 32, 8, 128, 16, torch.float32, True), (65, 64, 64, 2, 128, 16, torch.bfloat16, True)])
+def test_sharing_pays(rows, batch, Hq, Hkv, D, page, dtype, pays):
+    assert K.sharing_pays(rows, batch, Hq, Hkv, D, page, dtype) is pays

@@ -238,3 +238,45 @@ def test_a_wait_that_runs_out_is_reported(groups):
         K.set_wait_limit(before)
     assert torch.equal(K.tree_attention_shared(**a), want)
     K.check_attention(torch.device(DEV))
+
+
+def test_full_tree_tiles_go_to_the_call_that_reads_per_request():
+    """Fourteen requests with trees that fill tree_attention's units: the wrapper takes
+    that call, and the shared one after single tokens; both answers are the same up to the
+    rounding of the probabilities and of the output."""
+    page, Hq, Hkv, D, B = 16, 32, 8, 128, 14
+    pool = KvCachePool(160, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, B, 16)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    gen = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(DEV)
+    calls, real = [], (K.tree_attention, K.tree_attention_shared)
+
+    def step(rows, parents):
+        bp = cache.extend(rows, [len(p) for p in parents])
+        w.set_tree_masks(torch.tensor(sum(parents, []), dtype=torch.int32, device=DEV), bp, max(map(len, parents)))
+        T = sum(map(len, parents))
+        q = rnd(T, Hq, D)
+        K.tree_attention = lambda *a, **kw: (calls.append("tree"), real[0](*a, **kw))[1]
+        K.tree_attention_shared = lambda *a, **kw: (calls.append("shared"), real[1](*a, **kw))[1]
+        try:
+            out = w.computeAttention(q, rnd(T, Hkv, D), rnd(T, Hkv, D), pool.cache_data[0], "tree", bp,
+                                     AttentionRotaryParams(), 0)
+        finally:
+            K.tree_attention, K.tree_attention_shared = real
+        args = (q, pool.cache_data[0], bp.seq_indptr, bp.kv_page_indptr, bp.kv_page_indices, bp.kv_last_page_len,
+                w._plan["bits"], w._plan["max_qo"], w._plan["max_kv"])
+        a = real[0](*args).double()
+        b = real[1](*args, bp.group_indptr, bp.shared_pages).double()
+        # sum p |v| is at most the largest |v|: two roundings to 2^-8 of each, and the output's
+        most = pool.cache_data[0][:, 1].abs().max().item()
+        assert (a - b).abs().max().item() <= 2 * (2 * 2.0 ** -8 + 2.0 ** -12) * most
+        assert torch.equal(out.view(T, Hq, D).double(), a if calls[-1] == "tree" else b)
+
+    step([0], [chain(70)])
+    cache.fork([0] * (B - 1), list(range(1, B)))
+    step(list(range(B)), [tree(i, 8, 8) for i in range(B)])
+    cache.truncate(list(range(B)), [72] * B)
+    step(list(range(B)), [chain(1)] * B)
+    cache.check()
+    assert calls == ["shared", "tree", "shared"]
