@@ -350,7 +350,8 @@ int pts_kv_compact(void* kv_pool, int num_layers, int max_pages, int page_len, i
  * The calls write an int32 status: 0, or a sum of
  *   1 a row outside the table or a negative count   2 a row listed twice
  *   4 a sequence longer than the table is wide       8 not enough free pages
- * pts_cache_fork and pts_cache_extend change nothing when it is not 0.  At most
+ * pts_cache_fork and pts_cache_extend change nothing when it is not 0, and the batch
+ * of such an extend is one of empty sequences (an append to it writes nothing).  At most
  * 2^17 rows, 2^20 pages, 1024 forks and 4096 extended rows a call.  Calls on the
  * same state belong on one stream.
  *

@@ -54,7 +54,8 @@ class PageState:
         return 0
 
     def extend(self, rows: Sequence[int], add: Sequence[int], groups: Optional[Sequence[int]] = None):
-        """(status, page lists, lengths, shared leading pages per group)."""
+        """(status, page lists, lengths, shared leading pages per group); a call that cannot
+        be done changes nothing and returns a batch of empty sequences."""
         code, seen, grow = 0, set(), []
         for r, a in zip(rows, add):
             if not 0 <= r < len(self.table) or a < 0:
@@ -95,14 +96,13 @@ class PageState:
                 self.refs[p] = 1
             for r, a in zip(rows, add):
                 self.lens[r] += a
-        valid = [0 <= r < len(self.table) and a >= 0 for r, a in zip(rows, add)]
-        lists = [self._pages(r) if ok else [] for r, ok in zip(rows, valid)]
-        lens = [self.lens[r] if ok else 0 for r, ok in zip(rows, valid)]
+        lists = [[] if code else self._pages(r) for r in rows]
+        lens = [0 if code else self.lens[r] for r in rows]
         shared = []
         if groups is not None:
             for a, z in zip(groups[:-1], groups[1:]):
                 n = 0
-                while a < z and all(n < old[i] // self.page_len and lists[i][n] == lists[a][n] for i in range(a, z)):
+                while not code and a < z and all(n < old[i] // self.page_len and lists[i][n] == lists[a][n] for i in range(a, z)):
                     n += 1
                 shared.append(n)
         return code, lists, lens, shared

@@ -211,8 +211,9 @@ class SharedKvCache:
     (sequence numbers) and lengths may be lists or int32 tensors on the pool's device;
     tensors keep every call free of host copies and synchronisations, so a step can be
     captured in a CUDA graph (not ``compact``, which replaces the state's tensors).  A
-    call that cannot be done changes nothing; ``check`` raises for it.  The cache takes
-    all pages of the pool, which must be free, until ``close``."""
+    call that cannot be done changes nothing (the batch position of such an ``extend`` has
+    empty sequences, so an append to it writes nothing); ``check`` raises for it.  The
+    cache takes all pages of the pool, which must be free, until ``close``."""
 
     def __init__(self, pool: KvCachePool, max_sequences: int, max_pages_per_sequence: int):
         if pool.num_free_pages() != pool.max_pages:
@@ -299,7 +300,8 @@ class SharedKvCache:
         self.truncate(rows)
 
     def compact(self) -> torch.Tensor:
-        """Close the pool's gaps; returns the map from old to new page (-1: free)."""
+        """Close the pool's gaps; returns the map from old to new page (-1: free).  Batch
+        positions from before name the old pages."""
         r = K.cache_compact(self.pool.cache_data, self.page_refs, self.page_table)
         self.page_refs, self.page_table = r.page_refs, r.page_table
         return r.page_map

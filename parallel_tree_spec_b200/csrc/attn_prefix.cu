@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
   for (int g = warp; g < a.groups; g += warps) {
     int lead;
     const int pages = group_shared_pages(a, g, &lead);
-    const int b0 = a.group_indptr[g], b1 = a.group_indptr[g + 1];
-    const int tok0 = a.qo_indptr[b0], rows = (a.qo_indptr[b1] - tok0) * a.g;
+    const int2 range = group_requests(a, g);
+    const int tok0 = a.qo_indptr[range.x], rows = (a.qo_indptr[range.y] - tok0) * a.g;
     if (lane == 0) {
       const int tokens = rows > 0 ? pages * a.page_len : 0;
       entry[g] = Entry{tokens, tokens, rows, tok0, rows > 0 ? a.page_indptr[lead] : 0, 0, 0, rows > 0 ? pages : 0};

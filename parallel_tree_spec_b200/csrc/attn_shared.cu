@@ -71,13 +71,14 @@ __global__ void __launch_bounds__(kWarps * 32) parts_kernel(const PartsParams p)
     own = false;
     int left = blockIdx.x, gi = 0;
     for (; gi < a.groups; ++gi) {
-      n_tok = a.qo_indptr[a.group_indptr[gi + 1]] - a.qo_indptr[a.group_indptr[gi]];
+      const int2 range = group_requests(a, gi);
+      n_tok = a.qo_indptr[range.y] - a.qo_indptr[range.x];
       const int tiles = (n_tok * a.g + kRows - 1) / kRows;
       if (left < tiles) break;
       left -= tiles;
     }
     if (gi == a.groups) return;
-    b0 = a.group_indptr[gi];
+    b0 = group_requests(a, gi).x;
     tok0 = a.qo_indptr[b0];
     row0 = left * kRows;
     // the table of the group's first request with rows

@@ -43,7 +43,13 @@ struct SharedAttnParams {
 // Tokens of request b's cache and, of those, the ones before its query rows.
 __device__ __forceinline__ int kv_tokens(const SharedAttnParams& p, int b) {
   const int n = p.page_indptr[b + 1] - p.page_indptr[b];
-  return n > 0 ? (n - 1) * p.page_len + p.last_page_len[b] : 0;
+  return n > 0 ? (n - 1) * p.page_len + min(max(p.last_page_len[b], 0), p.page_len) : 0;
+}
+
+// The requests of group gi, within the batch whatever group_indptr holds.
+__device__ __forceinline__ int2 group_requests(const SharedAttnParams& p, int gi) {
+  const int b0 = min(max(p.group_indptr[gi], 0), p.batch);
+  return make_int2(b0, min(max(p.group_indptr[gi + 1], b0), p.batch));
 }
 
 // The pages of group gi that its rows attend together: shared_pages[gi], but none
@@ -52,7 +58,8 @@ __device__ __forceinline__ int kv_tokens(const SharedAttnParams& p, int b) {
 // request with rows, or the one past its last.
 __device__ __forceinline__ int group_shared_pages(const SharedAttnParams& p, int gi, int* lead = nullptr) {
   const int lane = threadIdx.x & 31;
-  const int b0 = p.group_indptr[gi], b1 = p.group_indptr[gi + 1];
+  const int2 range = group_requests(p, gi);
+  const int b0 = range.x, b1 = range.y;
   int s = p.shared_pages[gi], first = b1;
 #pragma unroll 4
   for (int b = b0 + lane; b < b1; b += 32) {

@@ -283,7 +283,6 @@ struct ExtendParams {
   int page_len;
   int32_t* page_indptr;
   int32_t* page_indices;
-  int64_t capacity;          // entries of page_indices
   int32_t* last_page_len;
   int32_t* seq_lens;
   int32_t* shared_pages;     // null: not wanted
@@ -299,7 +298,7 @@ struct ExtendParams {
 };
 
 struct RowPlan {
-  int r, old_len, need, copy, n_old, n_new;
+  int r, old_len, need, copy, n_new;
 };
 
 template <int kPerThread>
@@ -324,7 +323,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
     const int i = tid * per_row + k;
-    row[k] = RowPlan{-1, 0, 0, 0, 0, 0};
+    row[k] = RowPlan{-1, 0, 0, 0, 0};
     last[k] = -1;
     if (k >= per_row || i >= p.batch) continue;
     const int r = p.rows[i], add = p.add_each ? p.add_each[i] : p.add;
@@ -341,15 +340,16 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
     }
     row[k].r = r;
     row[k].old_len = len;
-    row[k].n_old = row[k].n_new = (int)(((long long)len + p.page_len - 1) / p.page_len);
+    row[k].n_new = (int)(((long long)len + p.page_len - 1) / p.page_len);
     if (now > most) {
       atomicOr(&bad, kTooLong);
       continue;
     }
+    const int n_old = row[k].n_new;
     row[k].n_new = (int)((now + p.page_len - 1) / p.page_len);
-    row[k].need = row[k].n_new - row[k].n_old;
+    row[k].need = row[k].n_new - n_old;
     if (add > 0 && len % p.page_len) {
-      const int page = p.s.table[r * p.s.stride + row[k].n_old - 1];
+      const int page = p.s.table[r * p.s.stride + n_old - 1];
       if (page >= 0 && page < p.s.pages && __ldcg(p.s.refs + page) > 1) {
         last[k] = page;
         p.holders[page] = 0;
@@ -407,25 +407,15 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
   }
   int failed = bad;
   if (!failed && want > have) failed = kNoPages;
-  if (failed) {
-    // unchanged: the batch's lists as they are, rows outside the table empty
-    lists = 0;
-#pragma unroll
-    for (int k = 0; k < kPerThread; ++k) {
-      row[k].need = row[k].copy = 0;
-      row[k].n_new = row[k].n_old;
-      lists += row[k].n_new;
-    }
-    list_before = (int)block_scan((unsigned long long)(unsigned)lists, part, &totals);
-    totals <<= 32;
-  }
+  // Unchanged, and a batch of empty sequences: an append to it writes nothing (its tokens'
+  // positions would otherwise be the last ones that are there, on pages that others may hold)
   if (tid == 0) {
     *p.status = failed;
     p.page_indptr[0] = 0;
   }
   if (p.shared_pages)
     for (int g = tid; g < p.groups; g += kPlanThreads)
-      p.shared_pages[g] = p.group_indptr[g + 1] > p.group_indptr[g] ? INT_MAX : 0;
+      p.shared_pages[g] = !failed && p.group_indptr[g + 1] > p.group_indptr[g] ? INT_MAX : 0;
   __syncthreads();
   // each listed row: its length and its place in the batch's lists; its shared page goes back
 #pragma unroll
@@ -433,8 +423,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
     const int i = tid * per_row + k;
     if (k >= per_row || i >= p.batch) continue;
     const int add = p.add_each ? p.add_each[i] : p.add;
-    const int now = row[k].old_len + (failed || row[k].r < 0 ? 0 : add);
-    list_before += row[k].n_new;
+    const int now = failed ? 0 : row[k].old_len + add;
+    list_before = failed ? 0 : list_before + row[k].n_new;
     p.page_indptr[i + 1] = list_before;
     p.seq_lens[i] = now;
     p.last_page_len[i] = now > 0 ? (now - 1) % p.page_len + 1 : 0;
@@ -449,7 +439,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
         p.pairs[3 * at + 2] = row[k].old_len % p.page_len;
       }
     }
-    if (p.shared_pages && p.groups > 0) {
+    if (!failed && p.shared_pages && p.groups > 0) {
       int lo = 0, hi = p.groups;                        // the group of row i
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -529,7 +519,7 @@ __global__ void __launch_bounds__(kCopyThreads) cache_extend_apply_kernel(const 
     int differs = INT_MAX;
     for (int j = lane; j < n; j += 32) {
       const int page = mine[j];
-      if (at + j < p.capacity) p.page_indices[at + j] = page;
+      p.page_indices[at + j] = page;
       if (j < limit && differs == INT_MAX && first[j] != page) differs = j;
     }
     if (limit > 0) {
@@ -742,7 +732,6 @@ extern "C" int pts_cache_extend(const pts_cache_extend_args* args, void* workspa
   p.page_len = x.page_len;
   p.page_indptr = x.page_indptr;
   p.page_indices = x.page_indices;
-  p.capacity = x.page_indices_size;
   p.last_page_len = x.last_page_len;
   p.seq_lens = x.seq_lens;
   p.shared_pages = x.shared_pages;

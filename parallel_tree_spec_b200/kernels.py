@@ -975,7 +975,7 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     ``tree_attention_shared``.  ``out``: (page_indptr [B + 1], page_indices [B * W],
     last_page_len [B], seq_lens [B], shared_pages [G] or None) to write into; entries of
     page_indices past page_indptr[B] are left as they are.  A call that cannot be done
-    (see the status) changes nothing."""
+    (see the status) changes nothing and returns a batch of empty sequences."""
     index = _page_state(page_refs, page_table, kv_lens)
     L, P, pl, row_bytes = _page_pool(pool, page_refs)
     B, (R, W) = _cache_ints("rows", rows, index).shape[0], page_table.shape

@@ -280,3 +280,32 @@ def test_full_tree_tiles_go_to_the_call_that_reads_per_request():
     step(list(range(B)), [chain(1)] * B)
     cache.check()
     assert calls == ["shared", "tree", "shared"]
+
+
+def test_a_failed_extend_leaves_the_cache_to_later_calls_of_the_step():
+    """The step goes on before its status is read: the append to the failed batch must not
+    write over the sequences' last tokens, whose pages others hold."""
+    page, Hkv, D = 4, 2, 64
+    pool = KvCachePool(5, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, 3, 6)
+    w = BeFlashinferWrapper(4, Hkv, 4 * D, page, torch.device(DEV))
+    ones = lambda n, h: torch.ones(n, h, D, dtype=torch.bfloat16, device=DEV)
+
+    def step(rows, n):
+        bp = cache.extend(rows, n)
+        w.set_tree_masks(torch.tensor(chain(n) * len(rows), dtype=torch.int32, device=DEV), bp, n)
+        T = n * len(rows)
+        return bp, w.computeAttention(ones(T, 4), ones(T, Hkv), 2 * ones(T, Hkv), pool.cache_data[0], "tree", bp,
+                                      AttentionRotaryParams(), 0)
+
+    pool.cache_data.zero_()
+    bp, out = step([0], 14)
+    assert bp.kv_page_indptr.tolist() == [0, 4] and (out == 2).all()
+    cache.fork([0, 0], [1, 2])
+    before = pool.cache_data.clone()
+    bp, out = step([1, 2], 3)                                 # two copies and two pages: only one is free
+    assert torch.equal(pool.cache_data, before)
+    assert bp.kv_page_indptr.tolist() == [0, 0, 0] and bp.shared_pages.tolist() == [0] and (out == 0).all()
+    with pytest.raises(RuntimeError):
+        cache.check()
+    assert cache.kv_lens.tolist() == [14, 14, 14]
