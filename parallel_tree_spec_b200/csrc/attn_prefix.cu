@@ -49,7 +49,10 @@ static_assert(128 * kHelperRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, 
 constexpr int kMaxSplits = 32;            // block ranges of a column set
 constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in own_attn_kernel
 constexpr int kDirectCost = 3600;          // in tokens' time: the rounds' 3 us count 600 each
-constexpr int kFewRows = 16;              // rows per KV head up to which own_attn_kernel takes them
+// Rows per KV head up to which own_attn_kernel takes the own columns: 64 requests of 8192
+// shared and 300 own tokens take, with it and with work items, 46 and 63 us at 4 rows, 55
+// and 76 at 8, 73 and 84 at 12, 97 and 93 at 16 (114 and 120 with 2048 and 1500 tokens).
+constexpr int kFewRows = 16;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
 
@@ -190,7 +193,8 @@ constexpr int kPlanCache = 512;           // entries that the plan keeps in shar
 // The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
 // and end cost about one and a half), and the launch about the larger of the total over
 // the CTAs and the large items' rounds; the cheapest of up to 32 ranges of
-// ceil(longest / k) blocks is taken.
+// ceil(longest / k) blocks is taken.  Bound by the chain of its loads and barriers: 4-6 us,
+// 7-8 from a cold cache, for 64 requests as for 16.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p) {
   __shared__ int sums[64 + 4];                          // [2][32] items, large items; red
   __shared__ Entry cache[kPlanCache];                   // the first entries, as in p.entries
@@ -322,6 +326,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
 // the end.  Transposed, a product's 16 rows are tokens or dimensions, all of them
 // in use, and the 8 columns are query rows: half the products of the plain form at 8
 // rows or fewer.
+// 64 requests with 225 own tokens on average, 8 KV heads of 128 (59 MB): 19 us by itself,
+// 3.1 TB/s -- a pair's 14 runs are over before the ring has paid for its start -- and 35 us
+// beside prefix_attn_kernel, whose 25 us it hides.
 // kDirect: all columns, the shared ones too, and the output itself: for small calls, where
 // reading a short prefix once per request costs less than the plan and the join.
 template <int D, int NR, int NW, bool kDirect>
@@ -616,6 +623,13 @@ __device__ __forceinline__ bool masked_block(const Item& it, int j) {
   return it.own && (it.ja + j + 1) * kBlock > it.prefix;
 }
 
+// Bound by the chain of a stream's block: scores from TMEM, their maximum, the exponentials,
+// P to TMEM, the two products.  128 tokens of 256 rows of head_dim 128 take 2.2 us (7.6
+// TFLOP/s of an SM; all of them 68 % of the measured matrix rate), of which the products
+// alone are 2048 clocks and the exponentials as many.  An item costs 5-9 us more for its
+// start and its parts.  16 requests of up to 65 nodes with 4096 shared tokens: 77-90 us,
+// the matrix pipe 30 % busy over the launch; 32 decoding requests with 65536 shared tokens:
+// the cache at 5.2 TB/s.
 template <int D>
 __global__ void __launch_bounds__(kBoundThreads, 1)
     prefix_attn_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kv_map) {
@@ -1163,7 +1177,8 @@ __device__ __forceinline__ Entry load_entry(const Entry* e) {
 // quads per warp, so that both the parts ([quad][row]) and the output are touched in
 // 64-byte pieces -- and, with few rows, every slices-th of the parts.  Bound by the
 // latency of reading what other SMs have just written: the first O values are asked for
-// together with the parts' m and l, which become weights e^(m - M) meanwhile.
+// together with the parts' m and l, which become weights e^(m - M) meanwhile.  256 rows of
+// 8 KV heads with 17 parts each (18 MB): 5-7 us.
 constexpr int kJoinRows = 16;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinAhead = 6;             // O values in flight per thread
@@ -1305,7 +1320,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_parts_kernel(const Prefi
 
 // The same where own columns are work items: many rows and few parts, so a warp takes four
 // rows, and a lane the quads q, q + 8, .. of one; a part's m, l and O are all asked for at
-// once, and the sums are rescaled as the maximum grows.
+// once, and the sums are rescaled as the maximum grows.  3500 rows of 8 KV heads with two
+// parts each (29 MB and 7 MB of output): 10 us, 16 from a cold cache; through the kernel
+// above, two barriers between its loads, 18.
 constexpr int kTilesThreads = 128;
 
 template <int D>
@@ -1385,9 +1402,9 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   f.own_rows = rows <= 8 ? 8 : 16;
   f.ctas = sm_count();
   // One launch that reads each request's columns takes about 3 us + 5 ns a token for each
-  // round of (request, KV head) pairs over the SMs (512 tokens: 6.4 us at 48 pairs of
-  // head_dim 64, 7.7 at 128 pairs of 128; 1900: 12.4 and 14.4); the plan, the work items
-  // and the join take 16 to 25 us for the same calls.
+  // round of (request, KV head) pairs over the SMs.  It and the other way, in us: 512
+  // tokens 6.6 and 16.1 with 48 pairs of head_dim 64, 7.9 and 18.6 with 128 of 128; 1900
+  // tokens 12.1 and 17.6, 14.2 and 21.8; 1100 tokens, 240 pairs of 128 19.3 and 21.5.
   f.direct = f.few && ((batch * (int64_t)Hkv + f.ctas - 1) / f.ctas) * (600 + (int64_t)max_kv_len) <= kDirectCost;
   if (f.direct) {
     f.own_splits = 1;

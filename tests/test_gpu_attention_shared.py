@@ -235,6 +235,21 @@ def test_bad_value_reaches_only_the_rows_that_see_it(dtype):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("shared,rows", [(3, 1), (3, 6), (0, 1), (40, 13)])
+def test_nan_key_makes_the_rows_that_see_it_nan(dtype, shared, rows):
+    """A NaN score is no masked one: its row is NaN in every dimension, the other KV
+    head's rows and the other requests' are not; a shared key reaches all requests."""
+    for at in ["own"] + ["shared"] * (shared > 0):
+        c = Case([(shared, [(9, chain(rows)), (6, chain(1))])], dtype=dtype, seed=8)
+        page = c.tables[0][shared if at == "own" else shared - 1]
+        c.kv[page, 0, 2, 1, 5] = float("nan")
+        out = K.tree_attention_shared(**c.device()).float()
+        g = c.Hq // c.Hkv
+        assert torch.isnan(out[:rows, g:2 * g]).all() and torch.isfinite(out[:, :g]).all()
+        assert (torch.isnan if at == "shared" else torch.isfinite)(out[rows:, g:2 * g]).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_large_scores(dtype):
     """Scores far apart and rising along the cache: the running maximum moves often."""
     c = Case([(40, [(50, chain(1)), (70, tree(1, 3, 3))])], dtype=dtype, seed=7, k_std=6.0)
