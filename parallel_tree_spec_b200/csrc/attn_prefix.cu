@@ -1410,7 +1410,7 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
     f.own_splits = 1;
     f.max_items = 0;
     f.head = f.entries = f.items = f.parts = f.own_ml = f.own_o = 0;
-    f.bytes = 256;
+    f.bytes = 0;
     return f;
   }
   // own columns: slices for about six CTAs of two warps per SM, each warp with two runs at least

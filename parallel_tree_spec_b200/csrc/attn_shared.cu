@@ -356,7 +356,7 @@ extern "C" int pts_tree_attn_run_shared(const pts_shared_attn_args* args, void* 
   const size_t need = pts_tree_attn_shared_workspace_size(x.batch, x.num_groups, x.total_q, x.max_qo_len, x.max_kv_len,
                                                           x.max_own_len, x.num_qo_heads, x.num_kv_heads, x.head_dim, x.page_len,
                                                           x.elem_bytes);
-  if (!workspace || workspace_bytes < need)
+  if ((!workspace && need) || workspace_bytes < need)
     return set_error(PTS_ERR_CAPACITY, "workspace of %zu bytes (%zu needed)", workspace_bytes, need);
   SharedAttnParams a{};
   a.q = x.q;

@@ -7,7 +7,6 @@ raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -627,8 +626,8 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
         raise ValueError("q must be [T, Hq, D] and kv_layer [max_pages, 2, page_len, Hkv, D] with the same D")
     if kv_layer.get_device() != index:
         raise ValueError("all tensors must be on the same device")
-    B = _cache_ints("qo_indptr", qo_indptr, index).shape[0] - 1
-    G = _cache_ints("shared_pages", shared_pages, index).shape[0]
+    B = _cache_ints("qo_indptr", qo_indptr, index) - 1
+    G = _cache_ints("shared_pages", shared_pages, index)
     _cache_ints("page_indptr", page_indptr, index, B + 1)
     _cache_ints("page_indices", page_indices, index)
     _cache_ints("last_page_len", last_page_len, index, B)
@@ -644,19 +643,18 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like q")
     max_qo, max_kv = int(max_qo_len), min(int(max_kv_len), 2 ** 31 - 1)
-    own = int(max_own_len) if max_own_len is not None else 0
+    own = min(int(max_own_len), max_kv) if max_own_len is not None else 0
     es = 2 if q.dtype is torch.bfloat16 else 4
-    with _on(index):
-        nbytes = _shared_attn_workspace(index, B, G, T, max_qo, max_kv, own, Hq, Hkv, D, pl, es)
-        ws = qo_indptr.new_empty((nbytes + 3) // 4)
-        err = _ERROR_WORDS.get(index)
-        if err is None:
-            err = _error_word(index)
-        _lib.call("pts_tree_attn_run_shared", _lib.pack_shared_attn(
-            q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
-            last_page_len.data_ptr(), bits, group_indptr.data_ptr(), shared_pages.data_ptr(), out.data_ptr(),
-            err.data_ptr() if err is not None else 0, words, G, B, T, max_qo, max_kv, own, Hq, Hkv, D, pl, P, es,
-            sm_scale if sm_scale is not None else D ** -0.5), ws.data_ptr(), nbytes, _raw_stream(index))
+    nbytes = _shared_attn_workspace(index, B, G, T, max_qo, max_kv, own, Hq, Hkv, D, pl, es)
+    ws = qo_indptr.new_empty((nbytes + 3) // 4) if nbytes else None
+    err = _ERROR_WORDS.get(index)
+    if err is None:
+        err = _error_word(index)
+    _call_on(index, "pts_tree_attn_run_shared", _lib.pack_shared_attn(
+        q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
+        last_page_len.data_ptr(), bits, group_indptr.data_ptr(), shared_pages.data_ptr(), out.data_ptr(),
+        err.data_ptr() if err is not None else 0, words, G, B, T, max_qo, max_kv, own, Hq, Hkv, D, pl, P, es,
+        sm_scale if sm_scale is not None else D ** -0.5), ws.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
     if _CHECK_ATTENTION:
         check_attention(q.device)
     return out
@@ -681,9 +679,10 @@ def sharing_pays(max_qo_len: int, batch: int, num_qo_heads: int, num_kv_heads: i
 
 @functools.lru_cache(maxsize=512)
 def _shared_attn_workspace(index: int, *sizes: int) -> int:
-    """pts_tree_attn_shared_workspace_size on device ``index`` (at least 256 bytes, so that
-    sizes it refuses reach the launch's own checks)."""
-    return max(_lib.lib().pts_tree_attn_shared_workspace_size(*sizes), 256)
+    """pts_tree_attn_shared_workspace_size on device ``index`` (0 also for sizes that the
+    launch refuses)."""
+    with torch.cuda.device(index):
+        return _lib.lib().pts_tree_attn_shared_workspace_size(*sizes)
 
 
 _ERROR_WORDS: Dict[int, torch.Tensor] = {}
@@ -892,54 +891,69 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _on(index: int):
-    """Device ``index`` as the current one (a no-op context where it is already)."""
-    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+def _call_on(index: int, *call) -> None:
+    """``_lib.call`` with device ``index`` as the current one."""
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(*call)
+    else:
+        with torch.cuda.device(index):
+            _lib.call(*call)
 
 
-_HERE = contextlib.nullcontext()
+_INT32 = torch.int32
 
 
-def _cache_ints(name: str, t: torch.Tensor, index: int, size: Optional[int] = None) -> torch.Tensor:
-    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+# (the checks below cost as much as a launch in the small calls that they guard: each
+# attribute of a tensor is asked for once)
+def _cache_ints(name: str, t: torch.Tensor, index: int, size: Optional[int] = None) -> int:
+    """Checks a list of integers; returns its length."""
+    n = t.numel()
+    if t.dtype is not _INT32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
     if t.get_device() != index:
         raise ValueError("all tensors must be on the same device")
-    if size is not None and t.numel() != size:
-        raise ValueError(f"{name} has {t.numel()} entries, expected {size}")
-    return t
+    if size is not None and n != size:
+        raise ValueError(f"{name} has {n} entries, expected {size}")
+    return n
 
 
-def _page_state(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: Optional[torch.Tensor]) -> int:
+def _page_state(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: Optional[torch.Tensor]):
+    """Checks the state; returns (device, pages, rows, width, row stride)."""
     index = page_refs.get_device()
     if index < 0:
         raise ValueError("tensors must be on a CUDA device (this path has no CPU implementation)")
-    _cache_ints("page_refs", page_refs, index)
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 or \
-            page_table.stride(0) < page_table.shape[1]:
+    P = _cache_ints("page_refs", page_refs, index)
+    if page_table.dtype is not _INT32 or page_table.dim() != 2:
+        raise ValueError("page_table must be a 2-D int32 tensor with contiguous rows")
+    (R, W), (stride, one) = page_table.shape, page_table.stride()
+    if one != 1 or stride < W:
         raise ValueError("page_table must be a 2-D int32 tensor with contiguous rows")
     if page_table.get_device() != index:
         raise ValueError("all tensors must be on the same device")
     if kv_lens is not None:
-        _cache_ints("kv_lens", kv_lens, index, page_table.shape[0])
-    return index
+        _cache_ints("kv_lens", kv_lens, index, R)
+    return index, P, R, W, stride
 
 
-def _page_pool(pool: torch.Tensor, page_refs: torch.Tensor):
-    if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous():
+def _page_pool(pool: torch.Tensor, index: int, pages: int):
+    """Checks the pool; returns (layers, page length, bytes of a token)."""
+    if pool.dim() != 6 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous [L, max_pages, 2, page_len, Hkv, D] tensor")
-    if pool.get_device() != page_refs.get_device():
+    L, P, two, pl, H, D = pool.shape
+    if two != 2:
+        raise ValueError("pool must be a contiguous [L, max_pages, 2, page_len, Hkv, D] tensor")
+    if pool.get_device() != index:
         raise ValueError("all tensors must be on the same device")
-    L, P, _, pl, H, D = pool.shape
-    if P != page_refs.shape[0]:
+    if P != pages:
         raise ValueError("page_refs needs one count per page of the pool")
-    return L, P, pl, H * D * pool.element_size()
+    return L, pl, H * D * pool.element_size()
 
 
-def _status_word(status: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+def _status_word(status: Optional[torch.Tensor], like: torch.Tensor, index: int) -> torch.Tensor:
     if status is None:
         return like.new_empty(1)
-    return _cache_ints("status", status, like.get_device(), 1)
+    _cache_ints("status", status, index, 1)
+    return status
 
 
 def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, src_rows: torch.Tensor,
@@ -951,17 +965,14 @@ def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch
     partial page when one of its holders grows.  ``page_refs`` [P], ``page_table``
     [R, W] (-1 past a sequence's end) and ``kv_lens`` [R] are int32 and updated in
     place.  Returns the status word (``check_cache_status``)."""
-    index = _page_state(page_refs, page_table, kv_lens)
-    n = _cache_ints("src_rows", src_rows, index).shape[0]
+    index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("src_rows", src_rows, index)
     _cache_ints("dst_rows", dst_rows, index, n)
-    status = _status_word(status, page_refs)
+    status = _status_word(status, page_refs, index)
     if n == 0:
         return status.zero_()
-    R, W = page_table.shape
-    with _on(index):
-        _lib.call("pts_cache_fork", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                  kv_lens.data_ptr(), R, W, page_refs.shape[0], src_rows.data_ptr(), dst_rows.data_ptr(), n,
-                  status.data_ptr(), _raw_stream(index))
+    _call_on(index, "pts_cache_fork", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(), R, W, P,
+             src_rows.data_ptr(), dst_rows.data_ptr(), n, status.data_ptr(), _raw_stream(index))
     return status
 
 
@@ -976,43 +987,44 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     last_page_len [B], seq_lens [B], shared_pages [G] or None) to write into; entries of
     page_indices past page_indptr[B] are left as they are.  A call that cannot be done
     (see the status) changes nothing and returns a batch of empty sequences."""
-    index = _page_state(page_refs, page_table, kv_lens)
-    L, P, pl, row_bytes = _page_pool(pool, page_refs)
-    B, (R, W) = _cache_ints("rows", rows, index).shape[0], page_table.shape
+    index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
+    L, pl, row_bytes = _page_pool(pool, index, P)
+    B = _cache_ints("rows", rows, index)
     if B == 0:
         raise ValueError("rows is empty")
     each, add_all = 0, 0
     if isinstance(add, torch.Tensor):
-        each = _cache_ints("add", add, index, B).data_ptr()
+        _cache_ints("add", add, index, B)
+        each = add.data_ptr()
     else:
         add_all = int(add)
         if not 0 <= add_all < 2 ** 31:
             raise ValueError(f"add {add_all} is negative or too large")
     G = 0
     if group_indptr is not None:
-        G = _cache_ints("group_indptr", group_indptr, index).shape[0] - 1
+        G = _cache_ints("group_indptr", group_indptr, index) - 1
         if G < 1:
             raise ValueError("group_indptr needs at least two entries")
     if out is None:
         e = page_refs.new_empty
-        indptr, indices, last, lens, shared = e(B + 1), e(B * W), e(B), e(B), e(G) if G else None
+        entries = B * W
+        indptr, indices, last, lens, shared = e(B + 1), e(entries), e(B), e(B), e(G) if G else None
     else:
         indptr, indices, last, lens, shared = out[:5]
         _cache_ints("page_indptr", indptr, index, B + 1)
-        _cache_ints("page_indices", indices, index)
+        entries = _cache_ints("page_indices", indices, index)
         _cache_ints("last_page_len", last, index, B)
         _cache_ints("seq_lens", lens, index, B)
         if G:
             _cache_ints("shared_pages", shared, index, G)
-    status = _status_word(status, page_refs)
+    status = _status_word(status, page_refs, index)
     words = 2 * P + 3 * B + 4                                # pts_cache_workspace_size
     ws = page_refs.new_empty(words)
-    with _on(index):
-        _lib.call("pts_cache_extend", _lib.pack_cache_extend(
-            pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-            kv_lens.data_ptr(), rows.data_ptr(), each, group_indptr.data_ptr() if G else 0, indptr.data_ptr(),
-            indices.data_ptr(), indices.numel(), last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else 0,
-            status.data_ptr(), L, P, pl, R, W, add_all, B, G), ws.data_ptr(), 4 * words, _raw_stream(index))
+    _call_on(index, "pts_cache_extend", _lib.pack_cache_extend(
+        pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(),
+        rows.data_ptr(), each, group_indptr.data_ptr() if G else 0, indptr.data_ptr(), indices.data_ptr(), entries,
+        last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else 0, status.data_ptr(), L, P, pl, R, W, add_all, B,
+        G), ws.data_ptr(), 4 * words, _raw_stream(index))
     return CacheBatch(indptr, indices, last, lens, shared, status)
 
 
@@ -1022,18 +1034,16 @@ def cache_truncate(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: t
     """Cut the listed sequences to ``new_lens`` tokens (int32 [n]; None frees them):
     pages past the new length lose this holder.  A sequence already shorter keeps its
     length.  Returns the status word; rows outside the table are skipped."""
-    index = _page_state(page_refs, page_table, kv_lens)
-    n = _cache_ints("rows", rows, index).shape[0]
+    index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
+    n = _cache_ints("rows", rows, index)
     if new_lens is not None:
         _cache_ints("new_lens", new_lens, index, n)
-    status = _status_word(status, page_refs)
+    status = _status_word(status, page_refs, index)
     if n == 0:
         return status.zero_()
-    R, W = page_table.shape
-    with _on(index):
-        _lib.call("pts_cache_truncate", page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                  kv_lens.data_ptr(), R, W, page_refs.shape[0], int(page_len), rows.data_ptr(),
-                  new_lens.data_ptr() if new_lens is not None else None, n, status.data_ptr(), _raw_stream(index))
+    _call_on(index, "pts_cache_truncate", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(), R, W,
+             P, int(page_len), rows.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, n,
+             status.data_ptr(), _raw_stream(index))
     return status
 
 
@@ -1041,16 +1051,14 @@ def cache_compact(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch
     """Close the gaps of ``pool``: its n live pages end up in pages 0 .. n-1, moving
     only those at or past n.  Returns the new counts and table (the inputs keep their
     values), the page map and the counts."""
-    index = _page_state(page_refs, page_table, None)
-    L, P, pl, row_bytes = _page_pool(pool, page_refs)
-    R, W = page_table.shape
+    index, P, R, W, stride = _page_state(page_refs, page_table, None)
+    L, pl, row_bytes = _page_pool(pool, index, P)
     refs, table, page_map, counts = (page_refs.new_empty(P), page_table.new_empty(R, W), page_refs.new_empty(P),
                                      page_refs.new_empty(2))
     words = 2 * P + 4                                        # pts_cache_workspace_size
     ws = page_refs.new_empty(words)
-    with _on(index):
-        _lib.call("pts_cache_compact", _lib.pack_cache_compact(
-            pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-            refs.data_ptr(), table.data_ptr(), page_map.data_ptr(), counts.data_ptr(), L, P, pl, R, W), ws.data_ptr(),
-            4 * words, _raw_stream(index))
+    _call_on(index, "pts_cache_compact", _lib.pack_cache_compact(
+        pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), stride, refs.data_ptr(),
+        table.data_ptr(), page_map.data_ptr(), counts.data_ptr(), L, P, pl, R, W), ws.data_ptr(), 4 * words,
+        _raw_stream(index))
     return CompactedCache(refs, table, page_map, counts)

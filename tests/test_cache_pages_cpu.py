@@ -130,3 +130,11 @@ def test_oracle_counts_holders():
     (65, 16, 32, 8, 128, 16, torch.float32, True), (65, 64, 64, 2, 128, 16, torch.bfloat16, True)])
 def test_sharing_pays(rows, batch, Hq, Hkv, D, page, dtype, pays):
     assert K.sharing_pays(rows, batch, Hq, Hkv, D, page, dtype) is pays
+
+
+def test_small_calls_need_no_workspace():
+    size = _lib.lib().pts_tree_attn_shared_workspace_size
+    assert size(6, 1, 6, 1, 600, 0, 32, 8, 64, 16, 2) == 0
+    assert size(64, 1, 64, 1, 9000, 300, 32, 8, 128, 16, 2) > 0
+    assert size(6, 1, 6, 1, 600, 0, 32, 8, 64, 16, 4) > 0      # fp32
+    assert size(0, 1, 6, 1, 600, 0, 32, 8, 64, 16, 2) == 0     # refused by the call
