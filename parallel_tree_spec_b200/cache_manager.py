@@ -25,6 +25,7 @@ several samples of one prompt, beams, requests under one system prompt.
 from __future__ import annotations
 
 import math
+from itertools import accumulate
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
@@ -209,8 +210,9 @@ class SharedKvCache:
     batch position for the append and the attention, with each group's common pages;
     ``truncate`` and ``release`` give pages back; ``compact`` closes the pool's gaps.  Rows
     (sequence numbers) and lengths may be lists or int32 tensors on the pool's device;
-    tensors keep every call free of host copies and synchronisations, so a step can be
-    captured in a CUDA graph (not ``compact``, which replaces the state's tensors).  A
+    with tensors (and one int for all rows in ``extend``) no call copies from the host or
+    waits for it, so a step can be captured in a CUDA graph (not ``compact``, which
+    replaces the state's tensors).  A
     call that cannot be done changes nothing (the batch position of such an ``extend`` has
     empty sequences, so an append to it writes nothing); ``check`` raises for it.  The
     cache takes all pages of the pool, which must be free, until ``close``."""
@@ -263,17 +265,19 @@ class SharedKvCache:
         adds = [int(add)] * B if isinstance(add, int) else [int(n) for n in add]
         if len(adds) != B:
             raise ValueError(f"add has {len(adds)} entries, expected {B}")
+        if not adds or min(adds) < 0:
+            raise ValueError("add is empty or negative")
         dev = self.page_refs.device
-        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
-        gi = i32([0, B]) if groups is None else self._ints(groups)
-        out = K.cache_extend(self.pool.cache_data, self.page_refs, self.page_table, self.kv_lens, r,
-                             adds[0] if len(set(adds)) == 1 else i32(adds), group_indptr=gi)
+        up_to = lambda n: torch.arange(n, dtype=torch.int32, device=dev)    # (made there: nothing is copied)
+        if min(adds) == max(adds):
+            each, seq = adds[0], up_to(B + 1) * adds[0]
+        else:
+            each, seq = self._ints(adds), self._ints(accumulate(adds, initial=0))
+        gi = up_to(2) * B if groups is None else self._ints(groups)
+        out = K.cache_extend(self.pool.cache_data, self.page_refs, self.page_table, self.kv_lens, r, each, group_indptr=gi)
         self._note(out.status)
-        seq = [0]
-        for n in adds:
-            seq.append(seq[-1] + n)
-        bp = KvCacheBatchPosition(i32(seq), out.page_indptr, out.page_indices, out.last_page_len, None, None)
-        bp.batch_indices, bp.positions = K.batch_positions(bp.seq_indptr, out.seq_lens, seq[-1])
+        bp = KvCacheBatchPosition(seq, out.page_indptr, out.page_indices, out.last_page_len, None, None)
+        bp.batch_indices, bp.positions = K.batch_positions(seq, out.seq_lens, sum(adds)) if any(adds) else (up_to(0), up_to(0))
         if isinstance(rows, torch.Tensor):
             top = max(self._bound) + max(adds)
             self._bound = [min(top, self._limit())] * len(self._bound)

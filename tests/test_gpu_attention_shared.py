@@ -298,6 +298,30 @@ def test_long_prefix_and_long_own(dtype):
     check(Case([(520, [(int(x), chain(1)) for x in (3000, 10, 700)])], Hq=4, Hkv=1, D=128, dtype=dtype, seed=12))
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("rows", [1, 9])
+@pytest.mark.parametrize("bounds", [dict(max_kv_len=1), dict(max_kv_len=1 << 30), dict(max_kv_len=2 ** 40, max_own_len=1),
+                                    dict(max_own_len=0), dict(max_own_len=1 << 40)])
+def test_wrong_length_bounds_change_only_the_schedule(dtype, rows, bounds):
+    check(Case([(60, [(200, chain(rows)), (3, chain(1))] * 5), (0, [(90, chain(rows))])], dtype=dtype, seed=14), **bounds)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("D", [64, 128])
+def test_group_ranges_and_last_pages_are_cut(dtype, D):
+    """Group ends past the batch, and a last page said to hold more than a page: as if they
+    named the batch and the whole page."""
+    c = Case([(30, [(11, chain(n)), (25, chain(n))]) for n in (1, 7)], D=D, dtype=dtype, seed=15)
+    a = c.device()
+    B = a["last_page_len"].numel()
+    groups = a["group_indptr"].clone()
+    groups[-1] = B + 1000
+    check(c, group_indptr=groups)
+    full = a["last_page_len"].clone().fill_(c.pl)
+    want = K.tree_attention_shared(**dict(a, last_page_len=full))
+    assert torch.equal(K.tree_attention_shared(**dict(a, last_page_len=full + 1000)), want)
+
+
 def test_repeat_is_the_same():
     c = Case([(200, [(50, chain(1))] * 40)], Hq=32, Hkv=8, seed=13)
     a = c.device()

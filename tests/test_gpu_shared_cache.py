@@ -309,3 +309,72 @@ def test_a_failed_extend_leaves_the_cache_to_later_calls_of_the_step():
     with pytest.raises(RuntimeError):
         cache.check()
     assert cache.kv_lens.tolist() == [14, 14, 14]
+
+
+def test_a_step_of_the_cache_is_captured():
+    """The class's own calls with tensors, and the wrapper's: fork, extend, attention and
+    truncation captured once, each replay on the prompt as it then is."""
+    Hq, Hkv, D, page, n = 8, 2, 64, 16, 3
+    pool = KvCachePool(40, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, 4, 8)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    gen = torch.Generator().manual_seed(2)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    hist = torch.empty(0, 2, Hkv, D, dtype=torch.bfloat16, device=DEV)
+
+    def prompt(m):
+        nonlocal hist
+        bp = cache.extend([0], m)
+        k, v = rnd(m, Hkv, D), rnd(m, Hkv, D)
+        w.append_kv_cache(None, k, v, bp, pool.cache_data[0], page)
+        hist = torch.cat([hist, torch.stack([k, v], 1)])
+
+    src, dst, none, parents = i32([0] * 3), i32([1, 2, 3]), i32([0] * 3), i32(chain(n) * 3)
+    q, k, v = rnd(3 * n, Hq, D), rnd(3 * n, Hkv, D), rnd(3 * n, Hkv, D)
+    out = torch.empty(3 * n, Hq * D, dtype=torch.bfloat16, device=DEV)
+
+    def body():
+        cache.fork(src, dst)
+        bp = cache.extend(dst, n)
+        w.set_tree_masks(parents, bp, n)
+        out.copy_(w.computeAttention(q, k, v, pool.cache_data[0], "tree", bp, AttentionRotaryParams(), 0))
+        cache.truncate(dst, none)
+
+    prompt(21)
+    body()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        body()
+    for m in (0, 30, 1):
+        if m:
+            prompt(m)
+        for x in (q, k, v):
+            x.copy_(rnd(*x.shape))
+        g.replay()
+        for i in range(3):
+            kv = torch.cat([hist, torch.stack([k[i * n:(i + 1) * n], v[i * n:(i + 1) * n]], 1)])
+            mask = torch.ones(n, kv.shape[0], dtype=torch.bool, device=DEV).tril(kv.shape[0] - n)
+            o, A = dense(q[i * n:(i + 1) * n], kv, mask)
+            bad = (out.view(-1, Hq, D)[i * n:(i + 1) * n].double() - o).abs() / ((2 ** -7 + 2.0 ** -12) * A + 2 ** -8 * o.abs())
+            assert bad.max().item() <= 1.0
+        assert cache.kv_lens.tolist()[1:] == [0, 0, 0]
+    cache.check()
+
+
+def test_extend_by_nothing_lists_the_pages():
+    pool = KvCachePool(8, 1, 1, 64, 4, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, 2, 4)
+    cache.extend([0], 6)
+    cache.fork([0], [1])
+    bp = cache.extend([0, 1], 0)
+    assert bp.kv_page_indices[:4].tolist() == [0, 1, 0, 1] and bp.shared_pages.tolist() == [1]
+    assert bp.batch_indices.numel() == bp.positions.numel() == 0 and bp.seq_indptr.tolist() == [0, 0, 0]
+    for bad in (-1, [1, -1], [1], []):
+        with pytest.raises(ValueError):
+            cache.extend([0, 1], bad)
+    with pytest.raises(ValueError):
+        cache.extend([], 1)
+    cache.check()
+    assert cache.lengths() == [6, 6]
