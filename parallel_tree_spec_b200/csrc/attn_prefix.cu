@@ -14,13 +14,13 @@
 //   rows and every second block.  tcgen05 with S and O in TMEM, P written back over S as
 //   the A operand of the value product; K/V by TMA into a ring; one thread per row, so
 //   the softmax needs no shuffles.  Each item leaves one part per row (fp32 O, m, l).
-// own_attn_kernel, when requests have at most 16 query rows per KV head (decoding): their
-//   own columns.  So few rows fill an eighth of a 128-row tensor-core tile at most, and
-//   the K/V bytes serve those rows only, so HBM is the bound and mma.sync m16n8k16 on
-//   transposed products, fed by TMA through a small ring per warp, is enough.  It is
-//   launched to run beside the second kernel, which is bound by its arithmetic: a CTA of
-//   two warps fits an SM next to that kernel's CTA (its ring and its registers are kept
-//   that small).
+// own_attn_kernel, when requests have at most 16 query rows per KV head (decoding) or at
+//   most 16 more than whole tiles: those rows' own columns.  So few rows fill an eighth of
+//   a 128-row tensor-core tile at most, and the K/V bytes serve those rows only, so HBM is
+//   the bound and mma.sync m16n8k16 on transposed products, fed by TMA through a small ring
+//   per warp, is enough.  It is launched to run beside the second kernel, which is bound by
+//   its arithmetic: a CTA of two warps fits an SM next to that kernel's CTA (its ring and
+//   its registers are kept that small).
 // join_parts_kernel: joins every row's parts and writes the output (join_tiles_kernel where
 //   the own columns are work items).
 //
@@ -125,16 +125,24 @@ struct PrefixParams {
   // plan
   int ctas;                 // of prefix_attn_kernel
   int max_items;            // parts in the workspace
-  int own_items;            // own columns are work items
+  int own_items;            // own columns are work items, but for
+  int tail_rows;            // up to so many rows behind a request's last whole tile
   PlanHead* head;
   Entry* entries;
   Item* items;
   float* parts;
   // own columns in own_attn_kernel
   int own_splits;           // slices of a request's columns
-  float* own_o;             // [T * Hq][own_splits][D]
-  float2* own_ml;           // [T * Hq][own_splits]
+  float* own_o;             // [T * Hq][own_splits][D]; tails: [batch * Hkv * kFewRows][own_splits][D]
+  float2* own_ml;           // the same without D
 
+  // Where a request's rows per KV head that own_attn_kernel takes begin (all of them, where own
+  // columns are no work items); rows: none.
+  __device__ __forceinline__ int tail_from(int rows) const {
+    if (!own_items) return 0;
+    const int from = rows / kTileRows * kTileRows;
+    return rows - from <= tail_rows ? from : rows;
+  }
   __device__ __forceinline__ int page_of(int tok) const { return page_shift >= 0 ? tok >> page_shift : tok / a.page_len; }
 };
 
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
     for (int b = tid; b < a.batch; b += threads) {
       const int tok0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - tok0, pages = entry[group_of(a, b)].pages;
       const int len = n > 0 ? max(0, kv_tokens(a, b) - pages * a.page_len) : 0;
-      entry[a.groups + b] = Entry{len, len - n, n * a.g, tok0, a.page_indptr[b] + pages, 0, 0, 0};
+      entry[a.groups + b] = Entry{len, len - n, p.tail_from(n * a.g), tok0, a.page_indptr[b] + pages, 0, 0, 0};
     }
     __syncthreads();
   }
@@ -357,11 +365,12 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
   const bool last = !kDirect && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
   const int b = blockIdx.x, h = blockIdx.y;
   const int tok0 = a.qo_indptr[b], n_tok = a.qo_indptr[b + 1] - tok0, total_rows = n_tok * a.g;
-  if (total_rows <= 0) {
+  const int from = kDirect || total_rows <= 0 ? 0 : p.tail_from(total_rows);
+  if (total_rows <= from) {
     if (last) pdl_wait();
     return;
   }
-  const int rows = min(kRows, total_rows);
+  const int rows = min(kRows, total_rows - from);
   const int shared = kDirect ? 0 : group_shared_pages(a, group_of(a, b));
   const int32_t* table = a.page_indices + a.page_indptr[b] + shared;
   const int len = max(0, kv_tokens(a, b) - shared * a.page_len), prefix = len - n_tok;
@@ -401,10 +410,10 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
   uint32_t qb[NR][D / 16][2];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    const int r = 8 * n + gq, tk = p.div_g.div(r);
+    const int r = 8 * n + gq, R = from + r, tk = p.div_g.div(R);
     const bool valid = r < rows;
     const uint16_t* q =
-        (const uint16_t*)a.q + ((int64_t)(tok0 + (valid ? tk : 0)) * a.Hq + h * a.g + (valid ? r - tk * a.g : 0)) * D + 2 * tq;
+        (const uint16_t*)a.q + ((int64_t)(tok0 + (valid ? tk : 0)) * a.Hq + h * a.g + (valid ? R - tk * a.g : 0)) * D + 2 * tq;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       qb[n][k][0] = valid ? __ldg((const uint32_t*)(q + 16 * k)) : 0u;
@@ -449,7 +458,7 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int r = 8 * n + 2 * tq + j, node = p.div_g.div(r);
+          const int r = 8 * n + 2 * tq + j, node = p.div_g.div(from + r);
           seen[j] = r < rows ? (uint32_t)seen_columns(a, tok0 + node, node, c0, prefix, len) : 0u;
         }
       }
@@ -571,7 +580,7 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
     }
   __syncthreads();
   for (int e = threadIdx.x; e < rows * (D / 4); e += blockDim.x) {
-    const int r = e / (D / 4), quad = e % (D / 4), tk = p.div_g.div(r);
+    const int r = e / (D / 4), quad = e % (D / 4), tk = p.div_g.div(from + r);
     float M = -INFINITY;
     for (int w = 0; w < warps; ++w) M = fmaxf(M, ml[w][r].x);
     const float base = M == -INFINITY ? 0.0f : M;
@@ -586,14 +595,14 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
       acc.z = fmaf(f, v.z, acc.z);
       acc.w = fmaf(f, v.w, acc.w);
     }
-    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + r - tk * a.g;
+    const int64_t row = (int64_t)(tok0 + tk) * a.Hq + h * a.g + from + r - tk * a.g;
     if (kDirect) {
       const float f = L > 0.0f ? 1.0f / L : L == L ? 0.0f : L;    // nothing seen: 0
       *(uint2*)((uint16_t*)a.out + row * D + quad * 4) =
           make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
       continue;
     }
-    const int64_t part = row * p.own_splits + blockIdx.z;
+    const int64_t part = (p.own_items ? ((int64_t)b * a.Hkv + h) * kFewRows + r : row) * p.own_splits + blockIdx.z;
     *(float4*)(p.own_o + part * D + quad * 4) = acc;
     if (quad == 0) p.own_ml[part] = make_float2(M, L);
   }
@@ -627,7 +636,7 @@ __device__ __forceinline__ bool masked_block(const Item& it, int j) {
 // P to TMEM, the two products.  128 tokens of 256 rows of head_dim 128 take 2.2 us (7.6
 // TFLOP/s of an SM; all of them 68 % of the measured matrix rate), of which the products
 // alone are 2048 clocks and the exponentials as many.  An item costs 5-9 us more for its
-// start and its parts.  16 requests of up to 65 nodes with 4096 shared tokens: 77-90 us,
+// start and its parts.  16 requests of up to 65 nodes with 4096 shared tokens: 80-85 us,
 // the matrix pipe 30 % busy over the launch; 32 decoding requests with 65536 shared tokens:
 // the cache at 5.2 TB/s.
 template <int D>
@@ -1337,7 +1346,10 @@ __global__ void __launch_bounds__(kTilesThreads, 8) join_tiles_kernel(const Pref
   pdl_wait();                                           // (the lengths are no kernel's of this call)
   if (row0 >= rows) return;
   const Entry shared = load_entry(p.entries + group), own = load_entry(p.entries + a.groups + b);
-  const int r = min(row0 + (lane & 3), rows - 1), R = r + (tok0 - shared.tok0) * a.g, parts = shared.splits + own.splits;
+  const int r = min(row0 + (lane & 3), rows - 1), R = r + (tok0 - shared.tok0) * a.g, from = p.tail_from(rows);
+  const bool tail = row0 >= from;                       // (whole warps: a tile's rows are a multiple of four)
+  const int parts = shared.splits + (tail ? p.own_splits : own.splits);
+  const int64_t tail_part = (((int64_t)b * a.Hkv + h) * kFewRows + r - from) * p.own_splits;
   auto part_of = [&](const Entry& e, int at) -> const float* {
     return p.parts + ((int64_t)e.first + (int64_t)(h * tiles_of(e.rows) + at / kTileRows) * e.splits) * kPart +
            ((at >> 7) & 1) * kHalf + (at & 127);
@@ -1349,12 +1361,23 @@ __global__ void __launch_bounds__(kTilesThreads, 8) join_tiles_kernel(const Pref
   for (int j = 0; j < kQuads; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
   for (int k = 0; k < parts; ++k) {
-    const float* s = k < shared.splits ? s0 + (int64_t)k * kPart : s1 + (int64_t)(k - shared.splits) * kPart;
-    const int in = (k < shared.splits ? R : r) & 127;
-    const float m = __ldcg(s + 128 * D), l = __ldcg(s + 128 * D + 128);
+    float m, l;
     float4 v[kQuads];
+    if (tail && k >= shared.splits) {
+      const int64_t part = tail_part + (k - shared.splits);
+      const float2 x = __ldcg(p.own_ml + part);
+      m = x.x;
+      l = x.y;
 #pragma unroll
-    for (int j = 0; j < kQuads; ++j) v[j] = __ldcg((const float4*)(s - in + (8 * j + (lane >> 2)) * 512 + in * 4));
+      for (int j = 0; j < kQuads; ++j) v[j] = __ldcg((const float4*)(p.own_o + part * D) + 8 * j + (lane >> 2));
+    } else {
+      const float* s = k < shared.splits ? s0 + (int64_t)k * kPart : s1 + (int64_t)(k - shared.splits) * kPart;
+      const int in = (k < shared.splits ? R : r) & 127;
+      m = __ldcg(s + 128 * D);
+      l = __ldcg(s + 128 * D + 128);
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) v[j] = __ldcg((const float4*)(s - in + (8 * j + (lane >> 2)) * 512 + in * 4));
+    }
     const float top = fmaxf(M, m), base = top == -INFINITY ? 0.0f : top;
     const float f = fast_exp2(M - base), w = fast_exp2(m - base);
     L = f * L + w * l;
@@ -1378,7 +1401,7 @@ __global__ void __launch_bounds__(kTilesThreads, 8) join_tiles_kernel(const Pref
 }
 
 struct PrefixPlan {
-  int few, direct, own_rows, own_splits, max_items, ctas;
+  int few, direct, tail_rows, own_rows, own_splits, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
@@ -1399,6 +1422,12 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   const int g = Hq / Hkv;
   const int64_t rows = (int64_t)max_qo_len * g;
   f.few = rows <= kFewRows;
+  // A tree of a few rows more than whole tiles has a tile for them, which costs a CTA almost
+  // as much as a full one: own_attn_kernel takes them beside it instead (and those of the
+  // other requests).  16 requests of 260 rows per KV head after 4096 shared tokens: 102 us with
+  // it, 114 without; of 516 rows 190 and 195; 4 of 260 rows 52 and 60.  Half tiles do
+  // not gain by it (132 rows: 62 and 61, with 1500 own tokens 113 and 104).
+  f.tail_rows = !f.few && rows % kTileRows && rows % kTileRows <= kFewRows ? kFewRows : 0;
   f.own_rows = rows <= 8 ? 8 : 16;
   f.ctas = sm_count();
   // One launch that reads each request's columns takes about 3 us + 5 ns a token for each
@@ -1416,7 +1445,7 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   // own columns: slices for about six CTAs of two warps per SM, each warp with two runs at least
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
   f.own_splits = 1;
-  if (f.few)
+  if (f.few || f.tail_rows)
     f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({6ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
                                                                 (own + 4 * kRun - 1) / (4 * kRun), kMaxOwnSplits}));
   int64_t units = ((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups;
@@ -1433,7 +1462,7 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   f.entries = take(sizeof(Entry) * (groups + (f.few ? 0 : batch)));
   f.items = take(sizeof(Item) * f.max_items);
   f.parts = take((size_t)f.max_items * part * sizeof(float));
-  const size_t own_parts = f.few ? (size_t)total_q * Hq * f.own_splits : 0;
+  const size_t own_parts = (f.few ? (size_t)total_q * Hq : f.tail_rows ? (size_t)batch * Hkv * kFewRows : 0) * f.own_splits;
   f.own_ml = take(own_parts * sizeof(float2));
   f.own_o = take(own_parts * D * sizeof(float));
   f.bytes = at;
@@ -1462,7 +1491,7 @@ int launch_own(const PrefixParams& p, const CUtensorMap& map, cudaStream_t strea
 template <int D>
 int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cudaStream_t stream) {
   CUtensorMap run_map, block_map;
-  if (f.few)
+  if (f.few || f.tail_rows)
     if (int rc = encode_kv<D>(&run_map, p.a, kRun)) return rc;
   if (f.direct)
     return f.own_rows == 8 ? launch_own<D, 1, kDirectWarps, true>(p, run_map, stream)
@@ -1486,7 +1515,7 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
     return set_error(PTS_ERR_CUDA, "prefix_attn_kernel was built with %d registers (%d needed)", regs.load(), kLaunchRegs);
   PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
   if (int rc = launch_status("prefix_attn_kernel")) return rc;
-  if (f.few)
+  if (f.few || f.tail_rows)
     if (int rc = f.own_rows == 8 ? launch_own<D, 1, kOwnWarps, false>(p, run_map, stream)
                                  : launch_own<D, 2, kOwnWarps, false>(p, run_map, stream))
       return rc;
@@ -1530,6 +1559,7 @@ int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, i
   p.ctas = f.ctas;
   p.max_items = f.max_items;
   p.own_items = !f.few;
+  p.tail_rows = f.tail_rows;
   p.head = (PlanHead*)(ws + f.head);
   p.entries = (Entry*)(ws + f.entries);
   p.items = (Item*)(ws + f.items);
