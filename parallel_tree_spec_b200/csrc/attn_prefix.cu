@@ -50,8 +50,8 @@ constexpr int kMaxSplits = 32;            // block ranges of a column set
 constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in own_attn_kernel
 constexpr int kDirectCost = 3600;          // in tokens' time: the rounds' 3 us count 600 each
 // Rows per KV head up to which own_attn_kernel takes the own columns: 64 requests of 8192
-// shared and 300 own tokens take, with it and with work items, 46 and 63 us at 4 rows, 55
-// and 76 at 8, 73 and 84 at 12, 97 and 93 at 16 (114 and 120 with 2048 and 1500 tokens).
+// shared and 300 own tokens take, with it and with work items, 42 and 63 us at 4 rows, 55
+// and 76 at 8, 74 and 84 at 12, 92 and 93 at 16 (112 and 120 with 2048 and 1500 tokens).
 constexpr int kFewRows = 16;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -59,14 +59,15 @@ constexpr uint32_t kColS = 0, kColO = 256;
 // K (or V) in shared memory: [8-token group][64-dim half][8 tokens][64 dims],
 // 128-byte-swizzled rows.  One TMA copy brings a page's tokens (up to a block) with both
 // halves, and the groups of a half lie evenly apart, as the matrix descriptors want.
-template <int D>
+// SLOTS: of the ring, each K or V of a block.
+template <int D, int SLOTS = D == 128 ? 4 : 6>
 struct Shape {
   static constexpr int kHalves = D / 64;
   static constexpr uint32_t kGroupBytes = kHalves * 1024;
   static constexpr uint32_t kRunBytes = 2 * kGroupBytes;
   static constexpr uint32_t kSlotBytes = kRuns * kRunBytes;     // K or V of a block; Q of a stream
   static constexpr uint32_t kQHalfBytes = 128 * 128;            // Q: [half][128 rows][64 dims]
-  static constexpr int kSlots = D == 128 ? 4 : 6;
+  static constexpr int kSlots = SLOTS;
   static constexpr uint32_t kOffQ = 0;
   static constexpr uint32_t kOffRing = 2 * kSlotBytes;
   static constexpr uint32_t kOffBars = kOffRing + kSlots * kSlotBytes;
@@ -335,8 +336,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
 // in use, and the 8 columns are query rows: half the products of the plain form at 8
 // rows or fewer.
 // 64 requests with 225 own tokens on average, 8 KV heads of 128 (59 MB): 19 us by itself,
-// 3.1 TB/s -- a pair's 14 runs are over before the ring has paid for its start -- and 35 us
-// beside prefix_attn_kernel, whose 25 us it hides.
+// 3.1 TB/s -- a pair's 14 runs are over before the ring has paid for its start -- and, two
+// CTAs beside prefix_attn_kernel's on an SM, about as long as that kernel (one: 35 us
+// beside its 25).
 // kDirect: all columns, the shared ones too, and the output itself: for small calls, where
 // reading a short prefix once per request costs less than the plan and the join.
 template <int D, int NR, int NW, bool kDirect>
@@ -616,9 +618,12 @@ constexpr size_t own_smem() {
   static_assert(ring >= o, "the rings hold the warps' O, m and l");
   return NW * (ring + 8 * kOwnStages);
 }
-// with prefix_attn_kernel's CTA beside it (in whole KB, and one more that the system takes
-// for each)
-static_assert((own_smem<128, 2, kOwnWarps>() + 1023) / 1024 + (Shape<128>::kSmem + 1023) / 1024 + 2 <= 228, "both fit an SM");
+// with prefix_attn_kernel's CTA beside it, and two with the narrow one (each in 128 bytes
+// and 1 KB more that the system takes)
+constexpr size_t sm_share(size_t smem) { return (smem + 127) / 128 * 128 + 1024; }
+static_assert(sm_share(own_smem<128, 2, kOwnWarps>()) + sm_share(Shape<128>::kSmem) <= 228 * 1024 &&
+                  2 * sm_share(own_smem<128, 2, kOwnWarps>()) + sm_share(Shape<128, 3>::kSmem) <= 228 * 1024,
+              "they fit an SM");
 
 // ------------------------------------------------------------------- work items
 // Ring positions of block i's K and V among n blocks, in load order.  Two row tiles use
@@ -639,10 +644,10 @@ __device__ __forceinline__ bool masked_block(const Item& it, int j) {
 // start and its parts.  16 requests of up to 65 nodes with 4096 shared tokens: 80-85 us,
 // the matrix pipe 30 % busy over the launch; 32 decoding requests with 65536 shared tokens:
 // the cache at 5.2 TB/s.
-template <int D>
+template <int D, int SLOTS>
 __global__ void __launch_bounds__(kBoundThreads, 1)
     prefix_attn_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap kv_map) {
-  using S = Shape<D>;
+  using S = Shape<D, SLOTS>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars& bars = *reinterpret_cast<Bars*>(smem + S::kOffBars);
   const SharedAttnParams& a = p.a;
@@ -1401,7 +1406,7 @@ __global__ void __launch_bounds__(kTilesThreads, 8) join_tiles_kernel(const Pref
 }
 
 struct PrefixPlan {
-  int few, direct, tail_rows, own_rows, own_splits, max_items, ctas;
+  int few, direct, narrow, tail_rows, own_rows, own_splits, max_items, ctas;
   size_t head, entries, items, parts, own_ml, own_o, bytes;
 };
 
@@ -1444,6 +1449,10 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   }
   // own columns: slices for about six CTAs of two warps per SM, each warp with two runs at least
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
+  // Decoding with more own columns than shared ones: prefix_attn_kernel gives a slot of its ring
+  // to a second own_attn_kernel CTA beside it.  64 requests of 8192 shared and 300 own tokens
+  // 41.9 us with it, 45.5 without; 32 of 65536 and 500 85.9 and 77.7.
+  f.narrow = f.few && max_own_len > 0 && (int64_t)batch * max_own_len >= (int64_t)groups * (max_kv_len - max_own_len);
   f.own_splits = 1;
   if (f.few || f.tail_rows)
     f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({6ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
@@ -1488,6 +1497,24 @@ int launch_own(const PrefixParams& p, const CUtensorMap& map, cudaStream_t strea
   return launch_status("own_attn_kernel");
 }
 
+template <int D, int SLOTS>
+int launch_items(const PrefixParams& p, const PrefixPlan& f, const CUtensorMap& map, cudaStream_t stream) {
+  auto kernel = prefix_attn_kernel<D, SLOTS>;
+  constexpr size_t smem = Shape<D, SLOTS>::kSmem;
+  if (int rc = ensure_smem_attr((const void*)kernel, smem, true)) return rc;
+  // setmaxnreg.inc would wait for good for registers that the launch does not have
+  static std::atomic<int> regs{0};
+  if (!regs.load()) {
+    cudaFuncAttributes attr;
+    PTS_CUDA_TRY(cudaFuncGetAttributes(&attr, (const void*)kernel));
+    regs.store(attr.numRegs);
+  }
+  if (regs.load() < kLaunchRegs)
+    return set_error(PTS_ERR_CUDA, "prefix_attn_kernel was built with %d registers (%d needed)", regs.load(), kLaunchRegs);
+  PTS_CUDA_TRY(launch_pdl(kernel, dim3(f.ctas), dim3(kThreads), smem, stream, p, map));
+  return launch_status("prefix_attn_kernel");
+}
+
 template <int D>
 int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cudaStream_t stream) {
   CUtensorMap run_map, block_map;
@@ -1503,18 +1530,11 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
     return rc;
   PTS_CUDA_TRY(launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p));
   if (int rc = launch_status("plan_kernel")) return rc;
-  if (int rc = ensure_smem_attr((const void*)prefix_attn_kernel<D>, Shape<D>::kSmem, true)) return rc;
-  // setmaxnreg.inc would wait for good for registers that the launch does not have
-  static std::atomic<int> regs{0};
-  if (!regs.load()) {
-    cudaFuncAttributes attr;
-    PTS_CUDA_TRY(cudaFuncGetAttributes(&attr, (const void*)prefix_attn_kernel<D>));
-    regs.store(attr.numRegs);
+  if (D == 128 && f.narrow) {
+    if (int rc = launch_items<D, 3>(p, f, block_map, stream)) return rc;
+  } else if (int rc = launch_items<D, Shape<D>::kSlots>(p, f, block_map, stream)) {
+    return rc;
   }
-  if (regs.load() < kLaunchRegs)
-    return set_error(PTS_ERR_CUDA, "prefix_attn_kernel was built with %d registers (%d needed)", regs.load(), kLaunchRegs);
-  PTS_CUDA_TRY(launch_pdl(prefix_attn_kernel<D>, dim3(f.ctas), dim3(kThreads), Shape<D>::kSmem, stream, p, block_map));
-  if (int rc = launch_status("prefix_attn_kernel")) return rc;
   if (f.few || f.tail_rows)
     if (int rc = f.own_rows == 8 ? launch_own<D, 1, kOwnWarps, false>(p, run_map, stream)
                                  : launch_own<D, 2, kOwnWarps, false>(p, run_map, stream))
