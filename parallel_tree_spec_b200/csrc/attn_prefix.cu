@@ -642,7 +642,7 @@ __device__ __forceinline__ bool masked_block(const Item& it, int j) {
 // TFLOP/s of an SM; all of them 68 % of the measured matrix rate), of which the products
 // alone are 2048 clocks and the exponentials as many.  An item costs 5-9 us more for its
 // start and its parts.  16 requests of up to 65 nodes with 4096 shared tokens: 80-85 us,
-// the matrix pipe 30 % busy over the launch; 32 decoding requests with 65536 shared tokens:
+// the matrix pipe 35 % busy over the launch; 32 decoding requests with 65536 shared tokens:
 // the cache at 5.2 TB/s.
 template <int D, int SLOTS>
 __global__ void __launch_bounds__(kBoundThreads, 1)
