@@ -199,10 +199,14 @@ constexpr int kOwnWarps = 2, kDirectWarps = 8;
 constexpr int kOwnStages = 2;
 constexpr int kPlanCache = 512;           // entries that the plan keeps in shared memory
 
-// The plan.  With c blocks per range an item costs about c + 1.5 block times (its start
-// and end cost about one and a half), and the launch about the larger of the total over
-// the CTAs and the large items' rounds; the cheapest of up to 32 ranges of
-// ceil(longest / k) blocks is taken.  Bound by the chain of its loads and barriers: 4-6 us,
+// What an item costs besides its blocks, in half block times: its start and the storing of
+// its part, some three blocks, and the part's share of the join.  Over 34 mixed calls (10 to
+// 400 us) the geometric mean was, with 3, 9, 12, 16, 20 and 28: 53.6, 51.9, 51.5, 51.4, 51.4
+// and 52.0 us (others: 46.4, 45.3, 45.1, 45.0, 45.0, 45.3), single calls up to a third less.
+constexpr int kItemCost = 16;
+
+// The plan.  The launch costs about the larger of all items over the CTAs and of the large
+// items' rounds; the cheapest of up to 32 ranges of ceil(longest / k) blocks is taken.  Bound by the chain of its loads and barriers: 4-6 us,
 // 7-8 from a cold cache, for 64 requests as for 16.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p) {
   __shared__ int sums[64 + 4];                          // [2][32] items, large items; red
@@ -272,8 +276,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p
     const int c = ceil_div(longest, lane + 1), items = sums[lane], large = sums[32 + lane];
     unsigned cost = 0xffffffffu;
     if (lane == 0 || (lane < longest && items <= p.max_items))
-      cost = (unsigned)max(small_div(min(2 * blocks + 3 * items, (1 << 24) - 1), p.ctas),
-                           small_div(min(large, 1 << 20) + p.ctas - 1, p.ctas) * (2 * c + 3));
+      cost = (unsigned)max(small_div(min(2 * blocks + kItemCost * items, (1 << 24) - 1), p.ctas),
+                           small_div(min(large, 1 << 20) + p.ctas - 1, p.ctas) * (2 * c + kItemCost));
     const unsigned win = __reduce_min_sync(0xffffffffu, cost);
     const int chunk = __reduce_max_sync(0xffffffffu, cost == win ? c : 0);   // equal costs: fewer parts
     if (lane == 0) red[2] = chunk;
