@@ -50,8 +50,8 @@ constexpr int kMaxSplits = 32;            // block ranges of a column set
 constexpr int kMaxOwnSplits = 32;         // slices of a request's own columns in own_attn_kernel
 constexpr int kDirectCost = 3600;          // in tokens' time: the rounds' 3 us count 600 each
 // Rows per KV head up to which own_attn_kernel takes the own columns: 64 requests of 8192
-// shared and 300 own tokens take, with it and with work items, 42 and 63 us at 4 rows, 55
-// and 76 at 8, 74 and 84 at 12, 92 and 93 at 16 (112 and 120 with 2048 and 1500 tokens).
+// shared and 300 own tokens take, with it and with work items, 42 and 88 us at 4 rows, 56
+// and 89 at 8, 65 and 92 at 12, 71 and 93 at 16 (114 and 119 with 2048 and 1500 tokens).
 constexpr int kFewRows = 16;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -1455,7 +1455,7 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   const int own = max_own_len > 0 ? max_own_len : max_kv_len;
   // Decoding with more own columns than shared ones: prefix_attn_kernel gives a slot of its ring
   // to a second own_attn_kernel CTA beside it.  64 requests of 8192 shared and 300 own tokens
-  // 41.9 us with it, 45.5 without; 32 of 65536 and 500 85.9 and 77.7.
+  // 41.7 us with it, 46.1 without; 32 of 65536 and 500 85.9 and 77.7.
   f.narrow = f.few && max_own_len > 0 && (int64_t)batch * max_own_len >= (int64_t)groups * (max_kv_len - max_own_len);
   f.own_splits = 1;
   if (f.few || f.tail_rows)

@@ -668,8 +668,10 @@ def sharing_pays(max_qo_len: int, batch: int, num_qo_heads: int, num_kv_heads: i
     query heads per KV head) of a request and KV head per CTA, and joins nothing.  With 32
     query and 8 KV heads, 4096 shared tokens and 200 own ones it is the faster one once
     its units are three quarters full and there are about three quarters as many as SMs:
-    16 requests of 65 nodes 92 us against 102, of 49 nodes 90 against 92, but of 33 nodes
-    91 against 60; 4 requests of 65 nodes 62 against 52 (16384 tokens: 145 against 115)."""
+    16 requests of 65 nodes 93 us against 102, of 49 nodes 90 against 92, but of 33 nodes
+    91 against 61; 4 requests of 65 nodes 62 against 52 (16384 tokens: 146 against 99).
+    Shorter shared prefixes favour it more (40 requests of 65 nodes after 1024 tokens: 91
+    against 145), longer ones less (16 of 65 nodes after 16384: 319 against 294)."""
     rows = max_qo_len * (num_qo_heads // num_kv_heads)
     if dtype is not torch.bfloat16 or head_dim != 128 or page_len != 16 or num_qo_heads // num_kv_heads > 16:
         return True                                          # (tree_attention's slower kernel)
