@@ -353,7 +353,9 @@ int pts_kv_compact(void* kv_pool, int num_layers, int max_pages, int page_len, i
  * pts_cache_fork and pts_cache_extend change nothing when it is not 0, and the batch
  * of such an extend is one of empty sequences (an append to it writes nothing).  At most
  * 2^17 rows, 2^20 pages, 1024 forks and 4096 extended rows a call.  Calls on the
- * same state belong on one stream.
+ * same state belong on one stream.  The _noted forms do the same and also OR a status
+ * that is not 0 into *failures (nullable), which no call clears: one word of the caller's
+ * that keeps every failure, also those of a captured call's replays, until it is read.
  *
  * pts_cache_fork: page_table[dst_rows[i]] = page_table[src_rows[i]] as it was before
  * the call, for every i at once (a row may be a source and a destination, as in a
@@ -362,6 +364,9 @@ int pts_kv_compact(void* kv_pool, int num_layers, int max_pages, int page_len, i
 int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
                    int table_width, int max_pages, const int32_t* src_rows, const int32_t* dst_rows, int num_forks,
                    int32_t* status, pts_stream_t stream);
+int pts_cache_fork_noted(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
+                         int table_width, int max_pages, const int32_t* src_rows, const int32_t* dst_rows,
+                         int num_forks, int32_t* status, int32_t* failures, pts_stream_t stream);
 
 /* Make room for add_each[i] (or, where it is NULL, `add`) more tokens in every listed
  * row: a partial last page that other sequences hold too is copied first (its filled
@@ -397,6 +402,8 @@ typedef struct pts_cache_extend_args {
   int num_layers, max_pages, page_len, num_rows, table_width, add, batch, num_groups;
 } pts_cache_extend_args;
 int pts_cache_extend(const pts_cache_extend_args* args, void* workspace, size_t workspace_bytes, pts_stream_t stream);
+int pts_cache_extend_noted(const pts_cache_extend_args* args, int32_t* failures, void* workspace,
+                           size_t workspace_bytes, pts_stream_t stream);
 
 /* kv_lens[rows[i]] = min(kv_lens[rows[i]], new_lens[i]) (NULL or negative: 0); the
  * pages past the new length lose this holder and their entries become -1.  A row
@@ -405,6 +412,10 @@ int pts_cache_extend(const pts_cache_extend_args* args, void* workspace, size_t 
 int pts_cache_truncate(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int num_rows,
                        int table_width, int max_pages, int page_len, const int32_t* rows, const int32_t* new_lens,
                        int num, int32_t* status, pts_stream_t stream);
+int pts_cache_truncate_noted(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
+                             int num_rows, int table_width, int max_pages, int page_len, const int32_t* rows,
+                             const int32_t* new_lens, int num, int32_t* status, int32_t* failures,
+                             pts_stream_t stream);
 
 /* Close the pool's gaps: with n live pages (page_refs > 0), the k-th live page at or
  * past n moves, in every layer, to the k-th free page below n; the other pages stay.

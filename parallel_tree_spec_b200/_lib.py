@@ -106,8 +106,12 @@ SIGNATURES = {
     "pts_tree_attn_run_shared": (C.c_int, [vp, vp, sz, vp]),
     "pts_cache_workspace_size": (sz, [C.c_int, C.c_int]),
     "pts_cache_fork": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
+    "pts_cache_fork_noted": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp, vp]),
     "pts_cache_extend": (C.c_int, [vp, vp, sz, vp]),
+    "pts_cache_extend_noted": (C.c_int, [vp, vp, vp, sz, vp]),
     "pts_cache_truncate": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp, vp]),
+    "pts_cache_truncate_noted": (C.c_int, [vp, vp, i64, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, vp,
+                                           vp, vp]),
     "pts_cache_compact": (C.c_int, [vp, vp, sz, vp]),
     "pts_tree_mask_from_parents": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, vp]),
     "pts_tree_prepare": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp, vp, vp, vp]),

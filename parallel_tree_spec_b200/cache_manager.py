@@ -227,16 +227,13 @@ class SharedKvCache:
         self.page_table = torch.full((max_sequences, max_pages_per_sequence), -1, dtype=torch.int32, device=dev)
         self.kv_lens = torch.zeros(max_sequences, dtype=torch.int32, device=dev)
         self._bound = [0] * max_sequences                 # upper bounds of the lengths, for schedules only
-        self._statuses: List[torch.Tensor] = []
+        self._status = torch.zeros(1, dtype=torch.int32, device=dev)       # the last call's
+        self._failures = torch.zeros(1, dtype=torch.int32, device=dev)     # of all calls and replays since the last check
 
     def _ints(self, x) -> torch.Tensor:
         if isinstance(x, torch.Tensor):
             return x
         return torch.tensor(list(x), dtype=torch.int32, device=self.page_refs.device)
-
-    def _note(self, status: torch.Tensor) -> None:
-        self._statuses.append(status)
-        del self._statuses[:-256]
 
     def _limit(self) -> int:
         return self.page_table.shape[1] * self.pool.page_len
@@ -244,8 +241,8 @@ class SharedKvCache:
     def fork(self, src_rows, dst_rows) -> None:
         """``dst_rows[i]`` becomes a fork of ``src_rows[i]`` (all read before any is
         written; the destinations' former pages are given back)."""
-        self._note(K.cache_fork(self.page_refs, self.page_table, self.kv_lens, self._ints(src_rows),
-                                self._ints(dst_rows)))
+        K.cache_fork(self.page_refs, self.page_table, self.kv_lens, self._ints(src_rows), self._ints(dst_rows),
+                     self._status, self._failures)
         if isinstance(src_rows, torch.Tensor) or isinstance(dst_rows, torch.Tensor):
             self._bound = [max(self._bound)] * len(self._bound)
         else:
@@ -274,8 +271,8 @@ class SharedKvCache:
         else:
             each, seq = self._ints(adds), self._ints(accumulate(adds, initial=0))
         gi = up_to(2) * B if groups is None else self._ints(groups)
-        out = K.cache_extend(self.pool.cache_data, self.page_refs, self.page_table, self.kv_lens, r, each, group_indptr=gi)
-        self._note(out.status)
+        out = K.cache_extend(self.pool.cache_data, self.page_refs, self.page_table, self.kv_lens, r, each, group_indptr=gi,
+                             status=self._status, failures=self._failures)
         bp = KvCacheBatchPosition(seq, out.page_indptr, out.page_indices, out.last_page_len, None, None)
         bp.batch_indices, bp.positions = K.batch_positions(seq, out.seq_lens, sum(adds)) if any(adds) else (up_to(0), up_to(0))
         if isinstance(rows, torch.Tensor):
@@ -293,8 +290,8 @@ class SharedKvCache:
 
     def truncate(self, rows, new_lens=None) -> None:
         """Cut the listed sequences to ``new_lens`` tokens (None: free them)."""
-        self._note(K.cache_truncate(self.page_refs, self.page_table, self.kv_lens, self.pool.page_len,
-                                    self._ints(rows), None if new_lens is None else self._ints(new_lens)))
+        K.cache_truncate(self.page_refs, self.page_table, self.kv_lens, self.pool.page_len, self._ints(rows),
+                         None if new_lens is None else self._ints(new_lens), self._status, self._failures)
         if not isinstance(rows, torch.Tensor) and not isinstance(new_lens, torch.Tensor):
             for i, row in enumerate(rows):
                 if 0 <= row < len(self._bound):
@@ -316,11 +313,12 @@ class SharedKvCache:
         return list(self._bound)
 
     def check(self) -> None:
-        """Raise for a call since the last check that could not be done."""
-        pending, self._statuses = self._statuses, []
-        if pending:
-            for code in torch.cat(pending).tolist():
-                K.raise_cache_status(code)
+        """Raise for a call, or a replay of a captured one, since the last check that could
+        not be done (waits for the current stream)."""
+        code = int(self._failures.item())
+        if code:
+            self._failures.zero_()
+            K.raise_cache_status(code)
 
     def close(self) -> None:
         """Give the pool's pages back; the sequences are gone."""

@@ -43,6 +43,12 @@ struct PageState {
   int rows, width, pages;
 };
 
+// One thread of a call: its status, and a failure also in the caller's word.
+__device__ __forceinline__ void report(int32_t* status, int32_t* failures, int code) {
+  *status = code;
+  if (code && failures) atomicOr(failures, code);
+}
+
 // Marks row r in the bitmap; false if it was marked before.
 __device__ __forceinline__ bool mark(uint32_t* bitmap, int r) {
   const uint32_t bit = 1u << (r & 31);
@@ -59,7 +65,8 @@ __device__ __forceinline__ bool mark(uint32_t* bitmap, int r) {
 // other (128 forks of 95 columns: 49 KB in 6.4 us from a cold cache, 6 forks 4 us); an
 // entry that does not change (a child that keeps its parent's prefix) costs no atomics.
 __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, const int32_t* src, const int32_t* dst,
-                                                                  int n, int cols, int32_t* status) {
+                                                                  int n, int cols, int32_t* status,
+                                                                  int32_t* failures) {
   extern __shared__ uint32_t seen[];                    // rows listed as destinations
   __shared__ int32_t stage[kStageEntries];
   __shared__ int32_t from[kMaxForks], to[kMaxForks];
@@ -77,7 +84,7 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
     else if (!mark(seen, b)) atomicOr(&bad, kTwice);
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = bad;
+  if (blockIdx.x == 0 && threadIdx.x == 0) report(status, failures, bad);
   if (bad) return;
   const int c0 = blockIdx.x * cols;
   int32_t len[kMaxForks / kForkThreads];
@@ -132,7 +139,8 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(PageState s, c
 // atomics, so a row listed twice ends at the smaller length and gives each page
 // back once.  Bound by latency (512 rows 4.4-5 us from a cold cache).
 __global__ void __launch_bounds__(128) cache_truncate_kernel(PageState s, int page_len, const int32_t* rows,
-                                                             const int32_t* new_lens, int n, int32_t* status) {
+                                                             const int32_t* new_lens, int n, int32_t* status,
+                                                             int32_t* failures) {
   __shared__ int old_len;
   pdl_trigger();
   pdl_wait();
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(128) cache_truncate_kernel(PageState s, int pa
     bool bad = false;
     for (int i = threadIdx.x; i < n; i += 128) bad |= rows[i] < 0 || rows[i] >= s.rows;
     bad = __syncthreads_or(bad);
-    if (threadIdx.x == 0) *status = bad ? kBadIndex : 0;
+    if (threadIdx.x == 0) report(status, failures, bad ? kBadIndex : 0);
     return;
   }
   const int i = blockIdx.x, r = rows[i];
@@ -288,6 +296,7 @@ struct ExtendParams {
   int32_t* seq_lens;
   int32_t* shared_pages;     // null: not wanted
   int32_t* status;
+  int32_t* failures;         // nullable
   // workspace
   int32_t* holders;          // [P] listed rows that end in this page
   int32_t* final_row;        // [P] the last of them, + 1
@@ -419,7 +428,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_extend_plan_kernel(const E
   // Unchanged, and a batch of empty sequences: an append to it writes nothing (its tokens'
   // positions would otherwise be the last ones that are there, on pages that others may hold)
   if (tid == 0) {
-    *p.status = failed;
+    report(p.status, p.failures, failed);
     p.page_indptr[0] = 0;
   }
   if (p.shared_pages)
@@ -684,6 +693,14 @@ using namespace pts;
 extern "C" int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
                               int num_rows, int table_width, int max_pages, const int32_t* src_rows,
                               const int32_t* dst_rows, int num_forks, int32_t* status, pts_stream_t stream) {
+  return pts_cache_fork_noted(page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages, src_rows,
+                              dst_rows, num_forks, status, nullptr, stream);
+}
+
+extern "C" int pts_cache_fork_noted(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
+                                    int num_rows, int table_width, int max_pages, const int32_t* src_rows,
+                                    const int32_t* dst_rows, int num_forks, int32_t* status, int32_t* failures,
+                                    pts_stream_t stream) {
   if (int rc = check_state(page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages, true))
     return rc;
   PTS_CHECK_ARG(src_rows && dst_rows && status && num_forks > 0, "bad fork list");
@@ -697,19 +714,27 @@ extern "C" int pts_cache_fork(int32_t* page_refs, int32_t* page_table, int64_t t
   if (smem > 4 * 1024)
     if (int rc = ensure_smem_attr((const void*)cache_fork_kernel, smem)) return rc;
   PTS_CUDA_TRY(launch_pdl(cache_fork_kernel, dim3((table_width + cols - 1) / cols), dim3(kForkThreads), smem,
-                          (cudaStream_t)stream, s, src_rows, dst_rows, num_forks, cols, status));
+                          (cudaStream_t)stream, s, src_rows, dst_rows, num_forks, cols, status, failures));
   return launch_status("cache_fork_kernel");
 }
 
 extern "C" int pts_cache_truncate(int32_t* page_refs, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
                                   int num_rows, int table_width, int max_pages, int page_len, const int32_t* rows,
                                   const int32_t* new_lens, int num, int32_t* status, pts_stream_t stream) {
+  return pts_cache_truncate_noted(page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages,
+                                  page_len, rows, new_lens, num, status, nullptr, stream);
+}
+
+extern "C" int pts_cache_truncate_noted(int32_t* page_refs, int32_t* page_table, int64_t table_stride,
+                                        int32_t* kv_lens, int num_rows, int table_width, int max_pages, int page_len,
+                                        const int32_t* rows, const int32_t* new_lens, int num, int32_t* status,
+                                        int32_t* failures, pts_stream_t stream) {
   if (int rc = check_state(page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages, true))
     return rc;
   PTS_CHECK_ARG(rows && status && num > 0 && page_len > 0, "bad row list");
   const PageState s{page_refs, page_table, table_stride, kv_lens, num_rows, table_width, max_pages};
   PTS_CUDA_TRY(launch_pdl(cache_truncate_kernel, dim3(num + 1), dim3(128), 0, (cudaStream_t)stream, s, page_len, rows,
-                          new_lens, num, status));
+                          new_lens, num, status, failures));
   return launch_status("cache_truncate_kernel");
 }
 
@@ -720,6 +745,11 @@ extern "C" size_t pts_cache_workspace_size(int max_pages, int batch) {
 
 extern "C" int pts_cache_extend(const pts_cache_extend_args* args, void* workspace, size_t workspace_bytes,
                                 pts_stream_t stream) {
+  return pts_cache_extend_noted(args, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pts_cache_extend_noted(const pts_cache_extend_args* args, int32_t* failures, void* workspace,
+                                      size_t workspace_bytes, pts_stream_t stream) {
   PTS_CHECK_ARG(args, "null arguments");
   const pts_cache_extend_args& x = *args;
   if (int rc = check_state(x.page_refs, x.page_table, x.table_stride, x.kv_lens, x.num_rows, x.table_width, x.max_pages, true))
@@ -749,6 +779,7 @@ extern "C" int pts_cache_extend(const pts_cache_extend_args* args, void* workspa
   p.seq_lens = x.seq_lens;
   p.shared_pages = x.shared_pages;
   p.status = x.status;
+  p.failures = failures;
   p.holders = (int32_t*)workspace;
   p.final_row = p.holders + x.max_pages;
   p.pairs = p.final_row + x.max_pages;

@@ -958,29 +958,40 @@ def _status_word(status: Optional[torch.Tensor], like: torch.Tensor, index: int)
     return status
 
 
+def _failures_word(failures: Optional[torch.Tensor], index: int) -> int:
+    if failures is None:
+        return 0
+    _cache_ints("failures", failures, index, 1)
+    return failures.data_ptr()
+
+
 def cache_fork(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, src_rows: torch.Tensor,
-               dst_rows: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+               dst_rows: torch.Tensor, status: Optional[torch.Tensor] = None,
+               failures: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Make sequence ``dst_rows[i]`` a fork of ``src_rows[i]``: it holds the same
     pages and length, and its former pages lose a holder.  All rows are read before
     any is written, so a beam reorder may name a row as source and destination; no
     row is a destination twice.  No K/V moves: ``cache_extend`` copies a shared
     partial page when one of its holders grows.  ``page_refs`` [P], ``page_table``
     [R, W] (-1 past a sequence's end) and ``kv_lens`` [R] are int32 and updated in
-    place.  Returns the status word (``check_cache_status``)."""
+    place.  Returns the status word (``check_cache_status``).  ``failures``: an int32 word
+    into which the status is ORed and which no call clears, so that it keeps what any of
+    many calls, or of a captured call's replays, could not do."""
     index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
     n = _cache_ints("src_rows", src_rows, index)
     _cache_ints("dst_rows", dst_rows, index, n)
-    status = _status_word(status, page_refs, index)
+    status, noted = _status_word(status, page_refs, index), _failures_word(failures, index)
     if n == 0:
         return status.zero_()
-    _call_on(index, "pts_cache_fork", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(), R, W, P,
-             src_rows.data_ptr(), dst_rows.data_ptr(), n, status.data_ptr(), _raw_stream(index))
+    _call_on(index, "pts_cache_fork_noted", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(), R,
+             W, P, src_rows.data_ptr(), dst_rows.data_ptr(), n, status.data_ptr(), noted, _raw_stream(index))
     return status
 
 
 def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                  rows: torch.Tensor, add: Union[int, torch.Tensor], group_indptr: Optional[torch.Tensor] = None,
-                 out=None, status: Optional[torch.Tensor] = None) -> CacheBatch:
+                 out=None, status: Optional[torch.Tensor] = None,
+                 failures: Optional[torch.Tensor] = None) -> CacheBatch:
     """Make room for ``add`` more tokens (an int, or int32 [B]) in every listed
     sequence: a partial last page that others hold too is copied, then the lowest free
     pages follow.  Returns the batch of those rows; with ``group_indptr`` [G + 1]
@@ -988,7 +999,8 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
     ``tree_attention_shared``.  ``out``: (page_indptr [B + 1], page_indices [B * W],
     last_page_len [B], seq_lens [B], shared_pages [G] or None) to write into; entries of
     page_indices past page_indptr[B] are left as they are.  A call that cannot be done
-    (see the status) changes nothing and returns a batch of empty sequences."""
+    (see the status) changes nothing and returns a batch of empty sequences.
+    ``failures`` as for ``cache_fork``."""
     index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
     L, pl, row_bytes = _page_pool(pool, index, P)
     B = _cache_ints("rows", rows, index)
@@ -1019,33 +1031,34 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
         _cache_ints("seq_lens", lens, index, B)
         if G:
             _cache_ints("shared_pages", shared, index, G)
-    status = _status_word(status, page_refs, index)
+    status, noted = _status_word(status, page_refs, index), _failures_word(failures, index)
     words = 2 * P + 3 * B + 4                                # pts_cache_workspace_size
     ws = page_refs.new_empty(words)
-    _call_on(index, "pts_cache_extend", _lib.pack_cache_extend(
+    _call_on(index, "pts_cache_extend_noted", _lib.pack_cache_extend(
         pool.data_ptr(), row_bytes, page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(),
         rows.data_ptr(), each, group_indptr.data_ptr() if G else 0, indptr.data_ptr(), indices.data_ptr(), entries,
         last.data_ptr(), lens.data_ptr(), shared.data_ptr() if G else 0, status.data_ptr(), L, P, pl, R, W, add_all, B,
-        G), ws.data_ptr(), 4 * words, _raw_stream(index))
+        G), noted, ws.data_ptr(), 4 * words, _raw_stream(index))
     return CacheBatch(indptr, indices, last, lens, shared, status)
 
 
 def cache_truncate(page_refs: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, page_len: int,
                    rows: torch.Tensor, new_lens: Optional[torch.Tensor] = None,
-                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   status: Optional[torch.Tensor] = None, failures: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Cut the listed sequences to ``new_lens`` tokens (int32 [n]; None frees them):
     pages past the new length lose this holder.  A sequence already shorter keeps its
-    length.  Returns the status word; rows outside the table are skipped."""
+    length.  Returns the status word; rows outside the table are skipped.  ``failures`` as
+    for ``cache_fork``."""
     index, P, R, W, stride = _page_state(page_refs, page_table, kv_lens)
     n = _cache_ints("rows", rows, index)
     if new_lens is not None:
         _cache_ints("new_lens", new_lens, index, n)
-    status = _status_word(status, page_refs, index)
+    status, noted = _status_word(status, page_refs, index), _failures_word(failures, index)
     if n == 0:
         return status.zero_()
-    _call_on(index, "pts_cache_truncate", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(), R, W,
-             P, int(page_len), rows.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, n,
-             status.data_ptr(), _raw_stream(index))
+    _call_on(index, "pts_cache_truncate_noted", page_refs.data_ptr(), page_table.data_ptr(), stride, kv_lens.data_ptr(),
+             R, W, P, int(page_len), rows.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, n,
+             status.data_ptr(), noted, _raw_stream(index))
     return status
 
 

@@ -378,3 +378,67 @@ def test_extend_by_nothing_lists_the_pages():
         cache.extend([], 1)
     cache.check()
     assert cache.lengths() == [6, 6]
+
+
+def _full_cache():
+    """Two sequences of ten tokens that hold all six pages of the pool."""
+    pool = KvCachePool(6, 1, 1, 32, 4, torch.float32, torch.device(DEV))
+    cache = SharedKvCache(pool, 3, 4)
+    cache.extend([0, 1], 10)
+    cache.check()
+    return cache
+
+
+def test_a_failure_is_reported_however_many_calls_follow():
+    """300 steps without a check after one that could not be done: the check raises for
+    it, the next one does not."""
+    cache = _full_cache()
+    cache.extend([0, 1], 4)
+    for _ in range(300):
+        cache.fork([0], [0])
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.check()
+    cache.check()
+    cache.fork([0, 9, 1], [2, 2, 2])                          # two faults in one call
+    cache.truncate([5])
+    with pytest.raises(IndexError, match="listed twice"):
+        cache.check()
+    cache.check()
+
+
+def test_a_failed_replay_is_reported():
+    """Captured calls report in every replay, also after a check; those that could be done
+    report nothing."""
+    cache = _full_cache()
+    cache.release([1])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    rows, src, dst, gone = i32([0]), i32([0]), i32([2]), i32([2])
+
+    def body():
+        cache.fork(src, dst)
+        cache.extend(rows, 3)
+        cache.truncate(gone)
+
+    body()                                                    # 13 tokens in four pages
+    cache.check()
+    cache.truncate([0], [5])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        body()
+    cache.check()                                             # nothing has run
+    for n, fails in ((8, False), (11, False), (14, False), (14, True), (14, True)):
+        g.replay()
+        if fails:                                             # 17 tokens in a table of 16
+            with pytest.raises(RuntimeError, match="wide"):
+                cache.check()
+        cache.check()
+        assert cache.kv_lens.tolist() == [n, 0, 0]
+    g.replay()                                                # one more failure, then replays that could be done
+    for _ in range(300):
+        cache.truncate([0], [2])
+        g.replay()
+    with pytest.raises(RuntimeError, match="wide"):
+        cache.check()
+    assert cache.kv_lens.tolist() == [5, 0, 0]
+    cache.check()
