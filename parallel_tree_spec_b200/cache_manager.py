@@ -211,9 +211,8 @@ class SharedKvCache:
     ``truncate`` and ``release`` give pages back; ``compact`` closes the pool's gaps.  Rows
     (sequence numbers) and lengths may be lists or int32 tensors on the pool's device;
     with tensors (and one int for all rows in ``extend``) no call copies from the host or
-    waits for it, so a step can be captured in a CUDA graph (not ``compact``, which
-    replaces the state's tensors).  A
-    call that cannot be done changes nothing (the batch position of such an ``extend`` has
+    waits for it, so a step can be captured in a CUDA graph, ``compact`` too.  A call that
+    cannot be done changes nothing (the batch position of such an ``extend`` has
     empty sequences, so an append to it writes nothing); ``check`` raises for it.  The
     cache takes all pages of the pool, which must be free, until ``close``."""
 
@@ -302,9 +301,11 @@ class SharedKvCache:
 
     def compact(self) -> torch.Tensor:
         """Close the pool's gaps; returns the map from old to new page (-1: free).  Batch
-        positions from before name the old pages."""
+        positions from before name the old pages; captured steps of this class stay valid
+        (the state's tensors stay where they are)."""
         r = K.cache_compact(self.pool.cache_data, self.page_refs, self.page_table)
-        self.page_refs, self.page_table = r.page_refs, r.page_table
+        self.page_refs.copy_(r.page_refs)
+        self.page_table.copy_(r.page_table)
         return r.page_map
 
     def lengths(self) -> List[int]:

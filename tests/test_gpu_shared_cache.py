@@ -442,3 +442,76 @@ def test_a_failed_replay_is_reported():
         cache.check()
     assert cache.kv_lens.tolist() == [5, 0, 0]
     cache.check()
+
+
+@pytest.mark.parametrize("captured_compaction", [False, True])
+def test_a_captured_step_goes_on_after_a_compaction(captured_compaction):
+    """A step captured once, the pool compacted between its replays (as a call or as a
+    graph of its own): each replay reads and grows the sequences where they now are."""
+    Hq, Hkv, D, page, n = 8, 2, 64, 16, 3
+    pool = KvCachePool(30, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, 4, 8)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    gen = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    rows, parents = i32([0, 1]), i32(chain(n) * 2)
+    q, k, v = rnd(2 * n, Hq, D), rnd(2 * n, Hkv, D), rnd(2 * n, Hkv, D)
+    out = torch.empty(2 * n, Hq * D, dtype=torch.bfloat16, device=DEV)
+    hist = [torch.empty(0, 2, Hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+
+    def grow(row, m):
+        bp = cache.extend([row], m)
+        a, b = rnd(m, Hkv, D), rnd(m, Hkv, D)
+        w.append_kv_cache(None, a, b, bp, pool.cache_data[0], page)
+        hist[row] = torch.cat([hist[row], torch.stack([a, b], 1)])
+
+    def step():
+        bp = cache.extend(rows, n)
+        w.set_tree_masks(parents, bp, n)
+        out.copy_(w.computeAttention(q, k, v, pool.cache_data[0], "tree", bp, AttentionRotaryParams(), 0))
+
+    def noted():
+        for i in range(2):
+            hist[i] = torch.cat([hist[i], torch.stack([k[i * n:(i + 1) * n], v[i * n:(i + 1) * n]], 1)])
+
+    grow(2, 50)                                               # low pages, released below
+    grow(0, 21)
+    cache.fork([0], [1])
+    hist[1] = hist[0]
+    step()
+    noted()
+    cache.compact()                                           # (modules loaded before the captures)
+    torch.cuda.synchronize()
+    g, gc = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    if captured_compaction:
+        with torch.cuda.graph(gc):
+            cache.compact()
+    table = cache.page_table.tolist()
+    for gap in (2, None, 3):
+        if gap:
+            cache.release([gap])
+            gc.replay() if captured_compaction else cache.compact()
+            assert cache.page_table.tolist()[:2] != table[:2]     # pages moved
+            live = int((cache.page_refs > 0).sum())
+            assert (cache.page_refs[:live] > 0).all()
+        for x in (q, k, v):
+            x.copy_(rnd(*x.shape))
+        g.replay()
+        noted()
+        for i in range(2):
+            L = hist[i].shape[0]
+            o, A = dense(q[i * n:(i + 1) * n], hist[i], torch.ones(n, L, dtype=torch.bool, device=DEV).tril(L - n))
+            bad = (out.view(-1, Hq, D)[i * n:(i + 1) * n].double() - o).abs() / ((2 ** -7 + 2.0 ** -12) * A + 2 ** -8 * o.abs())
+            assert bad.max().item() <= 1.0
+        assert cache.kv_lens.tolist()[:2] == [h.shape[0] for h in hist[:2]]
+        held = np.bincount([p for r in cache.page_table.tolist() for p in r if p >= 0], minlength=30)
+        assert held.tolist() == cache.page_refs.tolist()
+        if gap == 2:
+            grow(3, 40)
+            for row, m in ((0, 20), (1, 9)):                  # pages behind row 3's
+                grow(row, m)
+        table = cache.page_table.tolist()
+    cache.check()
