@@ -194,6 +194,15 @@ __device__ __forceinline__ bool fill_unit(const AttnParams& p, int b, int h, int
   return s.kv_len > 0;
 }
 
+// Zeroes rows R0 .. R0 + n - 1 of the request at q0 and KV head h: without KV its rows see nothing.
+__device__ __forceinline__ void zero_rows(const AttnParams& p, int q0, int h, int R0, int n, int thread, int threads) {
+  for (int64_t i = thread; i < (int64_t)n * (kD / 8); i += threads) {
+    const int R = R0 + (int)(i / (kD / 8));
+    *(uint4*)(p.out + ((int64_t)(q0 + R / p.g) * p.Hq + h * p.g + R % p.g) * kD + i % (kD / 8) * 8) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // The CTA of the balanced schedule whose range holds block x.
 __device__ __forceinline__ int cta_of(const Sched& S, int x) {
   return (int)(((long long)(x + 1) * S.ctas - 1) / S.total);
@@ -295,6 +304,16 @@ __device__ void build_schedule(const AttnParams& p, Sched& S, int lane) {
     // spans at most kMaxSpan CTAs
     const int chunk = max(kMinBlocksPerCta, (mx + kMaxSpan - 2) / (kMaxSpan - 1));
     S.ctas = run > 0 ? max(1, min((int)gridDim.x, run / chunk)) : 0;
+  }
+}
+
+// Warp 15: the rows of every gridDim.x-th entry that has no blocks.
+__device__ void zero_empty_entries(const AttnParams& p, const Sched& S, int lane) {
+  for (int e = blockIdx.x; e < p.n_entries; e += gridDim.x) {
+    if (S.nblk[e] > 0) continue;
+    const int b = p.head_pages ? e / p.Hkv : e, q0 = p.qo_indptr[b], rows = (p.qo_indptr[b + 1] - q0) * p.g;
+    const int h0 = p.head_pages ? e % p.Hkv : 0, h1 = p.head_pages ? h0 + 1 : p.Hkv;
+    for (int h = h0; h < h1; ++h) zero_rows(p, q0, h, 0, rows, lane, 32);
   }
 }
 
@@ -403,11 +422,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncthreads();
-    if ((int)blockIdx.x >= S.ctas) return;            // no range (uniform over the CTA)
+    if ((int)blockIdx.x >= S.ctas) {                  // no range (uniform over the CTA)
+      if (warp == kScheduleWarp) zero_empty_entries(p, S, lane);
+      return;
+    }
   } else {
     Segment s0;
     int pos0 = 0;
-    if (!next_segment<kBalanced>(p, S, 0, pos0, s0)) return;     // no rows or no KV
+    if (!next_segment<kBalanced>(p, S, 0, pos0, s0)) {           // no rows or no KV
+      const int rows = min(kGroupRows, s0.n_nodes * p.g - s0.row0);
+      if (rows > 0) zero_rows(p, s0.q0, s0.h, s0.row0, rows, threadIdx.x, kThreads);
+      return;
+    }
   }
 
   if (threadIdx.x == 0) {
@@ -1076,6 +1102,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (kBalanced) named_bar_sync(1, kSyncWarps * 32);     // the merge area is free for the next segment
     }  // segments
+  } else if (kBalanced && warp == kScheduleWarp) {
+    zero_empty_entries(p, S, lane);
   }
   tc_fence_before();
   __syncthreads();

@@ -138,3 +138,72 @@ def test_repeat_is_deterministic():
     a = run_kernel(c)
     b = run_kernel(c)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("schedule", [K.ATTN_SCHEDULE_PER_UNIT, K.ATTN_SCHEDULE_BALANCED])
+@pytest.mark.parametrize("lens", [[0, 40, 0, 0], [0, 0, 0], [5000, 0]])
+def test_requests_without_tokens_are_zero(dtype, schedule, lens):
+    """Rows of a request whose cache is empty see nothing: they are 0, whatever `out` held,
+    and the other requests' rows are what they are without it (up to the rounding of the
+    probabilities and outputs, 2^-8 of the largest value each, in both calls); rows past the
+    last request are left."""
+    Hq, Hkv, D, pl, n = 8, 2, 128, 16, 70
+    gen = torch.Generator().manual_seed(sum(lens))
+    pages = [-(-L // pl) for L in lens]
+    layer = torch.randn(max(1, sum(pages)), 2, pl, Hkv, D, generator=gen).to(dtype).to(DEV)
+    T = n * len(lens)
+    q = torch.randn(T + 3, Hq, D, generator=gen).to(dtype).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    indices, last = i32(list(range(sum(pages))) or [0]), i32([(L - 1) % pl + 1 if L else 0 for L in lens])
+    prev = K.set_attention_schedule(schedule)
+    try:
+        out = torch.full_like(q, 7.0)
+        K.tree_attention(q, layer, i32([n * i for i in range(len(lens) + 1)]), i32(np.cumsum([0] + pages).tolist()),
+                         indices, last, None, n, max(max(lens), 1), out=out)
+        full = [i for i, L in enumerate(lens) if L]
+        rest = torch.full_like(q, 7.0)
+        if full:
+            K.tree_attention(torch.cat([q[n * i:n * (i + 1)] for i in full]), layer,
+                             i32([n * i for i in range(len(full) + 1)]),
+                             i32(np.cumsum([0] + [pages[i] for i in full]).tolist()), indices, last[full].contiguous(),
+                             None, n, max(lens), out=rest[:n * len(full)])
+    finally:
+        K.set_attention_schedule(prev)
+    for i, L in enumerate(lens):
+        got = out[n * i:n * (i + 1)].float()
+        if L:
+            j = full.index(i)
+            want = rest[n * j:n * (j + 1)].float()
+            most = layer[:, 1].float().abs().max().item()
+            assert (got - want).abs().max().item() <= 2 * (2 * 2.0 ** -8 + 2.0 ** -12) * most
+        else:
+            assert (got == 0).all()
+    assert (out[T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("schedule", [K.ATTN_SCHEDULE_PER_UNIT, K.ATTN_SCHEDULE_BALANCED])
+def test_heads_without_pages_are_zero(schedule):
+    """A KV head whose page list is empty: its rows are 0, the other heads' are not."""
+    Hq, Hkv, D, pl, n = 8, 2, 128, 16, 70
+    gen = torch.Generator().manual_seed(1)
+    layer = torch.randn(20, 2, pl, Hkv, D, generator=gen).to(torch.bfloat16).to(DEV)
+    q = torch.randn(2 * n, Hq, D, generator=gen).to(torch.bfloat16).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    prev = K.set_attention_schedule(schedule)
+    try:
+        out = K.tree_attention_head_pages(q, layer, i32([0, n, 2 * n]), i32([0, 5, 5, 5, 12]), i32(list(range(12))),
+                                          i32([10, 0, 0, 16]), None, n, 7 * pl, out=torch.full_like(q, 7.0))
+    finally:
+        K.set_attention_schedule(prev)
+    g = Hq // Hkv
+    assert (out[:n, g:] == 0).all() and (out[n:, :g] == 0).all()
+    for rows, heads, pages, last in ((slice(0, n), 0, range(5), 10), (slice(n, 2 * n), 1, range(5, 12), 16)):
+        kv = layer[list(pages), :, :, heads].transpose(0, 1).reshape(2, -1, D)[:, :pl * (len(pages) - 1) + last].float()
+        s = torch.einsum("ngd,ld->ngl", q[rows, heads * g:(heads + 1) * g].float(), kv[0]) / math.sqrt(D)
+        L = s.shape[-1]
+        s = s.masked_fill(~torch.ones(n, L, dtype=torch.bool, device=DEV).tril(L - n)[:, None], float("-inf"))
+        want = torch.softmax(s, -1) @ kv[1]
+        # probabilities and output rounded to bf16: 2^-8 of the largest value each
+        assert (out[rows, heads * g:(heads + 1) * g].float() - want).abs().max().item() <= \
+            (2 * 2.0 ** -8 + 2.0 ** -12) * kv[1].abs().max().item()

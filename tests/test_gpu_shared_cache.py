@@ -515,3 +515,25 @@ def test_a_captured_step_goes_on_after_a_compaction(captured_compaction):
                 grow(row, m)
         table = cache.page_table.tolist()
     cache.check()
+
+
+def test_a_failed_extend_of_full_trees_gives_zeros():
+    """Trees that the wrapper gives to tree_attention: a batch that could not be extended
+    is one of empty sequences, its outputs are 0 whatever the memory held."""
+    page, Hq, Hkv, D, B, n = 16, 32, 8, 128, 14, 65
+    pool = KvCachePool(20, 1, Hkv, D, page, torch.bfloat16, torch.device(DEV))
+    cache = SharedKvCache(pool, B, 16)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    cache.extend([0], 70)
+    cache.fork([0] * (B - 1), list(range(1, B)))
+    bp = cache.extend(list(range(B)), n)
+    assert not K.sharing_pays(n, B, Hq, Hkv, D, page, torch.bfloat16)
+    w.set_tree_masks(torch.tensor(chain(n) * B, dtype=torch.int32, device=DEV), bp, n)
+    x = lambda h: torch.ones(B * n, h, D, dtype=torch.bfloat16, device=DEV)
+    q, k = x(Hq), x(Hkv)
+    for _ in range(3):
+        junk = [torch.full((B * n, Hq, D), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+        del junk
+        assert (w.computeAttention(q, k, k, pool.cache_data[0], "tree", bp, AttentionRotaryParams(), 0) == 0).all()
+    with pytest.raises(RuntimeError):
+        cache.check()
