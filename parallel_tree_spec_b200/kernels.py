@@ -647,14 +647,13 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
     es = 2 if q.dtype is torch.bfloat16 else 4
     nbytes = _shared_attn_workspace(index, B, G, T, max_qo, max_kv, own, Hq, Hkv, D, pl, es)
     ws = qo_indptr.new_empty((nbytes + 3) // 4) if nbytes else None
-    err = _ERROR_WORDS.get(index)
-    if err is None:
-        err = _error_word(index)
+    stream = _raw_stream(index)
+    err = _error_word(index, stream)
     _call_on(index, "pts_tree_attn_run_shared", _lib.pack_shared_attn(
         q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
         last_page_len.data_ptr(), bits, group_indptr.data_ptr(), shared_pages.data_ptr(), out.data_ptr(),
         err.data_ptr() if err is not None else 0, words, G, B, T, max_qo, max_kv, own, Hq, Hkv, D, pl, P, es,
-        sm_scale if sm_scale is not None else D ** -0.5), ws.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
+        sm_scale if sm_scale is not None else D ** -0.5), ws.data_ptr() if nbytes else None, nbytes, stream)
     if _CHECK_ATTENTION:
         check_attention(q.device)
     return out
@@ -687,16 +686,33 @@ def _shared_attn_workspace(index: int, *sizes: int) -> int:
         return _lib.lib().pts_tree_attn_shared_workspace_size(*sizes)
 
 
-_ERROR_WORDS: Dict[int, torch.Tensor] = {}
+# In which tree_attention_shared's launches report that they gave up waiting: a word per
+# device and stream, and one per device (stream None) for captured launches, which run on
+# whatever stream replays them.
+_ERROR_WORDS: Dict[Tuple[int, Optional[int]], torch.Tensor] = {}
 
 
-def _error_word(index: int) -> Optional[torch.Tensor]:
-    """The word in which tree_attention_shared's launches on a device report that they gave
-    up waiting: one for all streams and graphs, made outside of captures."""
-    if index not in _ERROR_WORDS and not torch.cuda.is_current_stream_capturing():
-        _ERROR_WORDS[index] = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
-        torch.cuda.current_stream(index).synchronize()     # zero before another stream's launch writes it
-    return _ERROR_WORDS.get(index)
+def _error_word(index: int, stream: int) -> Optional[torch.Tensor]:
+    """The word for a launch on this stream (None: captured before the device's first
+    launch outside of a capture, which makes the captured launches' word)."""
+    if _capturing(index):
+        return _ERROR_WORDS.get((index, None))
+    word = _ERROR_WORDS.get((index, stream))
+    if word is None:
+        dev = torch.device("cuda", index)
+        if (index, None) not in _ERROR_WORDS:
+            shared = torch.zeros(64, dtype=torch.int32, device=dev)
+            torch.cuda.current_stream(index).synchronize()  # zero before another stream's launch writes it
+            _ERROR_WORDS[index, None] = shared
+        word = _ERROR_WORDS[index, stream] = torch.zeros(64, dtype=torch.int32, device=dev)
+    return word
+
+
+def _capturing(index: int) -> bool:
+    if torch._C._cuda_getDevice() == index:
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(index):
+        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 # PTS_B200_CHECK=1: read the attention kernels' error word after every call
@@ -706,16 +722,18 @@ _CHECK_ATTENTION = os.environ.get("PTS_B200_CHECK", "0") not in ("", "0")
 
 def check_attention(device: Optional[torch.device] = None) -> None:
     """Raise if an attention launch on the current stream gave up waiting
-    (pts_tree_attn_check: synchronises the stream, then clears the error)."""
+    (pts_tree_attn_check: synchronises the stream, then clears the error).  What a captured
+    tree_attention_shared reports in a replay is raised once, by the next check on any stream
+    of the device."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    status = C.c_int(0)
-    word = _error_word(dev.index if dev.index is not None else torch.cuda.current_device())
-    for ws in [workspace(dev, "attn", 256)] + ([word] if word is not None else []):
-        _lib.call("pts_tree_attn_check", ws.data_ptr(), C.addressof(status), _stream(dev))
-        if status.value != 0:
-            break
-    if status.value != 0:
-        raise RuntimeError(f"tree attention gave up waiting (error {status.value}); its output is not valid")
+    index = dev.index if dev.index is not None else torch.cuda.current_device()
+    stream, status, seen = _stream(dev), C.c_int(0), 0
+    for word in (workspace(dev, "attn", 256), _ERROR_WORDS.get((index, stream)), _ERROR_WORDS.get((index, None))):
+        if word is not None:
+            _lib.call("pts_tree_attn_check", word.data_ptr(), C.addressof(status), stream)
+            seen = seen or status.value
+    if seen != 0:
+        raise RuntimeError(f"tree attention gave up waiting (error {seen}); its output is not valid")
 
 
 def set_wait_limit(cycles: int) -> int:

@@ -537,3 +537,46 @@ def test_a_failed_extend_of_full_trees_gives_zeros():
         assert (w.computeAttention(q, k, k, pool.cache_data[0], "tree", bp, AttentionRotaryParams(), 0) == 0).all()
     with pytest.raises(RuntimeError):
         cache.check()
+
+
+def test_a_stream_reports_only_its_own_waits():
+    """A launch that gave up is reported on its own stream, whichever stream is checked
+    first."""
+    a = Case([(40, [(30, chain(1))] * 40)], Hq=32, Hkv=8, seed=2).device()
+    K.tree_attention_shared(**a)
+    torch.cuda.synchronize()
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    before = K.set_wait_limit(1)
+    try:
+        with torch.cuda.stream(s):
+            K.tree_attention_shared(**a)
+    finally:
+        K.set_wait_limit(before)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        K.tree_attention_shared(**a)
+        K.check_attention(torch.device(DEV))
+    with torch.cuda.stream(s):
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            K.check_attention(torch.device(DEV))
+        K.check_attention(torch.device(DEV))
+
+
+def test_a_captured_launch_that_gives_up_is_reported_after_its_replays():
+    a = Case([(40, [(30, chain(1))] * 40)], Hq=32, Hkv=8, seed=2).device()
+    K.tree_attention_shared(**a)
+    torch.cuda.synchronize()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    before = K.set_wait_limit(1)
+    try:
+        with torch.cuda.graph(g):
+            K.tree_attention_shared(**a)
+    finally:
+        K.set_wait_limit(before)
+    K.check_attention(torch.device(DEV))
+    for _ in range(2):
+        with torch.cuda.stream(s):
+            g.replay()
+            with pytest.raises(RuntimeError, match="gave up waiting"):
+                K.check_attention(torch.device(DEV))
+            K.check_attention(torch.device(DEV))
