@@ -1460,7 +1460,7 @@ PrefixPlan plan_prefix(int batch, int groups, int total_q, int max_qo_len, int m
   f.own_splits = 1;
   if (f.few || f.tail_rows)
     f.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({6ll * f.ctas / std::max<int64_t>((int64_t)batch * Hkv, 1),
-                                                                (own + 4 * kRun - 1) / (4 * kRun), kMaxOwnSplits}));
+                                                                ((int64_t)own + 4 * kRun - 1) / (4 * kRun), kMaxOwnSplits}));
   int64_t units = ((int64_t)total_q * g + kTileRows - 1) / kTileRows + groups;
   if (!f.few) units += ((int64_t)total_q * g + kTileRows - 1) / kTileRows + batch;
   f.max_items = (int)std::min<int64_t>(units * Hkv + 2 * f.ctas, 1 << 28);

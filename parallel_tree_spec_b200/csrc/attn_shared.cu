@@ -277,9 +277,9 @@ Plan make_plan(int batch, int groups, int total_q, int max_qo_len, int max_kv_le
   Plan pl;
   const int g = Hq / Hkv;
   pl.group_tiles = (int)(((int64_t)total_q * g + kRows - 1) / kRows) + groups;
-  pl.request_tiles = (max_qo_len * g + kRows - 1) / kRows;
+  pl.request_tiles = (int)(((int64_t)max_qo_len * g + kRows - 1) / kRows);
   const int64_t ctas = ((int64_t)pl.group_tiles + (int64_t)batch * pl.request_tiles) * Hkv;
-  const int64_t most = std::max<int64_t>(1, (max_kv_len + kTile - 1) / kTile);
+  const int64_t most = std::max<int64_t>(1, ((int64_t)max_kv_len + kTile - 1) / kTile);
   pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * 148 / std::max<int64_t>(ctas, 1), most, 32}));
   const size_t slots = (size_t)total_q * Hq * 2 * pl.splits;
   pl.part_o = align_up(slots * sizeof(float2), 256);
@@ -325,6 +325,7 @@ extern "C" size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups,
   if (batch <= 0 || num_groups <= 0 || total_q <= 0 || max_qo_len <= 0 || max_kv_len <= 0 || num_qo_heads <= 0 ||
       num_kv_heads <= 0 || num_qo_heads % num_kv_heads || head_dim <= 0)
     return 0;
+  max_qo_len = std::min(max_qo_len, total_q);           // (a request has at most all rows)
   if (prefix_attn_supports(head_dim, page_len, elem_bytes))
     return prefix_attn_workspace(batch, num_groups, total_q, max_qo_len, max_kv_len, max_own_len, num_qo_heads,
                                  num_kv_heads, head_dim);
@@ -379,9 +380,10 @@ extern "C" int pts_tree_attn_run_shared(const pts_shared_attn_args* args, void* 
   a.page_len = x.page_len;
   a.max_pages = x.max_pages;
   a.scale = x.sm_scale;
+  const int max_qo_len = std::min(x.max_qo_len, x.total_q);
   if (prefix_attn_supports(x.head_dim, x.page_len, x.elem_bytes))
-    return prefix_attn_launch(a, x.total_q, x.max_qo_len, x.max_kv_len, x.max_own_len, workspace, x.error, (cudaStream_t)stream);
-  const Plan pl = make_plan(x.batch, x.num_groups, x.total_q, x.max_qo_len, x.max_kv_len, x.num_qo_heads, x.num_kv_heads, x.head_dim);
+    return prefix_attn_launch(a, x.total_q, max_qo_len, x.max_kv_len, x.max_own_len, workspace, x.error, (cudaStream_t)stream);
+  const Plan pl = make_plan(x.batch, x.num_groups, x.total_q, max_qo_len, x.max_kv_len, x.num_qo_heads, x.num_kv_heads, x.head_dim);
   const int64_t gx = (int64_t)pl.group_tiles + (int64_t)x.batch * pl.request_tiles;
   if (gx > 2147483647ll) return set_error(PTS_ERR_CAPACITY, "grid too large");
   PartsParams p{a, pl.splits, pl.group_tiles, pl.request_tiles, (float*)((char*)workspace + pl.part_o),

@@ -138,3 +138,17 @@ def test_small_calls_need_no_workspace():
     assert size(64, 1, 64, 1, 9000, 300, 32, 8, 128, 16, 2) > 0
     assert size(6, 1, 6, 1, 600, 0, 32, 8, 64, 16, 4) > 0      # fp32
     assert size(0, 1, 6, 1, 600, 0, 32, 8, 64, 16, 2) == 0     # refused by the call
+
+
+@pytest.mark.parametrize("dtype_bytes,head_dim,page", [(4, 64, 16), (2, 96, 16), (2, 128, 8), (2, 128, 16), (2, 64, 16)])
+def test_the_largest_length_bounds_keep_the_columns_cut(dtype_bytes, head_dim, page):
+    """A bound of 2^31 - 1 tokens (no bound known) cuts the columns as finely as a bound of
+    a million does: the workspace, which holds a part per cut, is as large."""
+    size = _lib.lib().pts_tree_attn_shared_workspace_size
+    for rows in (1, 20, 65):                                  # single tokens, trees, trees with a tail tile
+        at = lambda max_kv, own=0, n=rows: size(2, 1, 2 * rows, n, max_kv, own, 8, 2, head_dim, page, dtype_bytes)
+        most = 2 ** 31 - 1
+        assert at(1 << 20) > 0
+        assert at(most) == at(1 << 20) == at(most - 40)
+        assert at(most, most) == at(1 << 20, 1 << 20)
+        assert at(1 << 20, 0, most) == at(1 << 20, 0, 2 * rows)   # no request has more rows than there are
