@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(32 * NW, kDirect ? 1 : 7)
           odd |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
         }
       }
-      odd = __any_sync(0xffffffffu, odd) && n_tok > 1;
+      odd = __any_sync(0xffffffffu, odd) && (n_tok > 1 || a.mask_bits);   // (a lone causal row sees all)
       __syncwarp();
     }
     if (!odd) {

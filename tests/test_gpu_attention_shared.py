@@ -391,3 +391,18 @@ def test_refusals():
     odd.q, odd.kv = odd.q[..., :48].contiguous(), odd.kv[..., :48].contiguous()
     with pytest.raises(Exception, match="head_dim"):
         K.tree_attention_shared(**odd.device())
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("shared,own", [(0, 0), (0, 5), (3, 0), (3, 21), (600, 40)])
+def test_a_lone_row_that_does_not_see_its_own_slot(dtype, bad, shared, own):
+    """One row per request, masked from its own slot, whose value is infinite or NaN."""
+    c = Case([(shared, [(own, chain(1)), (own + 16, chain(1))] * 8)], dtype=dtype, seed=17)
+    for b in range(0, 16, 3):
+        L = c.lens[b]
+        c.masks[b][0, L - 1] = False
+        c.kv[c.tables[b][(L - 1) // c.pl], 1, (L - 1) % c.pl] = bad
+    got = check(c)
+    if not shared and not own:
+        assert (got[0] == 0).all()
