@@ -25,6 +25,9 @@
 //   the own columns are work items).
 //
 // Scores are kept in units of log2: x = s * scale * log2(e), e^(s - m) = 2^(x - m').
+#include <float.h>
+#include <math.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -121,6 +124,11 @@ struct PrefixParams {
   int copy_tokens;          // tokens per TMA copy: the power of two in page_len, at most a block
   int page_shift;           // log2(page_len), or -1
   float scale_log2;
+  // prefix_attn_kernel takes a row's maximum before the scale, which therefore has to be
+  // positive there: a negative one changes the queries' signs instead, and 0 becomes the
+  // smallest normal number, 2^-126 (scores up to 2^100 count as 2^-26 at most)
+  float item_scale;
+  uint32_t flip;            // on two packed bf16
   int* error;
   long long wait_limit;
   // plan
@@ -743,6 +751,7 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
             const int tk = p.div_g.div(R);
             v[j] = make_uint4(0, 0, 0, 0);
             if (my0 + r < it.rows) v[j] = __ldg((const uint4*)(q + ((int64_t)tk * a.Hq + (R - tk * a.g)) * D));
+            v[j] = make_uint4(v[j].x ^ p.flip, v[j].y ^ p.flip, v[j].z ^ p.flip, v[j].w ^ p.flip);
           }
 #pragma unroll
           for (int j = 0; j < kLoads; ++j) {
@@ -791,7 +800,7 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
           x2 = fmax3(x2, __uint_as_float(s[c / 64][c % 64 + 4]), __uint_as_float(s[c / 64][c % 64 + 5]));
           x3 = fmax3(x3, __uint_as_float(s[c / 64][c % 64 + 6]), __uint_as_float(s[c / 64][c % 64 + 7]));
         }
-        const float top = fmax3(x0, x1, fmaxf(x2, x3)) * p.scale_log2;
+        const float top = fmax3(x0, x1, fmaxf(x2, x3)) * p.item_scale;
         const bool need = top > m + kRescale;
         float alpha = 1.0f;
         if (need) {
@@ -811,7 +820,7 @@ __global__ void __launch_bounds__(kBoundThreads, 1)
           }
         }
         const float sub = m == -INFINITY ? 0.0f : m;
-        const uint64_t sc2 = f2(p.scale_log2, p.scale_log2), nm2 = f2(-sub, -sub);
+        const uint64_t sc2 = f2(p.item_scale, p.item_scale), nm2 = f2(-sub, -sub);
         uint64_t l0 = f2(0.0f, 0.0f), l1 = l0;
         // P's two halves are handed over one by one: the first one's product runs during
         // the second one's exponentials
@@ -1578,6 +1587,8 @@ int prefix_attn_launch(const SharedAttnParams& a, int total_q, int max_qo_len, i
   for (int s = 0; s < 31; ++s)
     if (a.page_len == 1 << s) p.page_shift = s;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.item_scale = fabsf(p.scale_log2) < FLT_MIN ? FLT_MIN : fabsf(p.scale_log2);
+  p.flip = a.scale < 0.0f ? 0x80008000u : 0u;
   p.error = error;
   p.wait_limit = wait_limit_cycles();
   p.ctas = f.ctas;

@@ -406,3 +406,17 @@ def test_a_lone_row_that_does_not_see_its_own_slot(dtype, bad, shared, own):
     got = check(c)
     if not shared and not own:
         assert (got[0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("scale", [-0.25, 0.0, 1e-40, -1e-3])
+@pytest.mark.parametrize("shared,rows", [(5, 1), (5, 6), (700, 1), (20, 70)])
+def test_scales_that_are_not_positive(dtype, scale, shared, rows):
+    """Negative scales and 0 (the mean of what a row sees), through each of the kernels: the
+    queries' negatives with the scale's magnitude say what they give."""
+    c = Case([(shared, [(9, chain(rows)), (6, chain(1))])], dtype=dtype, seed=9)
+    c.scale = abs(scale)
+    q = c.q
+    if scale < 0:
+        c.q = -q
+    check(c, q=q.to(DEV), sm_scale=scale)
