@@ -80,7 +80,8 @@ class BeFlashinferWrapper:
     # ------------------------------------------------------------------ plan
     def prepareAttention(self, mode: str, batch_position: KvCacheBatchPosition, page_len: int, pos_encoding_mode,
                          dtype: torch.dtype, attention_mask: Optional[torch.Tensor] = None):
-        """Plan the next forward pass (``attention_wrapper.py:113-170``)."""
+        """Plan the next forward pass (``attention_wrapper.py:113-170``).  A mask for a batch
+        position whose lengths the host only bounds waits for the device."""
         if mode not in ("tree", "prefill", "decode"):
             raise ValueError(f"Invalid attention mode: {mode}")
         if page_len != self.page_len:
@@ -96,6 +97,11 @@ class BeFlashinferWrapper:
             kv_lens = [(pind[i + 1] - pind[i] - 1) * page_len + last[i] for i in range(len(last))]
         bits, words = None, 1
         if mode == "tree" and attention_mask is not None:
+            if bp.host_kv_bounds:
+                pind, last = bp.kv_page_indptr.tolist(), bp.kv_last_page_len.tolist()
+                kv_lens = [(b - a - 1) * page_len + n if b > a else 0 for a, b, n in zip(pind, pind[1:], last)]
+                if any(L < n for n, L in zip(qo_lens, kv_lens)):
+                    raise ValueError("a request has fewer tokens in its pages than rows (a failed extend)")
             words = K.mask_words_for(max(qo_lens))
             m = attention_mask.to(self.device, non_blocking=True).reshape(-1)
             mind = [0]

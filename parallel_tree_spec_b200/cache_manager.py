@@ -47,6 +47,8 @@ class KvCacheBatchPosition:
         self.positions = positions
         self.host_qo_lens = None
         self.host_kv_lens = None
+        # host_kv_lens are upper bounds, the lengths are on the device only (SharedKvCache)
+        self.host_kv_bounds = False
         # requests that share leading pages (SharedKvCache.extend, beam_search): groups of
         # consecutive requests and each group's common pages, for tree_attention_shared
         self.group_indptr = None
@@ -283,7 +285,7 @@ class SharedKvCache:
                 if 0 <= row < len(self._bound):
                     self._bound[row] = min(self._bound[row] + n, self._limit())
             lens = [self._bound[row] if 0 <= row < len(self._bound) else 0 for row in rows]
-        bp.host_qo_lens, bp.host_kv_lens = adds, [max(1, n) for n in lens]
+        bp.host_qo_lens, bp.host_kv_lens, bp.host_kv_bounds = adds, [max(1, n) for n in lens], True
         bp.group_indptr, bp.shared_pages = gi, out.shared_pages
         return bp
 

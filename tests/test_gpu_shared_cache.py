@@ -580,3 +580,41 @@ def test_a_captured_launch_that_gives_up_is_reported_after_its_replays():
             with pytest.raises(RuntimeError, match="gave up waiting"):
                 K.check_attention(torch.device(DEV))
             K.check_attention(torch.device(DEV))
+
+
+def test_boolean_masks_for_a_cache_whose_lengths_are_bounds():
+    """prepareAttention takes the masks' widths from the sequences' lengths, also where
+    the host only has bounds of them."""
+    page, Hq, Hkv, D = 16, 4, 2, 64
+    pool = KvCachePool(12, 1, Hkv, D, page, torch.float32, torch.device(DEV))
+    cache = SharedKvCache(pool, 3, 4)
+    w = BeFlashinferWrapper(Hq, Hkv, Hq * D, page, torch.device(DEV))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    cache.extend([0], 30)
+    cache.fork([0], [1])
+    cache.truncate([0, 1], i32([20, 11]))
+    n = [3, 2]
+    bp = cache.extend([0, 1], n)
+    lens = [23, 13]
+    masks = [torch.rand(a, L, generator=torch.Generator().manual_seed(L)) < 0.5 for a, L in zip(n, lens)]
+    for m, a, L in zip(masks, n, lens):
+        m[:, :L - a] = True
+    w.prepareAttention("tree", bp, page, "NONE", torch.float32, torch.cat([m.reshape(-1) for m in masks]))
+    want = [[sum(1 << j for j in range(a) if m[i, L - a + j]) for i in range(a)] for m, a, L in zip(masks, n, lens)]
+    assert w._plan["bits"][:, 0].tolist() == sum(want, [])
+    # the same through the attention: what set_tree_masks plans for chains
+    chains = [torch.ones(a, L, dtype=torch.bool).tril(L - a) for a, L in zip(n, lens)]
+    q, k = torch.randn(5, Hq, D, device=DEV), torch.randn(5, Hkv, D, device=DEV)
+    outs = []
+    for plan in (lambda: w.prepareAttention("tree", bp, page, "NONE", torch.float32, torch.cat([m.reshape(-1) for m in chains])),
+                 lambda: w.set_tree_masks(i32(chain(3) + chain(2)), bp, 3)):
+        plan()
+        outs.append(w.computeAttention(q, k, k, pool.cache_data[0], "tree", bp, AttentionRotaryParams(), 0))
+    assert torch.equal(*outs)
+    with pytest.raises(ValueError, match="entries"):
+        w.prepareAttention("tree", bp, page, "NONE", torch.float32, torch.cat([m.reshape(-1) for m in masks])[1:])
+    bp = cache.extend([0, 1], 60)                             # cannot be done: no request has tokens
+    with pytest.raises(ValueError, match="fewer tokens"):
+        w.prepareAttention("tree", bp, page, "NONE", torch.float32, torch.zeros(0, dtype=torch.bool))
+    with pytest.raises(RuntimeError):
+        cache.check()
