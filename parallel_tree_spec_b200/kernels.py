@@ -1043,6 +1043,8 @@ def cache_extend(pool: torch.Tensor, page_refs: torch.Tensor, page_table: torch.
         indptr, indices, last, lens, shared = e(B + 1), e(entries), e(B), e(B), e(G) if G else None
     else:
         indptr, indices, last, lens, shared = out[:5]
+        if G and shared is None:
+            raise ValueError("out needs shared_pages where group_indptr is given")
         _cache_ints("page_indptr", indptr, index, B + 1)
         entries = _cache_ints("page_indices", indices, index)
         _cache_ints("last_page_len", last, index, B)

@@ -237,3 +237,14 @@ def test_replayed_graph_and_another_stream():
         b.o.fork([0, 0, 1, 1], [2, 3, 4, 5]), b.o.extend([2, 3, 4, 5], [9] * 4)
         b.o.truncate([2, 3, 4, 5], [40, 41, 23, 30])
     b.check()
+
+
+def test_extend_refuses_an_output_without_shared_pages():
+    """Groups need a place for their pages; nothing has changed after the refusal."""
+    p = Pair(rows=2, width=3, pages=4, pl=4)
+    out = (i32([0, 0]), i32([0] * 3), i32([0]), i32([0]), None)
+    with pytest.raises(ValueError, match="shared_pages"):
+        K.cache_extend(p.pool, p.refs, p.table, p.lens, i32([0]), 1, group_indptr=i32([0, 1]), out=out)
+    p.check()
+    b = K.cache_extend(p.pool, p.refs, p.table, p.lens, i32([0]), 1, out=out)
+    assert b.status.item() == 0 and b.shared_pages is None
