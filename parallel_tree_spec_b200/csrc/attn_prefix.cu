@@ -1543,11 +1543,12 @@ int launch_prefix(const PrefixParams& p, const PrefixPlan& f, int max_qo_len, cu
     return rc;
   PTS_CUDA_TRY(launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p));
   if (int rc = launch_status("plan_kernel")) return rc;
-  if (D == 128 && f.narrow) {
-    if (int rc = launch_items<D, 3>(p, f, block_map, stream)) return rc;
-  } else if (int rc = launch_items<D, Shape<D>::kSlots>(p, f, block_map, stream)) {
-    return rc;
-  }
+  int rc = PTS_OK;
+  if constexpr (D == 128)
+    rc = f.narrow ? launch_items<D, 3>(p, f, block_map, stream) : launch_items<D, Shape<D>::kSlots>(p, f, block_map, stream);
+  else
+    rc = launch_items<D, Shape<D>::kSlots>(p, f, block_map, stream);
+  if (rc) return rc;
   if (f.few || f.tail_rows)
     if (int rc = f.own_rows == 8 ? launch_own<D, 1, kOwnWarps, false>(p, run_map, stream)
                                  : launch_own<D, 2, kOwnWarps, false>(p, run_map, stream))
