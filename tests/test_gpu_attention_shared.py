@@ -420,3 +420,44 @@ def test_scales_that_are_not_positive(dtype, scale, shared, rows):
     if scale < 0:
         c.q = -q
     check(c, q=q.to(DEV), sm_scale=scale)
+
+
+@pytest.mark.parametrize("rows,Hq,Hkv,pl", [(1, 32, 8, 16), (3, 32, 8, 48), (1, 8, 8, 128), (2, 48, 6, 16)])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_decoding_with_more_own_columns_than_shared(rows, Hq, Hkv, pl, groups):
+    """Few rows, head_dim 128 and a bound of the own columns that says that they are more
+    than the shared ones: the ring of three slots, own columns in slices beside it."""
+    rng = np.random.default_rng(rows + groups)
+    B = 60 // groups
+    gs = [(int(rng.integers(1, 30)), [(int(x), chain(rows)) for x in rng.integers(0, 300, size=B)]) for _ in range(groups)]
+    c = Case(gs, Hq=Hq, Hkv=Hkv, D=128, pl=pl, seed=30 + rows)
+    own = 300 + rows
+    longest = max(c.lens)
+    assert rows * Hq // Hkv <= 16 and B * groups * own >= groups * (longest - own)
+    assert -(-B * groups * Hkv // 148) * (600 + longest) > 3600     # not the one launch of small calls
+    check(c, max_own_len=own)
+
+
+@pytest.mark.parametrize("groups,per_group,rows", [(1, 511, 5), (1, 512, 5), (2, 260, 5), (512, 1, 1), (513, 1, 1), (600, 2, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_plans_of_more_column_sets_than_fit_shared_memory(groups, per_group, rows, D):
+    """512 column sets and more: the groups' shared columns and, for trees, each request's
+    own; from 513 on the plan is made in global memory."""
+    rng = np.random.default_rng(groups + per_group)
+    gs = [(int(rng.integers(0, 12)), [(int(rng.integers(0, 40)), tree(int(rng.integers(100)), 2, 2) if rows == 5 else chain(1))
+                                      for _ in range(per_group)]) for _ in range(groups)]
+    c = Case(gs, Hq=8, Hkv=2, D=D, seed=groups + rows)
+    assert all(len(p) == rows for p in c.parents)
+    assert rows > 4 or -(-len(c.parents) * 2 // 148) * (600 + max(c.lens)) > 3600
+    check(c)
+
+
+@pytest.mark.parametrize("rows,own", [(1, 0), (1, 300), (9, 40), (65, 70)])
+@pytest.mark.parametrize("pl", [112, 128, 192, 256, 1024])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_pages(D, pl, rows, own):
+    """Pages of a block and more: one copy per block, or several where a page's length is no
+    multiple of a block's."""
+    par = chain(rows) if rows < 9 else tree(rows, 8, 8) if rows == 65 else tree(rows, 2, 4)
+    reqs = [(own + i, par) for i in range(40 if rows == 1 else 3)]
+    check(Case([(3, reqs), (0, reqs[:2])], Hq=8 if rows > 1 else 32, Hkv=2 if rows > 1 else 8, D=D, pl=pl, seed=pl + rows))

@@ -618,3 +618,35 @@ def test_boolean_masks_for_a_cache_whose_lengths_are_bounds():
         w.prepareAttention("tree", bp, page, "NONE", torch.float32, torch.zeros(0, dtype=torch.bool))
     with pytest.raises(RuntimeError):
         cache.check()
+
+
+def test_bf16_beam_search_with_a_shared_prefix():
+    """The bf16 search with ``shared_prefix``: every attention of a step that shares pages is
+    what tree_attention gives for the same batch, up to the rounding of the probabilities
+    and of the output (2^-8 of the largest value each, in both calls); the search leaves the
+    pages that the one without it leaves."""
+    from tests.test_gpu_reference_flow import D, HKV, PAGE, V, _patched_model
+    model = _patched_model().to(torch.bfloat16)
+    ids = torch.randint(0, V, (1, 75), generator=torch.Generator().manual_seed(3)).to(DEV)
+    real, pairs, free = K.tree_attention_shared, [], []
+
+    def both(q, kv, qo, pi, px, last, bits, max_qo, max_kv, groups, shared, **kw):
+        got = real(q, kv, qo, pi, px, last, bits, max_qo, max_kv, groups, shared, **kw)
+        want = K.tree_attention(q, kv, qo, pi, px, last, bits, max_qo, max_kv, sm_scale=kw["sm_scale"])
+        pairs.append((shared.item(), (got.double() - want.double()).abs().max().item(), kv[px.long(), 1].abs().max().item()))
+        return got
+
+    for shared in (False, True):
+        pool = KvCachePool(64, 2, HKV, D, PAGE, torch.bfloat16, torch.device(DEV))
+        w = BeFlashinferWrapper(4, HKV, 256, PAGE, torch.device(DEV))
+        K.tree_attention_shared = both
+        try:
+            tree_, _, _ = pbs.beam_search(model, RequestKvCache(pool, PAGE, 0), ids,
+                                          pbs.BeamSearchConfig(topk_len=5, max_depth=6, shared_prefix=shared), w)
+        finally:
+            K.tree_attention_shared = real
+        assert len(tree_.nodes) > 20
+        free.append(pool.num_free_pages())
+        assert bool(pairs) == shared
+    assert all(n == 75 // PAGE and diff <= 2 * (2 * 2.0 ** -8 + 2.0 ** -12) * most for n, diff, most in pairs)
+    assert len(pairs) >= 2 * 5                                # two layers, five steps or more
