@@ -647,8 +647,11 @@ def tree_attention_shared(q: torch.Tensor, kv_layer: torch.Tensor, qo_indptr: to
     es = 2 if q.dtype is torch.bfloat16 else 4
     nbytes = _shared_attn_workspace(index, B, G, T, max_qo, max_kv, own, Hq, Hkv, D, pl, es)
     ws = qo_indptr.new_empty((nbytes + 3) // 4) if nbytes else None
-    stream = _raw_stream(index)
-    err = _error_word(index, stream)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    # (the default stream, 0, is never captured)
+    err = None if stream and torch._C._cuda_isCurrentStreamCapturing() else _ERROR_WORDS.get((index, stream))
+    if err is None:
+        err = _error_word(index, stream)
     _call_on(index, "pts_tree_attn_run_shared", _lib.pack_shared_attn(
         q.data_ptr(), kv_layer.data_ptr(), qo_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
         last_page_len.data_ptr(), bits, group_indptr.data_ptr(), shared_pages.data_ptr(), out.data_ptr(),
@@ -695,8 +698,9 @@ _ERROR_WORDS: Dict[Tuple[int, Optional[int]], torch.Tensor] = {}
 def _error_word(index: int, stream: int) -> Optional[torch.Tensor]:
     """The word for a launch on this stream (None: captured before the device's first
     launch outside of a capture, which makes the captured launches' word)."""
-    if _capturing(index):
-        return _ERROR_WORDS.get((index, None))
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            return _ERROR_WORDS.get((index, None))
     word = _ERROR_WORDS.get((index, stream))
     if word is None:
         dev = torch.device("cuda", index)
@@ -706,13 +710,6 @@ def _error_word(index: int, stream: int) -> Optional[torch.Tensor]:
             _ERROR_WORDS[index, None] = shared
         word = _ERROR_WORDS[index, stream] = torch.zeros(64, dtype=torch.int32, device=dev)
     return word
-
-
-def _capturing(index: int) -> bool:
-    if torch._C._cuda_getDevice() == index:
-        return torch._C._cuda_isCurrentStreamCapturing()
-    with torch.cuda.device(index):
-        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 # PTS_B200_CHECK=1: read the attention kernels' error word after every call
