@@ -576,7 +576,10 @@ int pts_tree_attn_run_any(const void* q, const void* kv_layer, const int32_t* qo
  * max_kv_len and max_own_len (tokens after the shared pages; 0: not known) only
  * choose the schedule.  workspace: pts_tree_attn_shared_workspace_size bytes with the
  * same arguments (0 for small calls of few rows: then it may be NULL), 256-byte aligned,
- * any contents.  error (nullable, zeroed before its first use) receives a code when a CTA gave up waiting; the output is then not
+ * any contents; bf16 with head_dim 64 or 128 takes 1 KB x (head_dim + 2) per KV head for
+ * each 256 rows per KV head and each group and, where a request may have more than 16 rows
+ * per KV head, again for each 256 rows and each request (512 requests of 49 rows, 32 query
+ * and 8 KV heads of 128: 1.4 GB).  error (nullable, zeroed before its first use) receives a code when a CTA gave up waiting; the output is then not
  * valid. */
 size_t pts_tree_attn_shared_workspace_size(int batch, int num_groups, int total_q, int max_qo_len, int max_kv_len,
                                            int max_own_len, int num_qo_heads, int num_kv_heads, int head_dim,

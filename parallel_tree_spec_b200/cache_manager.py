@@ -216,7 +216,14 @@ class SharedKvCache:
     waits for it, so a step can be captured in a CUDA graph, ``compact`` too.  A call that
     cannot be done changes nothing (the batch position of such an ``extend`` has
     empty sequences, so an append to it writes nothing); ``check`` raises for it.  The
-    cache takes all pages of the pool, which must be free, until ``close``."""
+    cache takes all pages of the pool, which must be free, until ``close``.
+
+    The host keeps bounds of the lengths for the attention's schedule: exact for lists (of
+    calls that could be done); device rows raise every sequence's bound and device
+    truncations lower none, so a loop of such calls should ask for ``lengths`` now and then
+    (small calls run in one launch only while their bounds are short).  Tokens after the
+    shared pages are not bounded: decoding is scheduled as by ``tree_attention_shared``
+    without ``max_own_len``."""
 
     def __init__(self, pool: KvCachePool, max_sequences: int, max_pages_per_sequence: int):
         if pool.num_free_pages() != pool.max_pages:

@@ -55,6 +55,8 @@ constexpr int kDirectCost = 3600;          // in tokens' time: the rounds' 3 us 
 // Rows per KV head up to which own_attn_kernel takes the own columns: 64 requests of 8192
 // shared and 300 own tokens take, with it and with work items, 42 and 88 us at 4 rows, 56
 // and 89 at 8, 65 and 92 at 12, 71 and 93 at 16 (114 and 119 with 2048 and 1500 tokens).
+// The two do not cross there: 16 rows are what a warp holds in registers, and own columns of
+// 17 to 128 rows pay for mostly empty tiles.
 constexpr int kFewRows = 16;
 constexpr float kRescale = 8.0f;          // O is rescaled when the row max grows by more than 2^8
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -211,11 +213,14 @@ constexpr int kPlanCache = 512;           // entries that the plan keeps in shar
 // its part, some three blocks, and the part's share of the join.  Over 34 mixed calls (10 to
 // 400 us) the geometric mean was, with 3, 9, 12, 16, 20 and 28: 53.6, 51.9, 51.5, 51.4, 51.4
 // and 52.0 us (others: 46.4, 45.3, 45.1, 45.0, 45.0, 45.3), single calls up to a third less.
+// One constant for shared ranges and own tiles, which would each like another: own columns of
+// 4 and 8 rows as work items (which no call has) took 63 and 76 us with 3, 88 and 89 with 16.
 constexpr int kItemCost = 16;
 
 // The plan.  The launch costs about the larger of all items over the CTAs and of the large
-// items' rounds; the cheapest of up to 32 ranges of ceil(longest / k) blocks is taken.  Bound by the chain of its loads and barriers: 4-6 us,
-// 7-8 from a cold cache, for 64 requests as for 16.
+// items' rounds; the cheapest of up to 32 ranges of ceil(longest / k) blocks is taken.  Bound by the chain
+// of its loads and barriers: 4-6 us with its inputs in L2, from a cold cache 7 for 16
+// requests and 8-9 for 64.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PrefixParams p) {
   __shared__ int sums[64 + 4];                          // [2][32] items, large items; red
   __shared__ Entry cache[kPlanCache];                   // the first entries, as in p.entries
