@@ -248,3 +248,33 @@ def test_extend_refuses_an_output_without_shared_pages():
     p.check()
     b = K.cache_extend(p.pool, p.refs, p.table, p.lens, i32([0]), 1, out=out)
     assert b.status.item() == 0 and b.shared_pages is None
+
+
+def test_failures_are_added_up_in_a_word_of_the_callers():
+    """Every call ORs its status into the word; calls that could be done leave it; a word of
+    another type, size or device is refused."""
+    p = Pair(rows=3, width=3, pages=5, pl=4)                 # 5 and 6 tokens in four pages; 11 and 12 take six
+    word = i32([0])
+    rows = lambda *r: i32(list(r))
+    p.extend([0, 1], [5, 6])
+    K.cache_fork(p.refs, p.table, p.lens, rows(0), rows(2), failures=word)
+    K.cache_truncate(p.refs, p.table, p.lens, 4, rows(2), failures=word)
+    K.cache_extend(p.pool, p.refs, p.table, p.lens, rows(0), 0, failures=word)
+    assert word.item() == 0
+    expect = 0
+    for code, call in ((2, lambda: K.cache_fork(p.refs, p.table, p.lens, rows(0, 1), rows(2, 2), failures=word)),
+                       (8, lambda: K.cache_extend(p.pool, p.refs, p.table, p.lens, rows(0, 1), 6, failures=word).status),
+                       (4, lambda: K.cache_extend(p.pool, p.refs, p.table, p.lens, rows(0), 99, failures=word).status),
+                       (1, lambda: K.cache_truncate(p.refs, p.table, p.lens, 4, rows(7), failures=word)),
+                       (0, lambda: K.cache_truncate(p.refs, p.table, p.lens, 4, rows(2), failures=word))):
+        assert call().item() == code
+        expect |= code
+        assert word.item() == expect
+    p.check()
+    for bad in (i32([0, 0]), torch.zeros(1, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int32)):
+        for call in (lambda: K.cache_fork(p.refs, p.table, p.lens, rows(0), rows(2), failures=bad),
+                     lambda: K.cache_extend(p.pool, p.refs, p.table, p.lens, rows(0), 1, failures=bad),
+                     lambda: K.cache_truncate(p.refs, p.table, p.lens, 4, rows(0), failures=bad)):
+            with pytest.raises(ValueError):
+                call()
+    p.check()
