@@ -461,3 +461,23 @@ def test_long_pages(D, pl, rows, own):
     par = chain(rows) if rows < 9 else tree(rows, 8, 8) if rows == 65 else tree(rows, 2, 4)
     reqs = [(own + i, par) for i in range(40 if rows == 1 else 3)]
     check(Case([(3, reqs), (0, reqs[:2])], Hq=8 if rows > 1 else 32, Hkv=2 if rows > 1 else 8, D=D, pl=pl, seed=pl + rows))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["beams", "decoding", "trees", "nan"])
+def test_pages_past_32_bits(dtype, D, kind):
+    """The pages are the last ones of a layer of more than 2^31 elements."""
+    par = tree(1, 8, 8) if kind in ("trees", "nan") else chain(1)
+    c = Case([(20, [(9, par), (30, chain(1))] * (40 if kind == "decoding" else 2))], Hq=32, Hkv=8, D=D, dtype=dtype, seed=18)
+    if kind == "nan":                                         # the last tree slot, which only its own row saw, holds one
+        L, n = c.lens[0], len(par)
+        c.masks[0][n - 1, L - 1] = False
+        c.kv[c.tables[0][(L - 1) // c.pl], 1, (L - 1) % c.pl] = float("nan")
+    a = c.device()
+    P = 2 ** 31 // (2 * c.pl * 8 * D) + c.kv.shape[0] + 100
+    layer = torch.empty(P, *c.kv.shape[1:], dtype=dtype, device=DEV)
+    assert layer.numel() > 2 ** 31
+    at = P - c.kv.shape[0]
+    layer[at:] = c.kv.to(DEV)
+    check(c, kv_layer=layer, page_indices=a["page_indices"] + at)

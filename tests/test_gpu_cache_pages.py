@@ -278,3 +278,55 @@ def test_failures_are_added_up_in_a_word_of_the_callers():
             with pytest.raises(ValueError):
                 call()
     p.check()
+
+
+def test_the_largest_tables():
+    """2^17 sequences over 2^20 pages, 4096 of them extended and 1024 forked at once."""
+    R, W, P = 1 << 17, 2, 1 << 20
+    p = Pair(rows=R, width=W, pages=P, pl=1, layers=1, heads=1, dim=4, seed=2)
+    rng = np.random.default_rng(6)
+    held = rng.permutation(P)[:R].reshape(R // 2, W).tolist()  # half the sequences hold two scattered pages
+    for r, pages in enumerate(held):
+        p.o.table[2 * r], p.o.lens[2 * r] = list(pages), 2
+        for page in pages:
+            p.o.refs[page] = 1
+    p.table.copy_(torch.tensor(p.o.table, dtype=torch.int32))
+    p.refs.copy_(torch.tensor(p.o.refs, dtype=torch.int32))
+    p.lens.copy_(torch.tensor(p.o.lens, dtype=torch.int32))
+    empty = (2 * rng.permutation(R // 2)[:4096] + 1).tolist()
+    p.extend(empty, rng.integers(0, 3, size=4096).tolist(), groups=[0, 1, 4000, 4096])
+    p.fork((2 * rng.permutation(R // 2)[:1024]).tolist(), rng.permutation(R)[:1024].tolist())
+    p.check()
+    p.truncate(rng.permutation(R)[:20000].tolist(), rng.integers(0, 2, size=20000).tolist())
+    p.compact()
+    p.check()
+
+
+@pytest.mark.parametrize("call", ["extend", "compact"])
+def test_pages_past_4_gb_of_a_layer(call):
+    """Copies between pages whose bytes lie past 32 bits, in both layers."""
+    L, P, pl, H, D = 2, 70000, 16, 8, 128                      # 4.6 GB a layer
+    pool = torch.empty(L, P, 2, pl, H, D, dtype=torch.bfloat16, device=DEV)
+    refs, table, lens = i32([0] * P), torch.full((3, 4), -1, dtype=torch.int32, device=DEV), i32([0] * 3)
+    src = [P - 3, P - 40000, 12]                               # 41 tokens: two pages and nine slots
+    table[0, :3], lens[0], refs[i32(src).long()] = i32(src), 41, 1
+    bits = pool.view(torch.int16)
+    for page in src:
+        bits[:, page] = torch.randint(-2 ** 15, 2 ** 15, (L, 2, pl, H, D), dtype=torch.int16, device=DEV)
+    if call == "extend":
+        last = P - 7
+        table[0, 2], refs[12], refs[last] = last, 0, 1
+        bits[:, last] = bits[:, 12]
+        others = refs == 0                                     # all other pages but one high one belong to someone
+        others[P - 1] = False
+        refs[others] = 1
+        K.cache_fork(refs, table, lens, i32([0]), i32([1]))
+        b = K.cache_extend(pool, refs, table, lens, i32([1]), 1)
+        assert b.status.item() == 0 and table[1].tolist() == [src[0], src[1], P - 1, -1]
+        assert torch.equal(bits[:, P - 1, :, :9], bits[:, last, :, :9])
+    else:
+        want = [bits[:, page].clone() for page in src]
+        r = K.cache_compact(pool, refs, table)
+        assert r.counts.tolist() == [3, 3] and sorted(r.page_table[0, :3].tolist()) == [0, 1, 2]
+        for page, x in zip(r.page_table[0, :3].tolist(), want):
+            assert torch.equal(bits[:, page], x)
